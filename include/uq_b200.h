@@ -17,7 +17,8 @@
  *    fallback.
  *  - Entry points never synchronise the stream unless documented (the E8
  *    calibration reads scalar results back to the host).
- *  - dtype codes: UQ_F32 = 0, UQ_F64 = 1.
+ *  - dtype codes: UQ_F32 = 0, UQ_F64 = 1; the 4-bit weight operators also
+ *    take UQ_BF16 = 2 and UQ_F16 = 3.
  */
 #ifndef UQ_B200_H
 #define UQ_B200_H
@@ -38,7 +39,7 @@ enum uq_status {
     UQ_ERR_TIMEOUT = 5       /* a device wait exceeded its bound */
 };
 
-enum uq_dtype { UQ_F32 = 0, UQ_F64 = 1 };
+enum uq_dtype { UQ_F32 = 0, UQ_F64 = 1, UQ_BF16 = 2, UQ_F16 = 3 };
 
 int uq_version(void);
 const char *uq_status_string(int status);
@@ -364,6 +365,100 @@ int uq_quant_e8_search(const void *W, int w_dtype, int64_t rows, int64_t n0, int
                        const double *H, double step, const double *signs, float *What, int16_t *idx,
                        int32_t *choice, double *lam_host, double *err, void *workspace,
                        size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------
+ * 4-bit weights with group scales (no counterpart in the reference)
+ * ------------------------------------------------------------------- */
+
+/* A weight matrix (N, K) is w[n, k] = s e[n, k / group] q[n, k]: q whole
+ * numbers in -8 .. 7, e one E4M3 value per group of `group` (32, 64, 128 or
+ * 256) values of a row, s one float per matrix.  K is a multiple of group.
+ *   codes   (mats, N, K / 2) bytes, u = q + 8 in 4 bits; the low halves of four
+ *           bytes hold elements 0, 4, 1, 5 of eight, the high halves 2, 6, 3, 7
+ *   scales  (mats, N, K / group) E4M3 bytes
+ *   scale   (mats) floats
+ * e q has at most 8 significant bits, so it is exact in bfloat16 and in
+ * float16; the products below form e q x exactly and add in float32.
+ * All pointers 16-byte aligned. */
+
+/* W (mats, rows, cols), row stride ldw, matrix stride rows * ldw, any dtype
+ * code (converted to float32 first).  s = the least power of two, at least
+ * 2^-117, with max|x| <= 3584 s over the groups whose values are all finite
+ * (1 if that is 0).  Per group: m = the first x of largest |x|; e = m / (-8 s)
+ * rounded to nearest even in E4M3, away from 0 to +-2^-9 if m != 0 would round
+ * to 0; q = x / (s e) rounded to nearest even (exactly), clipped to -8 .. 7.
+ * A group with a non-finite value gets e = NaN, q = 0.  Writes every byte of
+ * codes, scales and scale. */
+int uq_q4_encode(const void *W, int w_dtype, int64_t mats, int64_t rows, int64_t cols, int64_t ldw,
+                 int group, uint8_t *codes, uint8_t *scales, float *scale, void *stream);
+
+/* out (mats, rows, cols) contiguous, UQ_F32, UQ_BF16 or UQ_F16: s e q, one
+ * rounding (none to float32 while nothing underflows). */
+int uq_q4_decode(const uint8_t *codes, const uint8_t *scales, const float *scale, int64_t mats,
+                 int64_t rows, int64_t cols, int group, void *out, int out_dtype, void *stream);
+
+/* Group scales held in float32, c (mats, n) -> the stored form: s = the least
+ * power of two >= 2^-117 with max|c| <= 448 s over the finite values (1 if
+ * that is 0), e = c / s rounded to nearest even in E4M3 (+-2^-9 where c != 0
+ * would round to 0, NaN where c is not finite). */
+int uq_q4_round_scales(const float *c, int64_t mats, int64_t n, uint8_t *scales, float *scale,
+                       void *stream);
+
+/* y[t, n] = sum_k w[n, k] x[t, k].  x (T, K) UQ_BF16 or UQ_F16, row stride
+ * ldx; y (T, N) in x's dtype, row stride ldy.  offsets == NULL: one matrix
+ * (mats = 1) for all rows.  Otherwise offsets are mats + 1 int32 on the device:
+ * rows offsets[i] .. offsets[i + 1] - 1 are multiplied by matrix i; each offset
+ * is taken as at least its predecessors and at most T (a violation is reported
+ * by uq_q4_errors).  Rows outside offsets[0] .. offsets[mats] are set to zero if
+ * zero_rest, else left as they were.  x: 16-byte aligned, ldx a multiple of 8. */
+size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K);
+int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t *codes,
+                 const uint8_t *scales, const float *scale, int64_t mats, int64_t N, int64_t K,
+                 int group, const int32_t *offsets, void *y, int64_t ldy, int zero_rest,
+                 void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradient with respect to x: dx[t, k] = sum_n w[n, k] dy[t, n].  dy (T, N),
+ * row stride lddy (16-byte aligned, lddy a multiple of 8); dx (T, K), row
+ * stride lddx; the rest as above. */
+size_t uq_q4_linear_dx_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K);
+int uq_q4_linear_dx(const void *dy, int dtype, int64_t T, int64_t lddy, const uint8_t *codes,
+                    const uint8_t *scales, const float *scale, int64_t mats, int64_t N, int64_t K,
+                    int group, const int32_t *offsets, void *dx, int64_t lddx, int zero_rest,
+                    void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradient with respect to the effective group scales c = s e:
+ * dc[i, n, j] = sum_{k in group j} q[i, n, k] sum_t dy[t, n] x[t, k] over the
+ * rows t of matrix i; (mats, N, K / group) floats, zero for a matrix without
+ * rows. */
+size_t uq_q4_linear_dscale_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K, int group);
+int uq_q4_linear_dscale(const void *dy, const void *x, int dtype, int64_t T, int64_t lddy, int64_t ldx,
+                        const uint8_t *codes, int64_t mats, int64_t N, int64_t K, int group,
+                        const int32_t *offsets, float *dc, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* out[t, :] = alpha w[tokens[t], :], (T, K) contiguous, UQ_F32, UQ_BF16 or
+ * UQ_F16, one rounding after the float32 factor alpha s e.  tokens: int32, or
+ * int64 when tokens64.  A token outside 0 .. V - 1 gives a row of NaN and is
+ * reported by uq_q4_errors. */
+int uq_q4_embed(const void *tokens, int tokens64, int64_t T, const uint8_t *codes, const uint8_t *scales,
+                const float *scale, int64_t V, int64_t K, int group, float alpha, void *out, int out_dtype,
+                void *stream);
+
+/* Gradient of uq_q4_embed with respect to c = s e: dc[v, j] = alpha
+ * sum_{t: tokens[t] = v} sum_{k in group j} q[v, k] dout[t, k], (V, K / group)
+ * floats, written whole.  dout (T, K), row stride ld, UQ_F32, UQ_BF16 or
+ * UQ_F16.  The rows of a token are added in the order of t, in fixed pieces:
+ * the same call gives the same bits.  Tokens outside 0 .. V - 1 add nothing.
+ * T < 2^30. */
+size_t uq_q4_embed_dscale_workspace_bytes(int64_t T, int64_t V, int64_t K, int group);
+int uq_q4_embed_dscale(const void *tokens, int tokens64, int64_t T, const void *dout, int dtype, int64_t ld,
+                       const uint8_t *codes, int64_t V, int64_t K, int group, float alpha, float *dc,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
+/* Synchronises `stream` and reports (and clears) what the 4-bit operators met
+ * since the last call: a bounded wait that gave up (UQ_ERR_TIMEOUT; outputs
+ * are wrong), a token or an offset out of range (UQ_ERR_INVALID). */
+int uq_q4_errors(void *stream);
 
 /* ---------------------------------------------------------------------
  * Device status (no counterpart in the reference)

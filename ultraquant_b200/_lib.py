@@ -13,12 +13,13 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libuq_b200.so")
 
 UQ_OK, UQ_ERR_INVALID, UQ_ERR_UNSUPPORTED, UQ_ERR_CUDA, UQ_ERR_WORKSPACE, UQ_ERR_TIMEOUT = range(6)
-UQ_F32, UQ_F64 = 0, 1
+UQ_F32, UQ_F64, UQ_BF16, UQ_F16 = range(4)
 
 _p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _u32 = ctypes.c_uint32
+_f32 = ctypes.c_float
 _f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 
@@ -80,6 +81,19 @@ SIGNATURES = {
     "uq_quant_e8": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _f64, _i32, _p, _p, _p, _p, _p, _sz, _p]),
     "uq_quant_e8_b28_workspace_bytes": (_sz, [_i64, _i64]),
     "uq_quant_e8_b28": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _f64, _p, _p, _p, _p, _p, _sz, _p]),
+    "uq_q4_encode": (_i32, [_p, _i32, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _p]),
+    "uq_q4_decode": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p, _i32, _p]),
+    "uq_q4_round_scales": (_i32, [_p, _i64, _i64, _p, _p, _p]),
+    "uq_q4_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "uq_q4_linear": (_i32, [_p, _i32, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i32, _p, _p, _i64, _i32, _p, _sz, _p]),
+    "uq_q4_linear_dx_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
+    "uq_q4_linear_dx": (_i32, [_p, _i32, _i64, _i64, _p, _p, _p, _i64, _i64, _i64, _i32, _p, _p, _i64, _i32, _p, _sz, _p]),
+    "uq_q4_linear_dscale_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "uq_q4_linear_dscale": (_i32, [_p, _p, _i32, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i32, _p, _p, _p, _sz, _p]),
+    "uq_q4_embed": (_i32, [_p, _i32, _i64, _p, _p, _p, _i64, _i64, _i32, _f32, _p, _i32, _p]),
+    "uq_q4_embed_dscale_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "uq_q4_embed_dscale": (_i32, [_p, _i32, _i64, _p, _i32, _i64, _p, _i64, _i64, _i32, _f32, _p, _p, _sz, _p]),
+    "uq_q4_errors": (_i32, [_p]),
     "uq_device_errors": (_i32, [_p]),
     "uq_wait_timeout_selftest": (_i32, [_f64, _p]),
     "uq_inject_device_flag": (_i32, [_i32]),

@@ -1,0 +1,593 @@
+// 4-bit weights with group scales for sm_100a: codec, rounding of trained
+// scales, row lookup and the lookup's gradient with respect to the scales.
+#include "uq_q4.cuh"
+
+#include <algorithm>
+
+namespace {
+
+using namespace uq::q4;
+
+__device__ int g_q4_bad_token;   // a lookup met a token outside its table
+
+// ----------------------------------------------------------------------------
+// Codec
+// ----------------------------------------------------------------------------
+
+// Least power of two s >= 2^-117 with top <= 1.75 2^p s, from the bits of top
+// (finite, >= 0); 1 if top is 0.  1.75 2^11 = 8 x 448: the largest value is -8
+// steps of the largest E4M3 scale.  At s >= 2^-117 the smallest step, 2^-9 s,
+// is a normal number.
+__device__ __forceinline__ float scale_for(uint32_t top, int p) {
+    if (top == 0) return 1.0f;
+    int k = int(top >> 23) - 127 - p + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    k = k < -117 ? -117 : k;
+    return __uint_as_float(uint32_t(k + 127) << 23);
+}
+
+// E4M3 of v, never 0 for v != 0, NaN for a non-finite v.
+__device__ __forceinline__ uint8_t e4m3_of(float v) {
+    if (!(fabsf(v) <= 448.0f)) return 0x7f;
+    const uint8_t b = uint8_t(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
+    return (b & 0x7f) == 0 && v != 0.0f ? uint8_t(b | 1) : b;
+}
+
+template <typename T> __device__ __forceinline__ void load_weights(const T *p, bool vec, float (&x)[8]) {
+    if (vec) {
+        load8(p, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_float(p[i]);
+    }
+}
+
+// Largest |x| (as bits) of the group of 8 * lanes values that `lanes`
+// neighbouring threads hold eight each.
+__device__ __forceinline__ uint32_t group_top(const float (&x)[8], int lanes) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int o = lanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+struct EncArgs {
+    int64_t words, wrow, ldw, per_mat;   // 8-value words: all, per row, (values) row stride, per matrix
+    int group;
+    bool vec;
+};
+
+// top[mat] = max |x| bits over the groups without a non-finite value.
+template <typename T> __global__ void __launch_bounds__(256) q4_top_kernel(const T *W, EncArgs a, uint32_t *top) {
+    const int lanes = a.group / 8;
+    const int64_t step = int64_t(gridDim.x) * 256;
+    for (int64_t base = int64_t(blockIdx.x) * 256; base < a.words; base += step) {
+        const int64_t i = base + threadIdx.x;
+        const bool ok = i < a.words;
+        float x[8] = {};
+        if (ok) load_weights(W + (i / a.wrow) * a.ldw + (i % a.wrow) * 8, a.vec, x);
+        uint32_t m = group_top(x, lanes);
+        if (m >= 0x7f800000u) m = 0;
+        const int64_t mat = ok ? i / a.per_mat : 0, mat0 = base / a.per_mat;
+        const bool same = min(base + 255, a.words - 1) / a.per_mat == mat0;   // one matrix in this block's 256 words
+        if (same) {
+            m = __reduce_max_sync(0xffffffffu, m);
+            if ((threadIdx.x & 31) == 0 && m) atomicMax(top + mat0, m);
+        } else if (ok && m) {
+            atomicMax(top + mat, m);
+        }
+    }
+}
+
+__global__ void q4_scale_kernel(float *scale, int64_t mats, int p) {
+    const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (i < mats) scale[i] = scale_for(__float_as_uint(scale[i]), p);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, const float *scale, uint32_t *codes, uint8_t *scales) {
+    const int lanes = a.group / 8;
+    const int64_t step = int64_t(gridDim.x) * 256;
+    for (int64_t base = int64_t(blockIdx.x) * 256; base < a.words; base += step) {
+        const int64_t i = base + threadIdx.x;
+        const bool ok = i < a.words;
+        float x[8] = {};
+        if (ok) load_weights(W + (i / a.wrow) * a.ldw + (i % a.wrow) * 8, a.vec, x);
+        const uint32_t m = group_top(x, lanes);
+        // the first value of that size: place in the group and sign, the least of (place, sign)
+        const int sub = int(threadIdx.x) & (lanes - 1);
+        uint32_t first = 0xffffffffu;
+#pragma unroll
+        for (int j = 7; j >= 0; --j)
+            if ((__float_as_uint(x[j]) & 0x7fffffffu) == m) first = uint32_t(sub * 8 + j) * 2 + (__float_as_uint(x[j]) >> 31);
+        for (int o = lanes >> 1; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+        if (!ok) continue;   // whole groups: the shuffles above are over
+        const float s = scale[i / a.per_mat];
+        // -m / (8 s): s is a power of two, so the quotient is exact (or underflows, and e4m3_of keeps its sign)
+        const float size = __fdiv_rn(__uint_as_float(m), 8.0f * s);
+        uint8_t e = m >= 0x7f800000u ? uint8_t(0x7f) : e4m3_of(size == 0.0f && m ? 0x1p-20f : size);
+        if (e != 0x7f && m && !(first & 1u)) e |= 0x80;   // a positive m takes a negative scale
+        uint32_t word = 0x88888888u;
+        if (e != 0x7f && m) {
+            const float c = s * e4m3_value(e), rc = __frcp_rn(c), half = 0.5f * fabsf(c);
+            word = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                // q = rint(x / c) exactly: t is within 2^-22 of x / c relatively, so rint(t) is off by at most one and
+                // only next to a border; the remainder x - q c is exact (q c has 8 bits) and decides, ties to even
+                float q = rintf(x[j] * rc);
+                const float r = fmaf(-q, c, x[j]);
+                if (fabsf(r) > half || (fabsf(r) == half && (int(q) & 1))) q += ((r < 0.0f) != (c < 0.0f)) ? -1.0f : 1.0f;
+                const int u = int(fminf(fmaxf(q, -8.0f), 7.0f)) + 8;
+                word |= uint32_t(u) << (4 * ((j >> 1) + 4 * (j & 1)));
+            }
+        }
+        codes[i] = word;
+        if (sub == 0) scales[i / lanes] = e;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) q4_decode_kernel(const uint32_t *codes, const uint8_t *scales, const float *scale, int64_t words,
+                                                        int64_t per_mat, int lshift, T *out) {
+    const int64_t step = int64_t(gridDim.x) * 256;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < words; i += step) {
+        const uint32_t w = __ldg(codes + i);
+        const float c = __ldg(scale + (per_mat == words ? 0 : i / per_mat)) * e4m3_value(__ldg(scales + (i >> lshift)));
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = float(nibble(w, j) - 8) * c;
+        store8(out + i * 8, x);
+    }
+}
+
+__global__ void __launch_bounds__(256) q4_scales_top_kernel(const float *c, int64_t n, uint32_t *top) {
+    uint32_t m = 0;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+        const uint32_t b = __float_as_uint(__ldg(c + int64_t(blockIdx.y) * n + i)) & 0x7fffffffu;
+        if (b < 0x7f800000u) m = max(m, b);
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0 && m) atomicMax(top + blockIdx.y, m);
+}
+
+__global__ void __launch_bounds__(256) q4_round_scales_kernel(const float *c, int64_t n, const float *scale, uint8_t *scales) {
+    const float s = scale[blockIdx.y];
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+        const float v = __ldg(c + int64_t(blockIdx.y) * n + i);
+        const float t = __fdiv_rn(v, s);
+        scales[int64_t(blockIdx.y) * n + i] = e4m3_of(t == 0.0f && v != 0.0f ? copysignf(0x1p-20f, v) : t);
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Lookup
+// ----------------------------------------------------------------------------
+
+template <typename I> __device__ __forceinline__ int64_t token_at(const I *tokens, int64_t t, int64_t V) {
+    const int64_t v = int64_t(__ldg(tokens + t));
+    return v >= 0 && v < V ? v : -1;
+}
+
+template <typename I, typename T>
+__global__ void __launch_bounds__(256) q4_embed_kernel(const I *tokens, int64_t n, const uint32_t *codes, const uint8_t *scales,
+                                                       const float *scale, int64_t V, int wrow, int lshift, float alpha, T *out) {
+    const float f = alpha * __ldg(scale);
+    const int per = wrow >> lshift;
+    for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
+        const int64_t v = token_at(tokens, t, V);
+        if (v < 0 && threadIdx.x == 0) atomicExch(&g_q4_bad_token, 1);
+        for (int i = threadIdx.x; i < wrow; i += 256) {
+            float x[8];
+            if (v >= 0) {
+                const uint32_t w = __ldg(codes + v * wrow + i);
+                const float c = f * e4m3_value(__ldg(scales + v * per + (i >> lshift)));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = float(nibble(w, j) - 8) * c;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = __int_as_float(0x7fc00000);
+            }
+            store8(out + (t * wrow + i) * 8, x);
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Gradient of the lookup: positions sorted by token (stable), then each
+// token's rows added in order
+// ----------------------------------------------------------------------------
+
+constexpr int kTile = 1024, kMaxBits = 9, kMaxBins = 1 << kMaxBits, kMaxChunks = 64;
+
+struct SortPlan {
+    int passes, bits;       // digits of `bits` bits
+    int64_t chunk;          // consecutive entries of one block, a multiple of kTile
+    int chunks;
+};
+
+SortPlan sort_plan(int64_t T, int64_t V) {
+    SortPlan p;
+    int need = 1;
+    while ((int64_t(1) << need) <= V) ++need;   // keys 0 .. V (V: no token)
+    p.passes = (need + kMaxBits - 1) / kMaxBits;
+    p.bits = (need + p.passes - 1) / p.passes;
+    const int64_t tiles = (T + kTile - 1) / kTile;
+    p.chunk = (tiles + kMaxChunks - 1) / kMaxChunks * kTile;
+    p.chunks = int((T + p.chunk - 1) / p.chunk);
+    return p;
+}
+
+struct Keys {
+    const void *tokens;   // first pass: the tokens themselves
+    int tokens64;
+    int64_t V;
+    const uint32_t *keys;
+};
+
+__device__ __forceinline__ uint32_t key_at(const Keys &k, int64_t i) {
+    if (k.keys) return k.keys[i];
+    const int64_t v = k.tokens64 ? token_at(static_cast<const int64_t *>(k.tokens), i, k.V)
+                                 : token_at(static_cast<const int32_t *>(k.tokens), i, k.V);
+    return v < 0 ? uint32_t(k.V) : uint32_t(v);
+}
+
+// hist[bin * chunks + chunk]
+__global__ void __launch_bounds__(kTile) q4_hist_kernel(Keys k, int64_t T, int64_t chunk, int shift, int bits, int *hist) {
+    __shared__ int h[kMaxBins];
+    const int bins = 1 << bits;
+    for (int b = threadIdx.x; b < bins; b += kTile) h[b] = 0;
+    __syncthreads();
+    const int64_t lo = int64_t(blockIdx.x) * chunk, hi = min(lo + chunk, T);
+    for (int64_t i = lo + threadIdx.x; i < hi; i += kTile) atomicAdd(h + ((key_at(k, i) >> shift) & (bins - 1)), 1);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += kTile) hist[b * gridDim.x + blockIdx.x] = h[b];
+}
+
+// Moves each entry to its place: entries of smaller digits, then those of the
+// same digit in earlier chunks, earlier tiles, earlier warps, earlier lanes.
+__global__ void __launch_bounds__(kTile) q4_scatter_kernel(Keys k, const uint32_t *pos_in, int64_t T, int64_t chunk, int shift, int bits,
+                                                           const int *hist, uint32_t *keys_out, uint32_t *pos_out) {
+    __shared__ int start[kMaxBins];
+    __shared__ int wsum[kTile / 32];
+    __shared__ unsigned short count[kTile / 32][kMaxBins];
+    const int bins = 1 << bits, chunks = gridDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int total = 0, before = 0;
+    if (tid < bins) {
+        for (int c = 0; c < chunks; ++c) {
+            const int v = hist[tid * chunks + c];
+            before += c < int(blockIdx.x) ? v : 0;
+            total += v;
+        }
+    }
+    int incl = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 31) wsum[warp] = incl;
+    __syncthreads();
+    int off = 0;
+    for (int w = 0; w < warp; ++w) off += wsum[w];
+    if (tid < bins) start[tid] = off + incl - total + before;
+    const int64_t lo = int64_t(blockIdx.x) * chunk, hi = min(lo + chunk, T);
+    for (int64_t base = lo; base < hi; base += kTile) {
+        for (int b = lane; b < bins; b += 32) count[warp][b] = 0;
+        __syncthreads();
+        const int64_t i = base + tid;
+        const bool ok = i < hi;
+        const uint32_t key = ok ? key_at(k, i) : 0;
+        const uint32_t pos = ok ? (pos_in ? pos_in[i] : uint32_t(i)) : 0;
+        const int digit = ok ? int((key >> shift) & uint32_t(bins - 1)) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, digit);
+        const int rank = __popc(same & ((1u << lane) - 1u));
+        if (ok && rank == 0) count[warp][digit] = (unsigned short)__popc(same);
+        __syncthreads();
+        int sum = 0;
+        if (tid < bins) {
+            for (int w = 0; w < kTile / 32; ++w) {
+                const int v = count[w][tid];
+                count[w][tid] = (unsigned short)sum;
+                sum += v;
+            }
+        }
+        __syncthreads();
+        if (ok) {
+            const int at = start[digit] + count[warp][digit] + rank;
+            keys_out[at] = key;
+            pos_out[at] = pos;
+        }
+        __syncthreads();
+        if (tid < bins) start[tid] += sum;
+    }
+}
+
+__global__ void __launch_bounds__(256) q4_zero_kernel(float *p, int64_t n) {
+    const int64_t v = n / 4, step = int64_t(gridDim.x) * 256;
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < v; i += step) reinterpret_cast<float4 *>(p)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (blockIdx.x == 0 && threadIdx.x < (n & 3)) p[v * 4 + threadIdx.x] = 0.f;
+}
+
+// A block adds the rows of kSeg consecutive sorted entries, 2048 columns.  A
+// token whose entries all lie in the piece is written out; of one that goes
+// on from the piece before (head) or into the next (tail) the piece's part
+// goes to part[piece][head / tail].
+constexpr int kSeg = 32;
+
+template <typename T>
+__global__ void __launch_bounds__(256) q4_segment_kernel(const uint32_t *keys, const uint32_t *pos, int64_t n, const T *dout, int64_t ld,
+                                                         const uint32_t *codes, int64_t V, int wrow, int lshift, float alpha, float *dc,
+                                                         float *part) {
+    __shared__ uint32_t skey[kSeg + 2], spos[kSeg];
+    const int64_t lo = int64_t(blockIdx.x) * kSeg;
+    const int m = int(min(int64_t(kSeg), n - lo));
+    // skey[0]: the key before the piece, skey[m + 1]: the one behind it
+    for (int i = threadIdx.x; i < m + 2; i += 256) {
+        const int64_t j = lo + i - 1;
+        skey[i] = j >= 0 && j < n ? keys[j] : 0xffffffffu;
+    }
+    if (threadIdx.x < m) spos[threadIdx.x] = pos[lo + threadIdx.x];
+    __syncthreads();
+    const int col = blockIdx.y * 256 + threadIdx.x;   // word of the row
+    const bool in = col < wrow;
+    const int lanes = 1 << lshift, per = wrow >> lshift;
+    float acc[8] = {};
+    bool head = skey[0] == skey[1];
+    constexpr int U = 4;
+    for (int b = 0; b < m; b += U) {
+        float d[U][8];
+        uint32_t w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool ok = in && b + u < m && skey[b + u + 1] < uint32_t(V);
+            w[u] = ok ? __ldg(codes + int64_t(skey[b + u + 1]) * wrow + col) : 0;
+            if (ok) {
+                load8(dout + int64_t(spos[b + u]) * ld + col * 8, d[u]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[u][j] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (b + u >= m) break;
+            const uint32_t key = skey[b + u + 1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += d[u][j];
+            const bool last = b + u + 1 == m;
+            if (key >= uint32_t(V) || (!last && skey[b + u + 2] == key)) continue;
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sum = fmaf(float(nibble(w[u], j) - 8), acc[j], sum);
+                acc[j] = 0.f;
+            }
+            for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (in && (threadIdx.x & (lanes - 1)) == 0) {
+                const int g = col >> lshift;
+                const bool tail = last && skey[m + 1] == key;
+                if (head || tail) part[(int64_t(blockIdx.x) * 2 + (head ? 0 : 1)) * per + g] = sum;
+                else dc[int64_t(key) * per + g] = alpha * sum;
+            }
+            head = false;
+        }
+    }
+}
+
+// Adds the parts of each token that crosses pieces, in order.  Block: the
+// piece in which such a token begins (its tail part), then the head parts of
+// the pieces that follow while the token goes on.
+__global__ void __launch_bounds__(256) q4_join_kernel(const uint32_t *keys, int64_t n, int64_t V, int per, float alpha, const float *part, float *dc) {
+    const int64_t pieces = (n + kSeg - 1) / kSeg;
+    const int64_t p = blockIdx.x;
+    if (p + 1 >= pieces) return;
+    const int64_t end = (p + 1) * kSeg;              // first entry of the next piece
+    const uint32_t key = keys[end - 1];
+    if (key >= uint32_t(V) || keys[end] != key) return;                      // nothing goes on from here
+    if (p > 0 && keys[p * kSeg] == key && keys[p * kSeg - 1] == key) return;   // it began earlier
+    // last piece with this key: the first entry beyond p's that differs
+    int64_t lo = p + 1, hi = pieces - 1;             // piece lo begins with the key
+    while (lo < hi) {
+        const int64_t mid = (lo + hi + 1) / 2;
+        if (keys[mid * kSeg] == key) lo = mid; else hi = mid - 1;
+    }
+    for (int g = threadIdx.x; g < per; g += 256) {
+        float sum = part[(p * 2 + 1) * per + g];
+#pragma unroll 8
+        for (int64_t i = p + 1; i <= lo; ++i) sum += part[i * 2 * per + g];
+        dc[int64_t(key) * per + g] = alpha * sum;
+    }
+}
+
+int blocks_for(int64_t work, int per_sm) {
+    return int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(uq::num_sms()) * per_sm)));
+}
+
+template <typename T>
+int encode(const T *W, int64_t mats, int64_t rows, int64_t cols, int64_t ldw, int group, uint8_t *codes, uint8_t *scales, float *scale, cudaStream_t st) {
+    EncArgs a;
+    a.wrow = cols / 8;
+    a.per_mat = rows * a.wrow;
+    a.words = mats * a.per_mat;
+    a.ldw = ldw;
+    a.group = group;
+    a.vec = al16(W) && ldw * int64_t(sizeof(T)) % 16 == 0;
+    if (cudaMemsetAsync(scale, 0, size_t(mats) * 4, st) != cudaSuccess) return uq::check_cuda("uq_q4_encode");
+    const int grid = blocks_for((a.words + 255) / 256, 8);
+    if (a.words) { uq::ProfScope _p("q4_top", st); q4_top_kernel<T><<<grid, 256, 0, st>>>(W, a, reinterpret_cast<uint32_t *>(scale)); }
+    { uq::ProfScope _p("q4_scale", st); q4_scale_kernel<<<unsigned((mats + 255) / 256), 256, 0, st>>>(scale, mats, 11); }
+    if (a.words) { uq::ProfScope _p("q4_encode", st); q4_encode_kernel<T><<<grid, 256, 0, st>>>(W, a, scale, reinterpret_cast<uint32_t *>(codes), scales); }
+    return uq::check_cuda("q4_encode_kernel launch");
+}
+
+bool form_ok(int64_t mats, int64_t rows, int64_t cols, int group) {
+    return mats >= 0 && rows >= 0 && group_ok(group) && cols > 0 && cols % group == 0 && cols < (int64_t(1) << 31) &&
+           (rows == 0 || mats < (int64_t(1) << 48) / rows / cols);
+}
+
+struct Carve {
+    uint32_t *key[2], *pos[2];
+    int *hist;
+    float *part;
+    size_t bytes;
+};
+
+Carve carve(void *ws, size_t cap, int64_t T, const SortPlan &p, int64_t per) {
+    uq::Carver c(ws, cap);
+    Carve r;
+    for (int i = 0; i < 2; ++i) {
+        r.key[i] = c.take<uint32_t>(size_t(T));
+        r.pos[i] = c.take<uint32_t>(size_t(T));
+    }
+    r.hist = c.take<int>(size_t(p.chunks) << p.bits);
+    r.part = c.take<float>(size_t((T + kSeg - 1) / kSeg) * 2 * size_t(per));
+    r.bytes = c.off;
+    return r;
+}
+
+template <typename T>
+void segments(const Carve &c, int last, int64_t n, const void *dout, int64_t ld, const uint8_t *codes, int64_t V, int64_t K, int lshift,
+              float alpha, float *dc, cudaStream_t st) {
+    const int wrow = int(K / 8);
+    const dim3 grid(unsigned((n + kSeg - 1) / kSeg), unsigned((wrow + 255) / 256));
+    { uq::ProfScope _p("q4_segment", st);
+      q4_segment_kernel<T><<<grid, 256, 0, st>>>(c.key[last], c.pos[last], n, static_cast<const T *>(dout), ld,
+                                                reinterpret_cast<const uint32_t *>(codes), V, wrow, lshift, alpha, dc, c.part); }
+    if (grid.x > 1) { uq::ProfScope _p("q4_join", st); q4_join_kernel<<<grid.x - 1, 256, 0, st>>>(c.key[last], n, V, wrow >> lshift, alpha, c.part, dc); }
+}
+
+int lane_shift(int group) { return uq::ilog2(group) - 3; }
+
+}  // namespace
+
+extern "C" {
+
+int uq_q4_encode(const void *W, int w_dtype, int64_t mats, int64_t rows, int64_t cols, int64_t ldw, int group, uint8_t *codes,
+                 uint8_t *scales, float *scale, void *stream) {
+    if (!form_ok(mats, rows, cols, group) || ldw < cols)
+        return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: bad shape (mats=%lld rows=%lld cols=%lld ld=%lld group=%d; cols must be whole groups of 32, 64, 128 or 256)",
+                        (long long)mats, (long long)rows, (long long)cols, (long long)ldw, group);
+    if (mats == 0) return UQ_OK;
+    if (!scale || (rows && (!W || !codes || !scales))) return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: null pointer");
+    if (!al16(codes)) return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: codes not 16-byte aligned");
+    const cudaStream_t st = UQ_STREAM(stream);
+    switch (w_dtype) {
+        case UQ_F32: return encode(static_cast<const float *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
+        case UQ_F64: return encode(static_cast<const double *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
+        case UQ_BF16: return encode(static_cast<const __nv_bfloat16 *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
+        case UQ_F16: return encode(static_cast<const __half *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
+    }
+    return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: unknown dtype code %d", w_dtype);
+}
+
+int uq_q4_decode(const uint8_t *codes, const uint8_t *scales, const float *scale, int64_t mats, int64_t rows, int64_t cols, int group,
+                 void *out, int out_dtype, void *stream) {
+    if (!form_ok(mats, rows, cols, group))
+        return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: bad shape (mats=%lld rows=%lld cols=%lld group=%d)", (long long)mats, (long long)rows, (long long)cols, group);
+    if (mats == 0 || rows == 0) return UQ_OK;
+    if (!codes || !scales || !scale || !out) return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: null pointer");
+    if (!al16(codes) || !al16(out)) return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: codes or out not 16-byte aligned");
+    const int64_t per_mat = rows * cols / 8, words = mats * per_mat;
+    const cudaStream_t st = UQ_STREAM(stream);
+    const int grid = blocks_for((words + 255) / 256, 8), ls = lane_shift(group);
+    const uint32_t *cw = reinterpret_cast<const uint32_t *>(codes);
+    uq::ProfScope _p("q4_decode", st);
+    switch (out_dtype) {
+        case UQ_F32: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, per_mat, ls, static_cast<float *>(out)); break;
+        case UQ_BF16: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, per_mat, ls, static_cast<__nv_bfloat16 *>(out)); break;
+        case UQ_F16: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, per_mat, ls, static_cast<__half *>(out)); break;
+        default: return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: dtype code %d is not built", out_dtype);
+    }
+    return uq::check_cuda("q4_decode_kernel launch");
+}
+
+int uq_q4_round_scales(const float *c, int64_t mats, int64_t n, uint8_t *scales, float *scale, void *stream) {
+    if (mats < 0 || n < 0 || mats > 65535) return uq::fail(UQ_ERR_INVALID, "uq_q4_round_scales: bad shape (mats=%lld n=%lld)", (long long)mats, (long long)n);
+    if (mats == 0) return UQ_OK;
+    if (!scale || (n && (!c || !scales))) return uq::fail(UQ_ERR_INVALID, "uq_q4_round_scales: null pointer");
+    const cudaStream_t st = UQ_STREAM(stream);
+    if (cudaMemsetAsync(scale, 0, size_t(mats) * 4, st) != cudaSuccess) return uq::check_cuda("uq_q4_round_scales");
+    const dim3 grid(unsigned(std::max<int64_t>(1, std::min<int64_t>((n + 1023) / 1024, 1184 / std::min<int64_t>(mats, 1184)))), unsigned(mats));
+    { uq::ProfScope _p("q4_scales_top", st); q4_scales_top_kernel<<<grid, 256, 0, st>>>(c, n, reinterpret_cast<uint32_t *>(scale)); }
+    { uq::ProfScope _p("q4_scale", st); q4_scale_kernel<<<unsigned((mats + 255) / 256), 256, 0, st>>>(scale, mats, 8); }
+    if (n) { uq::ProfScope _p("q4_round_scales", st); q4_round_scales_kernel<<<grid, 256, 0, st>>>(c, n, scale, scales); }
+    return uq::check_cuda("q4_round_scales_kernel launch");
+}
+
+int uq_q4_embed(const void *tokens, int tokens64, int64_t T, const uint8_t *codes, const uint8_t *scales, const float *scale, int64_t V,
+                int64_t K, int group, float alpha, void *out, int out_dtype, void *stream) {
+    if (T < 0 || !form_ok(1, V, K, group))
+        return uq::fail(UQ_ERR_INVALID, "uq_q4_embed: bad shape (T=%lld V=%lld K=%lld group=%d)", (long long)T, (long long)V, (long long)K, group);
+    if (T == 0) return UQ_OK;
+    if (!tokens || !out || !scale || (V && (!codes || !scales))) return uq::fail(UQ_ERR_INVALID, "uq_q4_embed: null pointer");
+    if (!al16(codes) || !al16(out)) return uq::fail(UQ_ERR_INVALID, "uq_q4_embed: codes or out not 16-byte aligned");
+    const cudaStream_t st = UQ_STREAM(stream);
+    const int grid = blocks_for(T, 16), ls = lane_shift(group), wrow = int(K / 8);
+    const uint32_t *cw = reinterpret_cast<const uint32_t *>(codes);
+    uq::ProfScope _p("q4_embed", st);
+#define UQ_EMBED(TY)                                                                                                                     \
+    if (tokens64)                                                                                                                        \
+        q4_embed_kernel<<<grid, 256, 0, st>>>(static_cast<const int64_t *>(tokens), T, cw, scales, scale, V, wrow, ls, alpha, static_cast<TY *>(out)); \
+    else                                                                                                                                 \
+        q4_embed_kernel<<<grid, 256, 0, st>>>(static_cast<const int32_t *>(tokens), T, cw, scales, scale, V, wrow, ls, alpha, static_cast<TY *>(out))
+    switch (out_dtype) {
+        case UQ_F32: UQ_EMBED(float); break;
+        case UQ_BF16: UQ_EMBED(__nv_bfloat16); break;
+        case UQ_F16: UQ_EMBED(__half); break;
+        default: return uq::fail(UQ_ERR_INVALID, "uq_q4_embed: dtype code %d is not built", out_dtype);
+    }
+#undef UQ_EMBED
+    return uq::check_cuda("q4_embed_kernel launch");
+}
+
+size_t uq_q4_embed_dscale_workspace_bytes(int64_t T, int64_t V, int64_t K, int group) {
+    if (T <= 0 || T >= (int64_t(1) << 30) || !form_ok(1, V, K, group) || V >= (int64_t(1) << 31) - 1) return 0;
+    return carve(nullptr, 0, T, sort_plan(T, V), K / group).bytes;
+}
+
+int uq_q4_embed_dscale(const void *tokens, int tokens64, int64_t T, const void *dout, int dtype, int64_t ld, const uint8_t *codes, int64_t V,
+                       int64_t K, int group, float alpha, float *dc, void *workspace, size_t workspace_bytes, void *stream) {
+    if (T < 0 || T >= (int64_t(1) << 30) || !form_ok(1, V, K, group) || V >= (int64_t(1) << 31) - 1 || (T > 1 && ld < K) || K > (int64_t(1) << 26))
+        return uq::fail(UQ_ERR_INVALID, "uq_q4_embed_dscale: bad shape (T=%lld V=%lld K=%lld group=%d ld=%lld)", (long long)T, (long long)V, (long long)K, group, (long long)ld);
+    if (V == 0) return UQ_OK;
+    if (!dc || !codes || (T && (!tokens || !dout))) return uq::fail(UQ_ERR_INVALID, "uq_q4_embed_dscale: null pointer");
+    if (dtype != UQ_F32 && dtype != UQ_BF16 && dtype != UQ_F16) return uq::fail(UQ_ERR_INVALID, "uq_q4_embed_dscale: dtype code %d is not built", dtype);
+    if (!al16(codes) || !al16(dc) || !al16(dout) || ld % 8) return uq::fail(UQ_ERR_INVALID, "uq_q4_embed_dscale: codes, dout and dc have to be 16-byte aligned, ld a multiple of 8");
+    const cudaStream_t st = UQ_STREAM(stream);
+    const int64_t per = K / group;
+    { uq::ProfScope _p("q4_zero", st); q4_zero_kernel<<<blocks_for((V * per + 1023) / 1024, 8), 256, 0, st>>>(dc, V * per); }
+    if (T) {
+        const SortPlan p = sort_plan(T, V);
+        const Carve c = carve(workspace, workspace_bytes, T, p, per);
+        if (!workspace || c.bytes > workspace_bytes)
+            return uq::fail(UQ_ERR_WORKSPACE, "uq_q4_embed_dscale: workspace of %zu bytes, %zu needed", workspace_bytes, c.bytes);
+        for (int i = 0; i < p.passes; ++i) {
+            const Keys k{tokens, tokens64, V, i ? c.key[(i - 1) & 1] : nullptr};
+            { uq::ProfScope _p("q4_hist", st); q4_hist_kernel<<<p.chunks, kTile, 0, st>>>(k, T, p.chunk, i * p.bits, p.bits, c.hist); }
+            { uq::ProfScope _p("q4_scatter", st);
+              q4_scatter_kernel<<<p.chunks, kTile, 0, st>>>(k, i ? c.pos[(i - 1) & 1] : nullptr, T, p.chunk, i * p.bits, p.bits, c.hist, c.key[i & 1], c.pos[i & 1]); }
+        }
+        const int last = (p.passes - 1) & 1, ls = lane_shift(group);
+        switch (dtype) {
+            case UQ_F32: segments<float>(c, last, T, dout, ld, codes, V, K, ls, alpha, dc, st); break;
+            case UQ_BF16: segments<__nv_bfloat16>(c, last, T, dout, ld, codes, V, K, ls, alpha, dc, st); break;
+            default: segments<__half>(c, last, T, dout, ld, codes, V, K, ls, alpha, dc, st); break;
+        }
+    }
+    return uq::check_cuda("q4_segment_kernel launch");
+}
+
+int uq_q4_errors(void *stream) {
+    if (cudaStreamSynchronize(UQ_STREAM(stream)) != cudaSuccess) return uq::check_cuda("uq_q4_errors");
+    int bad = 0, zero = 0, timeout = 0, offset = 0;
+    if (cudaMemcpyFromSymbol(&bad, g_q4_bad_token, sizeof(int)) != cudaSuccess || !mm_take_flags(&timeout, &offset))
+        return uq::check_cuda("read 4-bit operator flags");
+    if (bad && cudaMemcpyToSymbol(g_q4_bad_token, &zero, sizeof(int)) != cudaSuccess) return uq::check_cuda("clear 4-bit operator flags");
+    if (timeout) return uq::fail(UQ_ERR_TIMEOUT, "a bounded device wait of a 4-bit product timed out");
+    if (bad) return uq::fail(UQ_ERR_INVALID, "a token lies outside the table");
+    if (offset) return uq::fail(UQ_ERR_INVALID, "offsets fall, or go beyond the rows");
+    return UQ_OK;
+}
+
+}  // extern "C"
