@@ -1,23 +1,461 @@
 // Products with 4-bit weights for sm_100a: y = x W^T, its gradient with respect
 // to x and to the group scales, for one matrix or one per run of rows.
+//
+// e q has at most 4 + 4 significant bits, so it is a bfloat16 (and a float16)
+// without rounding: the tensor cores multiply it by the activations exactly
+// and add in float32; the matrix's s multiplies the finished sum.
 #include "uq_q4.cuh"
+#include "uq_tc5.cuh"
 
 #include <algorithm>
 
 namespace {
 
 using namespace uq::q4;
+namespace tc5 = uq::tc5;
+namespace tma = uq::tma;
 
-__device__ int g_mm_bad_offset;
+__device__ int g_mm_bad_offset, g_mm_timeout;
 
-struct Mat {
-    const uint8_t *codes, *scales;
-    const float *scale;
-    int64_t N, K;
-    int gshift;
+// ----------------------------------------------------------------------------
+// Tiles: 128 weight columns of the result by up to `bt` rows of one matrix's
+// run, by one of `splits` parts of the contraction.
+// ----------------------------------------------------------------------------
+struct Runs {
+    const int32_t *offsets;   // null: one matrix, all rows
+    int64_t T, mats;
+    int bt;                   // rows of a tile
+    int wtiles, splits;
 };
 
-// Rows [lo, hi) of matrix i: each offset at least its predecessors, at most T.
+struct Tile {
+    int64_t mat, row0;
+    int rows, wt, split;
+};
+
+// Finds a warp's tiles in rising order: the 32 lanes hold 32 matrices' runs at a
+// time.  An offset counts as at least its predecessors and at most T.
+struct Finder {
+    int64_t first, base, lo, hi, incl, top, begin;   // matrices and row tiles before this block of 32; this lane's run
+    bool loaded;
+
+    __device__ __forceinline__ void start(const Runs &r) {
+        first = base = 0;
+        loaded = false;
+        if (r.offsets) {
+            const int64_t o = r.offsets[0];
+            top = min(max(o, int64_t(0)), r.T);
+            if (o != top) g_mm_bad_offset = 1;
+        } else {
+            top = 0;
+        }
+        begin = top;
+    }
+    __device__ __forceinline__ void load(const Runs &r) {
+        const int lane = threadIdx.x & 31;
+        const int64_t i = first + lane;
+        int64_t o = i < r.mats ? int64_t(r.offsets[i + 1]) : 0;
+        int64_t m = i < r.mats ? min(max(o, int64_t(0)), r.T) : 0;
+        m = max(m, top);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, m, d);
+            if (lane >= d) m = max(m, v);
+        }
+        if (i < r.mats && o != m) g_mm_bad_offset = 1;
+        hi = m;
+        lo = __shfl_up_sync(0xffffffffu, m, 1);
+        if (lane == 0) lo = top;
+        incl = (hi - lo + r.bt - 1) / r.bt;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += v;
+        }
+        top = __shfl_sync(0xffffffffu, hi, 31);
+        loaded = true;
+    }
+    // Tile number `t`; false beyond the last.
+    __device__ __forceinline__ bool find(const Runs &r, int64_t t, Tile &tile) {
+        tile.split = int(t % r.splits);
+        const int64_t u = t / r.splits;
+        tile.wt = int(u % r.wtiles);
+        const int64_t rt = u / r.wtiles;
+        if (!r.offsets) {
+            tile.mat = 0;
+            tile.row0 = rt * r.bt;
+            if (tile.row0 >= r.T) return false;
+            tile.rows = int(min(r.T - tile.row0, int64_t(r.bt)));
+            return true;
+        }
+        for (;;) {
+            if (!loaded) {
+                if (first >= r.mats) return false;
+                load(r);
+            }
+            const int64_t all = __shfl_sync(0xffffffffu, incl, 31);
+            if (rt < base + all) break;
+            base += all;
+            first += 32;
+            loaded = false;
+        }
+        const int at = __popc(__ballot_sync(0xffffffffu, base + incl <= rt));   // runs that end before the tile
+        const int64_t before = __shfl_sync(0xffffffffu, incl, at > 0 ? at - 1 : 0);
+        const int64_t l = __shfl_sync(0xffffffffu, lo, at), h = __shfl_sync(0xffffffffu, hi, at);
+        tile.mat = first + at;
+        tile.row0 = l + (rt - base - (at > 0 ? before : 0)) * r.bt;
+        tile.rows = int(min(h - tile.row0, int64_t(r.bt)));
+        return true;
+    }
+    // The end of the last run, once find() has gone beyond the last tile.
+    __device__ __forceinline__ int64_t end(const Runs &r) const { return r.offsets ? top : r.T; }
+};
+
+// ----------------------------------------------------------------------------
+// Weights in 16-bit halves
+// ----------------------------------------------------------------------------
+// The pair (2 i, 2 i + 1) of a word as 16 + u in two halves: u moved to the top
+// bits of the significand of 16.0.  Then e (16 + u) - 24 e = e q in one fused
+// multiply-add: 24 e and e q have at most 8 bits, so nothing rounds.
+template <bool BF16> struct Halves;
+template <> struct Halves<true> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ uint32_t raw(uint32_t w, int i) {
+        const uint32_t v = i == 0 ? w << 3 : w >> (4 * i - 3);
+        return (v & 0x00780078u) | 0x41804180u;
+    }
+    static __device__ __forceinline__ uint32_t pair(float e) {
+        const __nv_bfloat162 p = __float2bfloat162_rn(e);
+        return *reinterpret_cast<const uint32_t *>(&p);
+    }
+    static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+        uint32_t d;
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+        return d;
+    }
+};
+template <> struct Halves<false> {
+    using T = __half;
+    static __device__ __forceinline__ uint32_t raw(uint32_t w, int i) {
+        const uint32_t v = i == 0 ? w << 6 : i == 1 ? w << 2 : w >> (4 * i - 6);
+        return (v & 0x03c003c0u) | 0x4c004c00u;
+    }
+    static __device__ __forceinline__ uint32_t pair(float e) {
+        const __half2 p = __float2half2_rn(e);
+        return *reinterpret_cast<const uint32_t *>(&p);
+    }
+    static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
+        uint32_t d;
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+        return d;
+    }
+};
+
+// 32 codes of one group -> 16 registers of two halves each, in order.
+template <bool BF16> __device__ __forceinline__ void widen32(const uint4 &c, float e, uint32_t *out) {
+    const uint32_t s = Halves<BF16>::pair(e), z = Halves<BF16>::pair(-24.0f * e);
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[4 * j + i] = Halves<BF16>::fma(Halves<BF16>::raw(w[j], i), s, z);
+}
+
+__device__ __forceinline__ uint4 lds128(unsigned addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts128(unsigned addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+struct Weights {
+    const uint8_t *scales;
+    const float *scale;
+    int64_t N, K;
+    int gshift;       // group = 2^gshift
+};
+
+struct Out {
+    void *out;        // (rows, J) of 16 bits, or with splits the workspace: (splits, T, J) floats
+    int64_t ld, J, T;
+    bool zero_rest;
+};
+
+// Register j of lane i: row j, column i of a 32 x 32 piece of the result.
+// Rows [0, rows) and columns below J are written; one row's 32 columns are one
+// line of 64 (or 128) bytes.
+template <bool BF16>
+__device__ __forceinline__ void store_piece(const uint32_t (&r)[32], float s, const Out &o, int split, int splits, int64_t row0, int rows, int64_t col) {
+    using T = typename Halves<BF16>::T;
+    if (col >= o.J) return;
+    if (splits > 1) {
+        float *p = static_cast<float *>(o.out) + (int64_t(split) * o.T + row0) * o.J + col;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < rows) p[int64_t(j) * o.J] = __uint_as_float(r[j]);
+    } else {
+        T *p = static_cast<T *>(o.out) + row0 * o.ld + col;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < rows) p[int64_t(j) * o.ld] = from_float<T>(s * __uint_as_float(r[j]));
+    }
+}
+
+// Rows outside every run, a share of them for each block's eight warps.
+template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int64_t end) {
+    const int64_t rest = o.T - (end - begin);
+    for (int64_t i = blockIdx.x; i < rest; i += gridDim.x) {
+        T *p = static_cast<T *>(o.out) + (i < begin ? i : end + i - begin) * o.ld;
+        for (int64_t j = threadIdx.x; j < o.J; j += 256) p[j] = from_float<T>(0.0f);
+    }
+}
+
+// ----------------------------------------------------------------------------
+// The product kernel.  The result is formed transposed, weight columns in the
+// 128 lanes of tensor memory and up to BT rows in its columns, so that few rows
+// make a narrow instruction.  Stages of 64 contraction steps: `full_b` the rows'
+// tile (TMA, 128-byte swizzle), `full_a` the widened weights, `empty` both free
+// again.
+//   forward: lane n; the weights go from registers into tensor memory (32
+//            columns a stage), codes by TMA in chunks of 256 steps
+//   DX:      lane k; a stage is 64 rows n of 128 codes, widened into shared
+//            memory with k contiguous
+// Warps 0 .. 7 widen (four a stage, in turn) and write results; warp 8 copies
+// the rows, warp 9 the codes, warp 10 issues the products.
+// ----------------------------------------------------------------------------
+constexpr int kThreads = 352;
+
+template <int BT, bool DX> struct Cfg {
+    static constexpr int kStages = BT == 256 ? 4 : BT == 128 ? 6 : 8;
+    static constexpr int kChunks = DX ? (BT == 256 ? 2 : 4) : BT == 256 ? 4 : BT == 128 ? 6 : 8;
+    static constexpr int kStagesDx = BT == 256 ? 4 : BT == 128 ? 5 : 6;
+    static constexpr int NS = DX ? kStagesDx : kStages;
+    static constexpr int kB = BT * 128, kA = DX ? 16384 : 0, kC = 16384;
+    static constexpr int kBar = 3 * NS + 2 * kChunks + 2;
+    static constexpr int kSmem = 1024 + NS * (kB + kA) + kChunks * kC + kBar * 8 + 16;
+    static constexpr int kTmem = 512;
+    static_assert(kSmem <= 232448, "shared memory of one block");
+    static_assert(DX ? BT <= 512 : BT + 32 * NS <= 512, "tensor memory");
+};
+
+template <int BT, bool BF16, bool DX>
+__global__ void __launch_bounds__(kThreads, 1)
+q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_codes, Runs runs, Weights w, Out o) {
+    using C = Cfg<BT, DX>;
+    constexpr int NS = C::NS, NC = C::kChunks, kBox = BT / 4;
+    extern __shared__ uint8_t smem_raw[];
+    const unsigned base = (tc5::smem_addr(smem_raw) + 1023u) & ~1023u;
+    const unsigned sb = base, sa = sb + NS * C::kB, sc = sa + NS * C::kA, bars = sc + NC * C::kC;
+    const unsigned full_b = bars, full_a = bars + 8 * NS, empty = bars + 16 * NS, full_c = bars + 24 * NS, empty_c = full_c + 8 * NC,
+                   done = empty_c + 8 * NC, drained = done + 8, misc = drained + 8;
+    volatile int *gave_up = reinterpret_cast<volatile int *>(smem_raw + (misc + 4 - tc5::smem_addr(smem_raw)));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 10) tc5::tmem_alloc<C::kTmem>(misc);
+    if (threadIdx.x == 0) {
+        *gave_up = 0;
+        for (int i = 0; i < NS; ++i) {
+            tma::mbar_init(full_b + 8 * i, 1);
+            tma::mbar_init(full_a + 8 * i, 4);
+            tma::mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < NC; ++i) {
+            tma::mbar_init(full_c + 8 * i, 1);
+            tma::mbar_init(empty_c + 8 * i, 8);
+        }
+        tma::mbar_init(done, 1);
+        tma::mbar_init(drained, 8);
+        tma::mbar_init(misc + 8, 1);   // products in flight, where a wait gave up
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tc5::fence_before();
+    __syncthreads();
+    tc5::fence_after();
+    unsigned tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(misc));
+    const unsigned tmem_a = tmem + BT;
+
+    tc5::Waiter wt{gave_up, &g_mm_timeout};
+    Finder find;
+    find.start(runs);
+    Tile t;
+    const int64_t depth = DX ? w.N : w.K;
+    const int all = int((depth + 63) / 64);                                       // stages of the whole contraction
+    const int per = runs.splits > 1 ? ((all + 4 * runs.splits - 1) / (4 * runs.splits)) * 4 : all;   // of one part, whole chunks
+    unsigned it = 0, ct = 0, tiles = 0;                                           // stages, chunks, tiles so far
+
+    if (warp == 8) {
+        // rows
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, t); tile += gridDim.x) {
+            const int s0 = t.split * per, n = max(0, min(per, all - s0));
+            const int boxes = (((t.rows + 15) & ~15) + kBox - 1) / kBox;
+            for (int s = 0; s < n; ++s, ++it) {
+                const int slot = it % NS;
+                if (!wt.wait(empty + 8 * slot, ((it / NS) & 1) ^ 1)) break;
+                if (lane == 0) {
+                    tma::mbar_arrive_expect_tx(full_b + 8 * slot, boxes * kBox * 128);
+                    for (int b = 0; b < boxes; ++b)
+                        tma::load2d(sb + slot * C::kB + b * kBox * 128, &map_rows, (s0 + s) * 64, int(t.row0) + b * kBox, full_b + 8 * slot);
+                }
+            }
+        }
+        if (wt.fail)   // copies in flight land before the block ends
+            for (unsigned i = it > NS ? it - NS : 0; i < it; ++i) tc5::Waiter::drain(full_b + 8 * (i % NS), (i / NS) & 1);
+    } else if (warp == 9) {
+        // codes: 128 rows of 256 codes, or 256 rows of 128
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, t); tile += gridDim.x) {
+            const int s0 = t.split * per, n = max(0, min(per, all - s0));
+            for (int s = 0; s < n; s += 4, ++ct) {
+                const int slot = ct % NC;
+                if (!wt.wait(empty_c + 8 * slot, ((ct / NC) & 1) ^ 1)) break;
+                if (lane == 0) {
+                    tma::mbar_arrive_expect_tx(full_c + 8 * slot, C::kC);
+                    const int64_t row = t.mat * w.N;
+                    if (DX) tma::load2d(sc + slot * C::kC, &map_codes, t.wt * 64, int(row + (s0 + s) * 64), full_c + 8 * slot);
+                    else tma::load2d(sc + slot * C::kC, &map_codes, (s0 + s) * 32, int(row + t.wt * 128), full_c + 8 * slot);
+                }
+            }
+        }
+        if (wt.fail)
+            for (unsigned i = ct > NC ? ct - NC : 0; i < ct; ++i) tc5::Waiter::drain(full_c + 8 * (i % NC), (i / NC) & 1);
+    } else if (warp == 10) {
+        // products
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, t); tile += gridDim.x, ++tiles) {
+            const int s0 = t.split * per, n = max(0, min(per, all - s0));
+            const uint32_t idesc = tc5::idesc_f16(BF16, (t.rows + 15) & ~15, DX, false);
+            if (!wt.wait(drained, (tiles & 1) ^ 1)) break;
+            for (int s = 0; s < n; ++s, ++it) {
+                const int slot = it % NS;
+                const unsigned par = (it / NS) & 1;
+                if (!wt.wait(full_b + 8 * slot, par) || !wt.wait(full_a + 8 * slot, par)) break;
+                tc5::fence_after();
+                if (lane == 0) {
+                    const uint64_t b = tc5::desc128(sb + slot * C::kB, 16, 1024);
+                    const uint64_t a = tc5::desc128(sa + slot * C::kA, 8192, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (DX) tc5::mma_ss(tmem, a + k * 128, b + k * 2, idesc, s > 0 || k > 0);
+                        else tc5::mma_ts(tmem, tmem_a + slot * 32 + k * 8, b + k * 2, idesc, s > 0 || k > 0);
+                    }
+                    tc5::commit(empty + 8 * slot);
+                }
+                __syncwarp();
+            }
+            if (!wt.fail && lane == 0) tc5::commit(done);
+            __syncwarp();
+        }
+        if (wt.fail) {   // products in flight end before the block does
+            if (lane == 0) tc5::commit(misc + 8);
+            __syncwarp();
+            tc5::Waiter::drain(misc + 8, 0);
+        }
+    } else {
+        // widen, then write the result
+        const int half = warp >> 2, quad = warp & 3;
+        bool more;
+        for (int64_t tile = blockIdx.x; (more = find.find(runs, tile, t)) && !wt.fail; tile += gridDim.x, ++tiles) {
+            const int s0 = t.split * per, n = max(0, min(per, all - s0));
+            const float scale = __ldg(w.scale + t.mat);
+            // forward: this lane's weight row; DX: this lane's place in a stage
+            const int64_t row = DX ? 0 : int64_t(t.wt) * 128 + quad * 32 + lane;
+            const int64_t groups = w.K >> w.gshift;
+            const uint8_t *erow = w.scales + (t.mat * w.N + (DX ? 0 : min(row, w.N - 1))) * groups;
+            for (int c = 0; c < n; c += 4, ++ct) {
+                const int cslot = ct % NC, cn = min(4, n - c);
+                const unsigned cpar = (ct / NC) & 1;
+                bool seen = false;
+                for (int s = 0; s < cn; ++s, ++it) {
+                    if (int(it & 1) != half) continue;
+                    const int slot = it % NS;
+                    float e[2];
+                    if (DX) {
+                        const int64_t nn = int64_t(s0 + c + s) * 64 + (quad & 1) * 32 + lane, k0 = int64_t(t.wt) * 128 + (quad >> 1) * 64;
+#pragma unroll
+                        for (int p = 0; p < 2; ++p)
+                            e[p] = nn < w.N && k0 + 32 * p < w.K ? e4m3_value(__ldg(erow + nn * groups + ((k0 + 32 * p) >> w.gshift))) : 0.0f;
+                    } else {
+                        const int64_t k0 = int64_t(s0 + c + s) * 64;
+#pragma unroll
+                        for (int p = 0; p < 2; ++p)
+                            e[p] = row < w.N && k0 + 32 * p < w.K ? e4m3_value(__ldg(erow + ((k0 + 32 * p) >> w.gshift))) : 0.0f;
+                    }
+                    if (!seen && !wt.wait(full_c + 8 * cslot, cpar)) break;
+                    seen = true;
+                    if (!wt.wait(empty + 8 * slot, ((it / NS) & 1) ^ 1)) break;
+                    if (DX) {
+                        // row rr of 128 codes (64 bytes, 64-byte swizzle): this warp's 64 values are pieces 2 h, 2 h + 1
+                        const int rr = s * 64 + (quad & 1) * 32 + lane, h = quad >> 1;
+                        const unsigned line = sa + slot * C::kA + h * 8192 + ((quad & 1) * 32 + lane) * 128;
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            uint32_t v[16];
+                            widen32<BF16>(lds128(sc + cslot * C::kC + rr * 64 + (((2 * h + p) ^ ((rr >> 1) & 3)) << 4)), e[p], v);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                sts128(line + (((4 * p + q) ^ (lane & 7)) << 4), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                        }
+                        tma::fence_proxy_async();
+                    } else {
+                        const int rr = quad * 32 + lane;
+                        uint32_t v[32];
+#pragma unroll
+                        for (int p = 0; p < 2; ++p)
+                            widen32<BF16>(lds128(sc + cslot * C::kC + rr * 128 + (((2 * s + p) ^ (rr & 7)) << 4)), e[p], v + 16 * p);
+                        tc5::fence_after();
+                        tc5::st32(tmem_a + slot * 32 + (unsigned(quad * 32) << 16), v);
+                        tc5::wait_st();
+                        tc5::fence_before();
+                    }
+                    __syncwarp();
+                    if (lane == 0) tc5::mbar_arrive(full_a + 8 * slot);
+                }
+                if (wt.fail) break;
+                __syncwarp();
+                if (lane == 0) tc5::mbar_arrive(empty_c + 8 * cslot);
+            }
+            if (!wt.wait(done, tiles & 1)) break;
+            tc5::fence_after();
+            const int64_t col = int64_t(t.wt) * 128 + quad * 32 + lane;
+            for (int c = half; c * 32 < t.rows; c += 2) {
+                uint32_t r[32];
+                tc5::ld32(tmem + c * 32 + (unsigned(quad * 32) << 16), r);
+                tc5::wait_ld();
+                if (n == 0) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) r[j] = 0;
+                }
+                store_piece<BF16>(r, scale, o, t.split, runs.splits, t.row0 + c * 32, t.rows - c * 32, col);
+            }
+            tc5::fence_before();
+            __syncwarp();
+            if (lane == 0) tc5::mbar_arrive(drained);
+        }
+        if (o.zero_rest && runs.offsets && !wt.fail) zero_rows<typename Halves<BF16>::T>(o, find.begin, find.end(runs));
+    }
+    __syncthreads();
+    if (warp == 10) {
+        tc5::fence_after();
+        tc5::tmem_free<C::kTmem>(tmem);
+    }
+}
+
+// The parts of a split contraction, added in their order.
+template <bool BF16>
+__global__ void __launch_bounds__(256) q4_join_parts_kernel(const float *part, int splits, int64_t T, int64_t J, const float *scale, void *out, int64_t ld) {
+    using Ty = typename Halves<BF16>::T;
+    const float s = __ldg(scale);
+    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < T * J; i += int64_t(gridDim.x) * 256) {
+        float v = part[i];
+        for (int p = 1; p < splits; ++p) v += part[int64_t(p) * T * J + i];
+        static_cast<Ty *>(out)[(i / J) * ld + i % J] = from_float<Ty>(s * v);
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Gradient of the group scales (simple form): one block takes 8 weight rows and
+// one group
+// ----------------------------------------------------------------------------
 __device__ void run_of(const int32_t *offsets, int64_t i, int64_t T, int64_t &lo, int64_t &hi) {
     if (!offsets) { lo = 0; hi = T; return; }
     int64_t top = 0;
@@ -32,85 +470,35 @@ __device__ void run_of(const int32_t *offsets, int64_t i, int64_t T, int64_t &lo
     hi = min(max(top, o), T);
 }
 
-__device__ __forceinline__ float weight(const Mat &m, int64_t mat, int64_t n, int64_t k) {
-    const int64_t row = mat * m.N + n;
-    const uint32_t w = reinterpret_cast<const uint32_t *>(m.codes)[(row * m.K + k) >> 3];
-    return float(nibble(w, int(k & 7)) - 8) * e4m3_value(m.scales[(row * m.K + k) >> m.gshift]);
-}
-
-// out[t, j] = scale sum_i a[t, i] w(i, j): forward i = k, j = n; DX i = n, j = k.
-template <typename T, bool DX>
-__global__ void __launch_bounds__(256) q4_product_kernel(const T *a, int64_t lda, int64_t rows, Mat m, const int32_t *offsets, T *out, int64_t ldo) {
-    __shared__ float sa[64][17], sw[64][17];
-    const int64_t mat = blockIdx.z, I = DX ? m.N : m.K, J = DX ? m.K : m.N;
-    int64_t lo, hi;
-    run_of(offsets, mat, rows, lo, hi);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t j0 = int64_t(blockIdx.x) * 64;
-    for (int64_t t0 = lo + int64_t(blockIdx.y) * 64; t0 < hi; t0 += int64_t(gridDim.y) * 64) {
-        float acc[4][4] = {};
-        for (int64_t i0 = 0; i0 < I; i0 += 16) {
-            for (int e = threadIdx.x; e < 1024; e += 256) {
-                const int r = e >> 4, c = e & 15;
-                sa[r][c] = t0 + r < hi && i0 + c < I ? to_float(a[(t0 + r) * lda + i0 + c]) : 0.f;
-                const int64_t j = j0 + r, i = i0 + c;
-                sw[r][c] = j < J && i < I ? (DX ? weight(m, mat, i, j) : weight(m, mat, j, i)) : 0.f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < 16; ++c)
-#pragma unroll
-                for (int p = 0; p < 4; ++p)
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[p][q] = fmaf(sa[ty + 16 * p][c], sw[tx + 16 * q][c], acc[p][q]);
-            __syncthreads();
-        }
-        const float s = m.scale[mat];
-        for (int p = 0; p < 4; ++p)
-            for (int q = 0; q < 4; ++q) {
-                const int64_t t = t0 + ty + 16 * p, j = j0 + tx + 16 * q;
-                if (t < hi && j < J) out[t * ldo + j] = from_float<T>(s * acc[p][q]);
-            }
-    }
-}
-
-template <typename T> __global__ void q4_rest_kernel(const int32_t *offsets, int64_t mats, int64_t rows, int64_t J, T *out, int64_t ldo) {
-    int64_t lo, hi, d;
-    run_of(offsets, 0, rows, lo, d);
-    run_of(offsets, mats - 1, rows, d, hi);
-    for (int64_t t = blockIdx.x; t < rows; t += gridDim.x)
-        if (t < lo || t >= hi)
-            for (int64_t j = threadIdx.x; j < J; j += 256) out[t * ldo + j] = from_float<T>(0.f);
-}
-
-// One block: 8 weight rows x one group.
 template <typename T>
-__global__ void __launch_bounds__(256) q4_dscale_kernel(const T *dy, const T *x, int64_t lddy, int64_t ldx, int64_t rows, Mat m, const int32_t *offsets, float *dc) {
+__global__ void __launch_bounds__(256) q4_dscale_kernel(const T *dy, const T *x, int64_t lddy, int64_t ldx, int64_t rows, const uint8_t *codes, int64_t N,
+                                                        int64_t K, int gshift, const int32_t *offsets, float *dc) {
     const int64_t mat = blockIdx.z, n = int64_t(blockIdx.y) * 8 + (threadIdx.x >> 5), g = blockIdx.x;
     int64_t lo, hi;
     run_of(offsets, mat, rows, lo, hi);
-    if (n >= m.N) return;
+    if (n >= N) return;
     const int lane = threadIdx.x & 31;
-    const int64_t row = mat * m.N + n, per = m.K >> m.gshift;
+    const int64_t row = mat * N + n, per = K >> gshift;
     float sum = 0.f;
-    for (int64_t k = (g << m.gshift) + lane; k < ((g + 1) << m.gshift); k += 32) {
+    for (int64_t k = (g << gshift) + lane; k < ((g + 1) << gshift); k += 32) {
         float d = 0.f;
         for (int64_t t = lo; t < hi; ++t) d = fmaf(to_float(dy[t * lddy + n]), to_float(x[t * ldx + k]), d);
-        const uint32_t w = reinterpret_cast<const uint32_t *>(m.codes)[(row * m.K + k) >> 3];
+        const uint32_t w = reinterpret_cast<const uint32_t *>(codes)[(row * K + k) >> 3];
         sum = fmaf(float(nibble(w, int(k & 7)) - 8), d, sum);
     }
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) dc[row * per + g] = sum;
 }
 
+constexpr int64_t kMost = (int64_t(1) << 31) - 256;
+
 // Arguments that the three products share; `a` and `b`: the row operands (b may
 // be an output without alignment rules) with `na`, `nb` values a row.
 int check_args(const char *what, int dtype, int64_t T, int64_t mats, int64_t N, int64_t K, int group, const int32_t *offsets,
                const uint8_t *codes, const void *a, int64_t lda, int64_t na, const void *b, int64_t ldb, int64_t nb, bool b_read) {
     if (dtype != UQ_BF16 && dtype != UQ_F16) return uq::fail(UQ_ERR_INVALID, "%s: dtype code %d is not built (bfloat16, float16)", what, dtype);
-    constexpr int64_t most = (int64_t(1) << 31) - 256;
     if (T < 0 || mats < 0 || N < 0 || K <= 0 || !group_ok(group) || K % group || (!offsets && mats != 1) || mats > 65535 ||
-        T > most || N > most || K > most)
+        T > kMost || N > kMost || K > kMost || mats * N > kMost)
         return uq::fail(UQ_ERR_INVALID, "%s: bad shape (T=%lld mats=%lld N=%lld K=%lld group=%d)", what, (long long)T, (long long)mats,
                         (long long)N, (long long)K, group);
     if (T == 0 || N == 0 || mats == 0) return UQ_OK;
@@ -123,13 +511,72 @@ int check_args(const char *what, int dtype, int64_t T, int64_t mats, int64_t N, 
     return UQ_OK;
 }
 
-template <bool DX, typename T>
-void product(const void *a, int64_t lda, int64_t rows, Mat m, int64_t mats, const int32_t *offsets, void *out, int64_t ldo, bool zero, cudaStream_t st) {
-    const int64_t J = DX ? m.K : m.N;
-    const dim3 grid(unsigned((J + 63) / 64), unsigned(std::min<int64_t>((rows + 63) / 64, 64)), unsigned(mats));
-    { uq::ProfScope _p(DX ? "q4_dx" : "q4_linear", st);
-      q4_product_kernel<T, DX><<<grid, 256, 0, st>>>(static_cast<const T *>(a), lda, rows, m, offsets, static_cast<T *>(out), ldo); }
-    if (zero && offsets) { uq::ProfScope _p("q4_rest", st); q4_rest_kernel<T><<<148, 256, 0, st>>>(offsets, mats, rows, J, static_cast<T *>(out), ldo); }
+struct Plan {
+    int width;        // BT of the kernel
+    int bt;           // rows of a tile
+    int splits;
+    int64_t tiles;    // at most
+};
+
+// J result columns, `depth` contraction steps.
+Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
+    Plan p;
+    const int64_t each = std::max<int64_t>(1, T / std::max<int64_t>(mats, 1));   // rows a matrix, if even
+    p.width = each <= 64 ? 64 : each <= 128 ? 128 : 256;
+    p.bt = p.width;
+    p.splits = 1;
+    const int64_t wt = (J + 127) / 128;
+    const int64_t rt = runs ? std::min(T, T / p.bt + mats) : (T + p.bt - 1) / p.bt;
+    p.tiles = rt * wt;
+    const int sms = uq::num_sms();
+    if (!runs && p.tiles * 2 <= sms) {
+        const int64_t chunks = (depth + 255) / 256;
+        p.splits = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sms / p.tiles, chunks / 2), 16)));
+        p.tiles *= p.splits;
+    }
+    return p;
+}
+
+template <int BT, bool BF16, bool DX>
+int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, const Runs &r, const Weights &w, const Out &o, int64_t tiles, cudaStream_t st) {
+    using C = Cfg<BT, DX>;
+    CUtensorMap mr, mc;
+    const int64_t depth = DX ? w.N : w.K;
+    if (!tc5::encode2d(&mr, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rows, uint64_t(depth), uint64_t(r.T),
+                       uint64_t(lda) * 2, 64, BT / 4, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !tc5::encode2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, uint64_t(w.K / 2), uint64_t(mats * w.N), uint64_t(w.K / 2), DX ? 64 : 128,
+                       DX ? 256 : 128, DX ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B))
+        return uq::fail(UQ_ERR_CUDA, "tensor map of a 4-bit product");
+    auto kernel = q4_product_kernel<BT, BF16, DX>;
+    if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), C::kSmem) != cudaSuccess) return uq::check_cuda("q4_product_kernel attribute");
+    const int grid = int(std::min<int64_t>(tiles, uq::num_sms()));
+    uq::ProfScope _p(DX ? "q4_dx" : "q4_linear", st);
+    kernel<<<grid, kThreads, C::kSmem, st>>>(mr, mc, r, w, o);
+    return uq::check_cuda("q4_product_kernel launch");
+}
+
+template <bool BF16, bool DX>
+int product(const void *rows, int64_t lda, int64_t T, const uint8_t *codes, const Weights &w, int64_t mats, const int32_t *offsets, void *out,
+            int64_t ldo, bool zero, void *ws, size_t ws_bytes, cudaStream_t st) {
+    const int64_t J = DX ? w.K : w.N, depth = DX ? w.N : w.K;
+    const Plan p = plan_for(T, mats, offsets != nullptr, J, depth);
+    if (p.splits > 1 && (!ws || ws_bytes < size_t(p.splits) * T * J * 4))
+        return uq::fail(UQ_ERR_WORKSPACE, "4-bit product: workspace of %zu bytes, %zu needed", ws_bytes, size_t(p.splits) * T * J * 4);
+    const Runs r{offsets, T, mats, p.bt, int((J + 127) / 128), p.splits};
+    const Out o{p.splits > 1 ? ws : out, ldo, J, T, zero};
+    int rc = p.width == 64    ? launch<64, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st)
+             : p.width == 128 ? launch<128, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st)
+                              : launch<256, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st);
+    if (rc || p.splits == 1) return rc;
+    uq::ProfScope _p("q4_join_parts", st);
+    q4_join_parts_kernel<BF16><<<unsigned(std::min<int64_t>((T * J + 255) / 256, 1184)), 256, 0, st>>>(static_cast<const float *>(ws), p.splits, T, J, w.scale, out, ldo);
+    return uq::check_cuda("q4_join_parts_kernel launch");
+}
+
+size_t product_workspace(int64_t T, int64_t mats, int64_t J, int64_t depth) {
+    if (T <= 0 || mats != 1 || J <= 0 || depth <= 0 || T > kMost || J > kMost || depth > kMost) return 0;
+    const Plan p = plan_for(T, mats, false, J, depth);
+    return p.splits > 1 ? size_t(p.splits) * T * J * 4 : 0;
 }
 
 }  // namespace
@@ -138,16 +585,17 @@ namespace uq {
 namespace q4 {
 bool mm_take_flags(int *timeout, int *offset) {
     const int zero = 0;
-    *timeout = 0;
     return cudaMemcpyFromSymbol(offset, g_mm_bad_offset, sizeof(int)) == cudaSuccess &&
-           (!*offset || cudaMemcpyToSymbol(g_mm_bad_offset, &zero, sizeof(int)) == cudaSuccess);
+           cudaMemcpyFromSymbol(timeout, g_mm_timeout, sizeof(int)) == cudaSuccess &&
+           (!*offset || cudaMemcpyToSymbol(g_mm_bad_offset, &zero, sizeof(int)) == cudaSuccess) &&
+           (!*timeout || cudaMemcpyToSymbol(g_mm_timeout, &zero, sizeof(int)) == cudaSuccess);
 }
 }  // namespace q4
 }  // namespace uq
 
 extern "C" {
 
-size_t uq_q4_linear_workspace_bytes(int64_t, int64_t, int64_t, int64_t) { return 0; }
+size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K) { return product_workspace(T, mats, N, K); }
 
 int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t *codes, const uint8_t *scales, const float *scale,
                  int64_t mats, int64_t N, int64_t K, int group, const int32_t *offsets, void *y, int64_t ldy, int zero_rest,
@@ -155,13 +603,13 @@ int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t
     if (int rc = check_args("uq_q4_linear", dtype, T, mats, N, K, group, offsets, codes, x, ldx, K, y, ldy, N, false)) return rc;
     if (T == 0 || N == 0 || mats == 0) return UQ_OK;
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear: null pointer");
-    const Mat m{codes, scales, scale, N, K, uq::ilog2(group)};
-    if (dtype == UQ_BF16) product<false, __nv_bfloat16>(x, ldx, T, m, mats, offsets, y, ldy, zero_rest, UQ_STREAM(stream));
-    else product<false, __half>(x, ldx, T, m, mats, offsets, y, ldy, zero_rest, UQ_STREAM(stream));
-    return uq::check_cuda("q4_product_kernel launch");
+    const Weights w{scales, scale, N, K, uq::ilog2(group)};
+    const cudaStream_t st = UQ_STREAM(stream);
+    return dtype == UQ_BF16 ? product<true, false>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, workspace, workspace_bytes, st)
+                            : product<false, false>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, workspace, workspace_bytes, st);
 }
 
-size_t uq_q4_linear_dx_workspace_bytes(int64_t, int64_t, int64_t, int64_t) { return 0; }
+size_t uq_q4_linear_dx_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K) { return product_workspace(T, mats, K, N); }
 
 int uq_q4_linear_dx(const void *dy, int dtype, int64_t T, int64_t lddy, const uint8_t *codes, const uint8_t *scales, const float *scale,
                     int64_t mats, int64_t N, int64_t K, int group, const int32_t *offsets, void *dx, int64_t lddx, int zero_rest,
@@ -169,10 +617,10 @@ int uq_q4_linear_dx(const void *dy, int dtype, int64_t T, int64_t lddy, const ui
     if (int rc = check_args("uq_q4_linear_dx", dtype, T, mats, N, K, group, offsets, codes, dy, lddy, N, dx, lddx, K, false)) return rc;
     if (T == 0 || N == 0 || mats == 0) return UQ_OK;
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear_dx: null pointer");
-    const Mat m{codes, scales, scale, N, K, uq::ilog2(group)};
-    if (dtype == UQ_BF16) product<true, __nv_bfloat16>(dy, lddy, T, m, mats, offsets, dx, lddx, zero_rest, UQ_STREAM(stream));
-    else product<true, __half>(dy, lddy, T, m, mats, offsets, dx, lddx, zero_rest, UQ_STREAM(stream));
-    return uq::check_cuda("q4_product_kernel launch");
+    const Weights w{scales, scale, N, K, uq::ilog2(group)};
+    const cudaStream_t st = UQ_STREAM(stream);
+    return dtype == UQ_BF16 ? product<true, true>(dy, lddy, T, codes, w, mats, offsets, dx, lddx, zero_rest, workspace, workspace_bytes, st)
+                            : product<false, true>(dy, lddy, T, codes, w, mats, offsets, dx, lddx, zero_rest, workspace, workspace_bytes, st);
 }
 
 size_t uq_q4_linear_dscale_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int) { return 0; }
@@ -183,14 +631,13 @@ int uq_q4_linear_dscale(const void *dy, const void *x, int dtype, int64_t T, int
     if (int rc = check_args("uq_q4_linear_dscale", dtype, T, mats, N, K, group, offsets, codes, dy, lddy, N, x, ldx, K, true)) return rc;
     if (N == 0 || mats == 0) return UQ_OK;
     if (!dc) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear_dscale: null pointer");
-    const Mat m{codes, nullptr, nullptr, N, K, uq::ilog2(group)};
     const dim3 grid(unsigned(K / group), unsigned((N + 7) / 8), unsigned(mats));
     const cudaStream_t st = UQ_STREAM(stream);
     uq::ProfScope _p("q4_dscale", st);
     if (dtype == UQ_BF16)
-        q4_dscale_kernel<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16 *>(dy), static_cast<const __nv_bfloat16 *>(x), lddy, ldx, T, m, offsets, dc);
+        q4_dscale_kernel<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16 *>(dy), static_cast<const __nv_bfloat16 *>(x), lddy, ldx, T, codes, N, K, uq::ilog2(group), offsets, dc);
     else
-        q4_dscale_kernel<<<grid, 256, 0, st>>>(static_cast<const __half *>(dy), static_cast<const __half *>(x), lddy, ldx, T, m, offsets, dc);
+        q4_dscale_kernel<<<grid, 256, 0, st>>>(static_cast<const __half *>(dy), static_cast<const __half *>(x), lddy, ldx, T, codes, N, K, uq::ilog2(group), offsets, dc);
     return uq::check_cuda("q4_dscale_kernel launch");
 }
 
