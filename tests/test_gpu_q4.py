@@ -486,6 +486,32 @@ def test_refusals():
 
 # ---- together --------------------------------------------------------------------------------------------------
 
+def test_first_calls_of_a_thread():
+    """A thread that has made no CUDA call yet, as autograd's is at its first backward."""
+    import threading
+    w, q, c, wd = make((256, 512), 32, 1)
+    x = acts(300, 512, torch.bfloat16, 1)
+    dy = acts(300, 256, torch.bfloat16, 2)
+    lib = __import__("ultraquant_b200._lib", fromlist=["load"]).load()
+    st = torch.cuda.current_stream().cuda_stream
+    out, dx = torch.empty(300, 256, device="cuda", dtype=torch.bfloat16), torch.empty(300, 512, device="cuda", dtype=torch.bfloat16)
+    dc = torch.empty(256, 16, device="cuda")
+    ptr = (w.codes.data_ptr(), w.scales.data_ptr(), w.scale.data_ptr())
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    tail = (ws.data_ptr(), ws.numel(), st)
+    calls = [lambda: lib.uq_q4_linear(x.data_ptr(), 2, 300, 512, *ptr, 1, 256, 512, 32, None, out.data_ptr(), 256, 0, *tail),
+             lambda: lib.uq_q4_linear_dx(dy.data_ptr(), 2, 300, 256, *ptr, 1, 256, 512, 32, None, dx.data_ptr(), 512, 0, *tail),
+             lambda: lib.uq_q4_linear_dscale(dy.data_ptr(), x.data_ptr(), 2, 300, 256, 512, ptr[0], 1, 256, 512, 32, None, dc.data_ptr(), *tail)]
+    for call in calls:
+        got = []
+        t = threading.Thread(target=lambda: got.append((call(), lib.uq_last_error())))
+        t.start()
+        t.join()
+        assert got[0][0] == 0, got
+    close(out, x.double() @ wd.T, x.double().abs() @ wd.abs().T, 512)
+    close(dx, dy.double() @ wd, dy.double().abs() @ wd.abs(), 256)
+
+
 def test_streams_and_captured_graphs():
     m = q4()
     w, *_ = make((520, 1024), 32, 1)

@@ -228,10 +228,9 @@ template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int
 constexpr int kThreads = 352;
 
 template <int BT, bool DX> struct Cfg {
-    static constexpr int kStages = BT == 256 ? 4 : BT == 128 ? 6 : 8;
-    static constexpr int kChunks = DX ? (BT == 256 ? 2 : 4) : BT == 256 ? 4 : BT == 128 ? 6 : 8;
-    static constexpr int kStagesDx = BT == 256 ? 4 : BT == 128 ? 5 : 6;
-    static constexpr int NS = DX ? kStagesDx : kStages;
+    // stages: an even number, so that each slot is always widened by the same four warps
+    static constexpr int NS = DX ? (BT == 256 ? 4 : 6) : BT == 256 ? 4 : BT == 128 ? 6 : 8;
+    static constexpr int kChunks = DX ? (BT == 64 ? 4 : 2) : BT == 256 ? 4 : BT == 128 ? 6 : 8;
     static constexpr int kB = BT * 128, kA = DX ? 16384 : 0, kC = 16384;
     static constexpr int kBar = 3 * NS + 2 * kChunks + 2;
     static constexpr int kSmem = 1024 + NS * (kB + kA) + kChunks * kC + kBar * 8 + 16;
@@ -453,41 +452,255 @@ __global__ void __launch_bounds__(256) q4_join_parts_kernel(const float *part, i
 }
 
 // ----------------------------------------------------------------------------
-// Gradient of the group scales (simple form): one block takes 8 weight rows and
-// one group
+// Gradient of the group scales: dW = dy^T x over the rows of a matrix, reduced
+// with the codes before it leaves the chip (a 32nd to a 256th of dW is written).
+// One tile: 128 rows n by 256 columns k; both operands come as lines of 64
+// columns, one line per row t, in stages of 64 rows.  The sums of kPromote
+// stages are taken from tensor memory (two accumulators in turn), multiplied by
+// q and added in float32 registers, so that no long sum runs in the tensor core.
+// Warps 0 .. 7 reduce, warp 8 copies, warp 9 issues, warp 10 clears the rows
+// behind the last one of a run (they are another matrix's, and may be NaN).
 // ----------------------------------------------------------------------------
-__device__ void run_of(const int32_t *offsets, int64_t i, int64_t T, int64_t &lo, int64_t &hi) {
-    if (!offsets) { lo = 0; hi = T; return; }
-    int64_t top = 0;
-    for (int64_t j = 0; j <= i; ++j) {
-        const int64_t o = offsets[j];
-        if (o < top || o > T) g_mm_bad_offset = 1;
-        top = min(max(top, o), T);
-    }
-    lo = top;
-    const int64_t o = offsets[i + 1];
-    if (o < top || o > T) g_mm_bad_offset = 1;
-    hi = min(max(top, o), T);
-}
+constexpr int kPromote = 8, kBand = 12;
 
-template <typename T>
-__global__ void __launch_bounds__(256) q4_dscale_kernel(const T *dy, const T *x, int64_t lddy, int64_t ldx, int64_t rows, const uint8_t *codes, int64_t N,
-                                                        int64_t K, int gshift, const int32_t *offsets, float *dc) {
-    const int64_t mat = blockIdx.z, n = int64_t(blockIdx.y) * 8 + (threadIdx.x >> 5), g = blockIdx.x;
-    int64_t lo, hi;
-    run_of(offsets, mat, rows, lo, hi);
-    if (n >= N) return;
-    const int lane = threadIdx.x & 31;
-    const int64_t row = mat * N + n, per = K >> gshift;
-    float sum = 0.f;
-    for (int64_t k = (g << gshift) + lane; k < ((g + 1) << gshift); k += 32) {
-        float d = 0.f;
-        for (int64_t t = lo; t < hi; ++t) d = fmaf(to_float(dy[t * lddy + n]), to_float(x[t * ldx + k]), d);
-        const uint32_t w = reinterpret_cast<const uint32_t *>(codes)[(row * K + k) >> 3];
-        sum = fmaf(float(nibble(w, int(k & 7)) - 8), d, sum);
+struct DsCfg {
+    static constexpr int NS = 4, kA = 16384, kB = 32768, kBar = 3 * NS + 4;
+    static constexpr int kSmem = 1024 + NS * (kA + kB) + kBar * 8 + 32 + 512;
+};
+
+struct DsTile {
+    int64_t mat, lo, rows;
+    int nt, kt;
+};
+
+// Tile number -> matrix, run and place.  Consecutive tiles of a matrix form
+// bands of kBand row tiles, so that the blocks running at one time share both
+// operands' lines in L2.
+struct DsFinder {
+    int64_t at = -1, top = 0, lo = 0;   // runs up to matrix `at` are read
+    __device__ __forceinline__ bool find(const Runs &r, int64_t t, int ntiles, int ktiles, DsTile &d) {
+        const int64_t per = int64_t(ntiles) * ktiles;
+        d.mat = t / per;
+        if (d.mat >= r.mats) return false;
+        if (!r.offsets) {
+            d.lo = 0;
+            d.rows = r.T;
+        } else {
+            const int lane = threadIdx.x & 31;
+            if (at < 0) {
+                const int64_t o = r.offsets[0];
+                top = min(max(o, int64_t(0)), r.T);
+                if (o != top) g_mm_bad_offset = 1;
+            }
+            while (at < d.mat) {   // 32 offsets at a time: their running maximum
+                const int64_t n = min(d.mat - at, int64_t(32)), i = at + 1 + min(int64_t(lane), n - 1);
+                const int64_t o = r.offsets[i + 1];
+                int64_t m = max(min(max(o, int64_t(0)), r.T), top);
+#pragma unroll
+                for (int s = 1; s < 32; s <<= 1) {
+                    const int64_t v = __shfl_up_sync(0xffffffffu, m, s);
+                    if (lane >= s) m = max(m, v);
+                }
+                if (o != m && lane < n) g_mm_bad_offset = 1;
+                lo = n > 1 ? __shfl_sync(0xffffffffu, m, int(n) - 2) : top;
+                top = __shfl_sync(0xffffffffu, m, int(n) - 1);
+                at += n;
+            }
+            d.lo = lo;
+            d.rows = top - lo;
+        }
+        const int64_t u = t - d.mat * per, band = u / (int64_t(kBand) * ktiles), v = u - band * kBand * ktiles;
+        const int high = min(kBand, ntiles - int(band) * kBand);
+        d.nt = int(band) * kBand + int(v % high);
+        d.kt = int(v / high);
+        return true;
     }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) dc[row * per + g] = sum;
+};
+
+template <bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, Runs runs, const uint8_t *codes, int64_t N,
+                 int64_t K, int gshift, int ntiles, int ktiles, float *dc) {
+    using C = DsCfg;
+    constexpr int NS = C::NS;
+    extern __shared__ uint8_t smem_raw[];
+    const unsigned base = (tc5::smem_addr(smem_raw) + 1023u) & ~1023u;
+    const unsigned sa = base, sb = sa + NS * C::kA, bars = sb + NS * C::kB;
+    const unsigned full = bars, fixed = full + 8 * NS, empty = fixed + 8 * NS, done = empty + 8 * NS, drained = done + 16, misc = drained + 16;
+    uint8_t *const misc_ptr = smem_raw + (misc - tc5::smem_addr(smem_raw));
+    volatile int *gave_up = reinterpret_cast<volatile int *>(misc_ptr + 4);
+    const unsigned sums_full = misc + 16, sums_empty = misc + 24;
+    float *const other = reinterpret_cast<float *>(misc_ptr + 32);   // 128 sums of the second half
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == 9) tc5::tmem_alloc<512>(misc);
+    if (threadIdx.x == 0) {
+        *gave_up = 0;
+        for (int i = 0; i < NS; ++i) {
+            tma::mbar_init(full + 8 * i, 1);
+            tma::mbar_init(fixed + 8 * i, 1);
+            tma::mbar_init(empty + 8 * i, 2);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tma::mbar_init(done + 8 * i, 1);
+            tma::mbar_init(drained + 8 * i, 8);
+        }
+        tma::mbar_init(misc + 8, 1);
+        tma::mbar_init(sums_full, 4);
+        tma::mbar_init(sums_empty, 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    tc5::fence_before();
+    __syncthreads();
+    tc5::fence_after();
+    unsigned tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(misc));
+
+    tc5::Waiter wt{gave_up, &g_mm_timeout};
+    DsFinder find;
+    DsTile t;
+    unsigned it = 0, part = 0;   // stages, promoted parts so far
+
+    if (warp == 8) {
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x) {
+            const int n = int((t.rows + 63) / 64);
+            for (int s = 0; s < n; ++s, ++it) {
+                const int slot = it % NS;
+                if (!wt.wait(empty + 8 * slot, ((it / NS) & 1) ^ 1)) break;
+                if (lane == 0) {
+                    tma::mbar_arrive_expect_tx(full + 8 * slot, C::kA + C::kB);
+                    const int row = int(t.lo) + s * 64;
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) tma::load2d(sa + slot * C::kA + c * 8192, &map_dy, t.nt * 128 + c * 64, row, full + 8 * slot);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tma::load2d(sb + slot * C::kB + c * 8192, &map_x, t.kt * 256 + c * 64, row, full + 8 * slot);
+                }
+            }
+        }
+        if (wt.fail)
+            for (unsigned i = it > NS ? it - NS : 0; i < it; ++i) tc5::Waiter::drain(full + 8 * (i % NS), (i / NS) & 1);
+    } else if (warp == 10) {
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x) {
+            const int n = int((t.rows + 63) / 64);
+            for (int s = 0; s < n; ++s, ++it) {   // every stage, so that no phase of `full` goes by unseen
+                const int slot = it % NS, left = int(min(t.rows - int64_t(s) * 64, int64_t(64)));
+                if (!wt.wait(full + 8 * slot, (it / NS) & 1)) break;
+                if (left & 15) {
+                    const int rows = 16 - (left & 15);
+                    for (int i = lane; i < rows * 48; i += 32) {   // 6 blocks of lines, 8 pieces a line
+                        const int l = left + i / 48, b = i % 48;
+                        const unsigned at = b < 16 ? sa + slot * C::kA + (b >> 3) * 8192 : sb + slot * C::kB + ((b - 16) >> 3) * 8192;
+                        sts128(at + l * 128 + (b & 7) * 16, 0, 0, 0, 0);
+                    }
+                    tma::fence_proxy_async();
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    if (left & 15) tc5::mbar_arrive(fixed + 8 * slot);
+                    tc5::mbar_arrive(empty + 8 * slot);
+                }
+            }
+        }
+    } else if (warp == 9) {
+        unsigned parity = 0;   // bit per slot: of its next clearing
+        constexpr uint32_t idesc = tc5::idesc_f16(BF16, 256, true, true);
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x) {
+            const int n = int((t.rows + 63) / 64);
+            for (int s = 0; s < n; ++s, ++it) {
+                const int slot = it % NS;
+                const bool begin = s % kPromote == 0, end = s % kPromote == kPromote - 1 || s + 1 == n;
+                if (begin && !wt.wait(drained + 8 * (part & 1), ((part >> 1) & 1) ^ 1)) break;
+                if (!wt.wait(full + 8 * slot, (it / NS) & 1)) break;
+                const int left = int(min(t.rows - int64_t(s) * 64, int64_t(64)));
+                if (left & 15) {
+                    if (!wt.wait(fixed + 8 * slot, (parity >> slot) & 1)) break;
+                    parity ^= 1u << slot;
+                }
+                tc5::fence_after();
+                if (lane == 0) {
+                    const uint64_t a = tc5::desc128(sa + slot * C::kA, 8192, 1024), b = tc5::desc128(sb + slot * C::kB, 8192, 1024);
+                    const int steps = (left + 15) >> 4;
+                    for (int k = 0; k < steps; ++k) tc5::mma_ss(tmem + (part & 1) * 256, a + k * 128, b + k * 128, idesc, !begin || k > 0);
+                    tc5::commit(empty + 8 * slot);
+                    if (end) tc5::commit(done + 8 * (part & 1));
+                }
+                __syncwarp();
+                part += end;
+            }
+        }
+        if (wt.fail) {
+            if (lane == 0) tc5::commit(misc + 8);
+            __syncwarp();
+            tc5::Waiter::drain(misc + 8, 0);
+        }
+    } else {
+        const int half = warp >> 2, quad = warp & 3;
+        const int64_t groups = K >> gshift;
+        unsigned tiles = 0;
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x, ++tiles) {
+            const int parts = int((t.rows + 64 * kPromote - 1) / (64 * kPromote));
+            const int64_t n = int64_t(t.nt) * 128 + quad * 32 + lane, k0 = int64_t(t.kt) * 256 + half * 128;
+            uint4 code[4];
+            float sum[4] = {};
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                code[p] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+                if (n < N && k0 + 32 * p < K) code[p] = __ldg(reinterpret_cast<const uint4 *>(codes + ((t.mat * N + n) * K + k0 + 32 * p) / 2));
+            }
+            for (int c = 0; c < parts; ++c, ++part) {
+                if (!wt.wait(done + 8 * (part & 1), (part >> 1) & 1)) break;
+                tc5::fence_after();
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    uint32_t r[32];
+                    tc5::ld32(tmem + (part & 1) * 256 + half * 128 + p * 32 + (unsigned(quad * 32) << 16), r);
+                    tc5::wait_ld();
+                    uint32_t w[4] = {code[p].x, code[p].y, code[p].z, code[p].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) asm volatile("" : "+r"(w[i]));   // widened anew each part: 128 kept floats would spill
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        // u under the significand of 2^23: q = (2^23 + u) - (2^23 + 8)
+                        const uint32_t u = (w[i >> 3] >> (4 * (((i & 7) >> 1) + 4 * (i & 1)))) & 15u;
+                        sum[p] = fmaf(__uint_as_float(r[i]), __uint_as_float(0x4b000000u | u) - 8388616.0f, sum[p]);
+                    }
+                }
+                tc5::fence_before();
+                __syncwarp();
+                if (lane == 0) tc5::mbar_arrive(drained + 8 * (part & 1));
+            }
+            if (wt.fail) break;
+            float *const row = dc + (t.mat * N + n) * groups;
+            if (gshift < 8) {
+                const int span = 1 << (gshift - 5);   // pieces of a group
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    if ((p & (span - 1)) || n >= N || k0 + 32 * p >= K) continue;
+                    float v = sum[p];
+                    if (span >= 2) v += sum[p | 1];
+                    if (span == 4) v += sum[2] + sum[3];
+                    row[(k0 + 32 * p) >> gshift] = v;
+                }
+            } else {
+                const float v = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (half) {
+                    if (!wt.wait(sums_empty, (tiles & 1) ^ 1)) break;
+                    other[quad * 32 + lane] = v;
+                    __syncwarp();
+                    if (lane == 0) tc5::mbar_arrive(sums_full);
+                } else {
+                    if (!wt.wait(sums_full, tiles & 1)) break;
+                    if (n < N && k0 < K) row[k0 >> gshift] = v + other[quad * 32 + lane];
+                    __syncwarp();
+                    if (lane == 0) tc5::mbar_arrive(sums_empty);
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (warp == 9) {
+        tc5::fence_after();
+        tc5::tmem_free<512>(tmem);
+    }
 }
 
 constexpr int64_t kMost = (int64_t(1) << 31) - 256;
@@ -541,14 +754,16 @@ template <int BT, bool BF16, bool DX>
 int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, const Runs &r, const Weights &w, const Out &o, int64_t tiles, cudaStream_t st) {
     using C = Cfg<BT, DX>;
     CUtensorMap mr, mc;
+    auto kernel = q4_product_kernel<BT, BF16, DX>;
+    // before the maps: in a thread without a context (autograd's, at its first call) this binds the device's, which the
+    // map encoder needs
+    if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), C::kSmem) != cudaSuccess) return uq::check_cuda("q4_product_kernel attribute");
     const int64_t depth = DX ? w.N : w.K;
     if (!tc5::encode2d(&mr, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rows, uint64_t(depth), uint64_t(r.T),
                        uint64_t(lda) * 2, 64, BT / 4, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc5::encode2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, uint64_t(w.K / 2), uint64_t(mats * w.N), uint64_t(w.K / 2), DX ? 64 : 128,
                        DX ? 256 : 128, DX ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B))
         return uq::fail(UQ_ERR_CUDA, "tensor map of a 4-bit product");
-    auto kernel = q4_product_kernel<BT, BF16, DX>;
-    if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), C::kSmem) != cudaSuccess) return uq::check_cuda("q4_product_kernel attribute");
     const int grid = int(std::min<int64_t>(tiles, uq::num_sms()));
     uq::ProfScope _p(DX ? "q4_dx" : "q4_linear", st);
     kernel<<<grid, kThreads, C::kSmem, st>>>(mr, mc, r, w, o);
@@ -571,6 +786,25 @@ int product(const void *rows, int64_t lda, int64_t T, const uint8_t *codes, cons
     uq::ProfScope _p("q4_join_parts", st);
     q4_join_parts_kernel<BF16><<<unsigned(std::min<int64_t>((T * J + 255) / 256, 1184)), 256, 0, st>>>(static_cast<const float *>(ws), p.splits, T, J, w.scale, out, ldo);
     return uq::check_cuda("q4_join_parts_kernel launch");
+}
+
+template <bool BF16>
+int dscale(const void *dy, const void *x, int64_t T, int64_t lddy, int64_t ldx, const uint8_t *codes, int64_t mats, int64_t N, int64_t K, int group,
+           const int32_t *offsets, float *dc, cudaStream_t st) {
+    const CUtensorMapDataType ty = BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap md, mx;
+    auto kernel = q4_dscale_kernel<BF16>;
+    // before the maps, see launch()
+    if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), DsCfg::kSmem) != cudaSuccess) return uq::check_cuda("q4_dscale_kernel attribute");
+    if (!tc5::encode2d(&md, ty, dy, uint64_t(N), uint64_t(T), uint64_t(lddy) * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !tc5::encode2d(&mx, ty, x, uint64_t(K), uint64_t(T), uint64_t(ldx) * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B))
+        return uq::fail(UQ_ERR_CUDA, "tensor map of the scales' gradient");
+    const Runs r{offsets, T, mats, 0, 0, 1};
+    const int ntiles = int((N + 127) / 128), ktiles = int((K + 255) / 256);
+    const int grid = int(std::min<int64_t>(mats * ntiles * int64_t(ktiles), uq::num_sms()));
+    uq::ProfScope _p("q4_dscale", st);
+    kernel<<<grid, kThreads, DsCfg::kSmem, st>>>(md, mx, r, codes, N, K, uq::ilog2(group), ntiles, ktiles, dc);
+    return uq::check_cuda("q4_dscale_kernel launch");
 }
 
 size_t product_workspace(int64_t T, int64_t mats, int64_t J, int64_t depth) {
@@ -626,19 +860,15 @@ int uq_q4_linear_dx(const void *dy, int dtype, int64_t T, int64_t lddy, const ui
 size_t uq_q4_linear_dscale_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int) { return 0; }
 
 int uq_q4_linear_dscale(const void *dy, const void *x, int dtype, int64_t T, int64_t lddy, int64_t ldx, const uint8_t *codes, int64_t mats,
-                        int64_t N, int64_t K, int group, const int32_t *offsets, float *dc, void *workspace, size_t workspace_bytes,
-                        void *stream) {
+                        int64_t N, int64_t K, int group, const int32_t *offsets, float *dc, void *, size_t, void *stream) {
     if (int rc = check_args("uq_q4_linear_dscale", dtype, T, mats, N, K, group, offsets, codes, dy, lddy, N, x, ldx, K, true)) return rc;
     if (N == 0 || mats == 0) return UQ_OK;
     if (!dc) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear_dscale: null pointer");
-    const dim3 grid(unsigned(K / group), unsigned((N + 7) / 8), unsigned(mats));
     const cudaStream_t st = UQ_STREAM(stream);
-    uq::ProfScope _p("q4_dscale", st);
-    if (dtype == UQ_BF16)
-        q4_dscale_kernel<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16 *>(dy), static_cast<const __nv_bfloat16 *>(x), lddy, ldx, T, codes, N, K, uq::ilog2(group), offsets, dc);
-    else
-        q4_dscale_kernel<<<grid, 256, 0, st>>>(static_cast<const __half *>(dy), static_cast<const __half *>(x), lddy, ldx, T, codes, N, K, uq::ilog2(group), offsets, dc);
-    return uq::check_cuda("q4_dscale_kernel launch");
+    if (T == 0)
+        return cudaMemsetAsync(dc, 0, size_t(mats) * N * (K / group) * 4, st) == cudaSuccess ? UQ_OK : uq::check_cuda("uq_q4_linear_dscale");
+    return dtype == UQ_BF16 ? dscale<true>(dy, x, T, lddy, ldx, codes, mats, N, K, group, offsets, dc, st)
+                            : dscale<false>(dy, x, T, lddy, ldx, codes, mats, N, K, group, offsets, dc, st);
 }
 
 }  // extern "C"
