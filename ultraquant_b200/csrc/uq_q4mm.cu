@@ -177,6 +177,42 @@ struct Weights {
     int gshift;       // group = 2^gshift
 };
 
+// The scale bytes that one lane needs for a chunk of four stages, in one word;
+// 0 (e = 0, so that whatever the codes are the weights are 0) beyond the matrix.
+// Forward: byte j is group j of the chunk's 256 values of weight row `row`.
+// DX: bytes 0, 1 and 2, 3 are the two pieces of 32 values in this lane's row of
+// stages `half` and `half` + 2.
+template <bool DX>
+__device__ __forceinline__ uint64_t chunk_scales(const Weights &w, const uint8_t *e0, int64_t groups, int64_t row, int wt, int stage, int half, int quad) {
+    uint64_t v = 0;
+    if (DX) {
+        const int64_t k0 = int64_t(wt) * 128 + (quad >> 1) * 64;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t n = int64_t(stage + half + 2 * i) * 64 + (quad & 1) * 32 + (threadIdx.x & 31);
+            if (n >= w.N) continue;
+            const uint8_t *p = e0 + n * groups;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (k0 + 32 * j < w.K) v |= uint64_t(__ldg(p + ((k0 + 32 * j) >> w.gshift))) << (16 * i + 8 * j);
+        }
+    } else if (row < w.N) {
+        const int64_t g0 = (int64_t(stage) * 64) >> w.gshift;
+        const int count = 256 >> w.gshift;   // 8, 4, 2 or 1, aligned where rows are whole chunks
+        const uint8_t *p = e0 + g0;
+        if ((w.K & 255) == 0) {
+            if (count == 8) v = __ldg(reinterpret_cast<const unsigned long long *>(p));
+            else if (count == 4) v = __ldg(reinterpret_cast<const unsigned *>(p));
+            else if (count == 2) v = __ldg(reinterpret_cast<const unsigned short *>(p));
+            else v = __ldg(p);
+        } else {
+            for (int j = 0; j < count; ++j)
+                if (g0 + j < groups) v |= uint64_t(__ldg(p + j)) << (8 * j);
+        }
+    }
+    return v;
+}
+
 struct Out {
     void *out;        // (rows, J) of 16 bits, or with splits the workspace: (splits, T, J) floats
     int64_t ld, J, T;
@@ -352,36 +388,28 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     } else {
         // widen, then write the result
         const int half = warp >> 2, quad = warp & 3;
+        const int64_t groups = w.K >> w.gshift;
         bool more;
         for (int64_t tile = blockIdx.x; (more = find.find(runs, tile, t)) && !wt.fail; tile += gridDim.x, ++tiles) {
             const int s0 = t.split * per, n = max(0, min(per, all - s0));
             const float scale = __ldg(w.scale + t.mat);
-            // forward: this lane's weight row; DX: this lane's place in a stage
-            const int64_t row = DX ? 0 : int64_t(t.wt) * 128 + quad * 32 + lane;
-            const int64_t groups = w.K >> w.gshift;
-            const uint8_t *erow = w.scales + (t.mat * w.N + (DX ? 0 : min(row, w.N - 1))) * groups;
+            const int64_t row = int64_t(t.wt) * 128 + quad * 32 + lane;   // forward: this lane's weight row
+            const uint8_t *const e0 = w.scales + (t.mat * w.N + (DX ? 0 : min(row, w.N - 1))) * groups;
+            uint64_t eraw = chunk_scales<DX>(w, e0, groups, row, t.wt, s0, half, quad);
             for (int c = 0; c < n; c += 4, ++ct) {
                 const int cslot = ct % NC, cn = min(4, n - c);
                 const unsigned cpar = (ct / NC) & 1;
+                const uint64_t ecur = eraw;
+                if (c + 4 < n) eraw = chunk_scales<DX>(w, e0, groups, row, t.wt, s0 + c + 4, half, quad);   // a chunk ahead
                 bool seen = false;
-                for (int s = 0; s < cn; ++s, ++it) {
-                    if (int(it & 1) != half) continue;
-                    const int slot = it % NS;
-                    float e[2];
-                    if (DX) {
-                        const int64_t nn = int64_t(s0 + c + s) * 64 + (quad & 1) * 32 + lane, k0 = int64_t(t.wt) * 128 + (quad >> 1) * 64;
-#pragma unroll
-                        for (int p = 0; p < 2; ++p)
-                            e[p] = nn < w.N && k0 + 32 * p < w.K ? e4m3_value(__ldg(erow + nn * groups + ((k0 + 32 * p) >> w.gshift))) : 0.0f;
-                    } else {
-                        const int64_t k0 = int64_t(s0 + c + s) * 64;
-#pragma unroll
-                        for (int p = 0; p < 2; ++p)
-                            e[p] = row < w.N && k0 + 32 * p < w.K ? e4m3_value(__ldg(erow + ((k0 + 32 * p) >> w.gshift))) : 0.0f;
-                    }
+                for (int s = half; s < cn; s += 2) {
+                    const int slot = (it + s) % NS;
                     if (!seen && !wt.wait(full_c + 8 * cslot, cpar)) break;
                     seen = true;
-                    if (!wt.wait(empty + 8 * slot, ((it / NS) & 1) ^ 1)) break;
+                    if (!wt.wait(empty + 8 * slot, (((it + s) / NS) & 1) ^ 1)) break;
+                    float e[2];
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) e[p] = e4m3_value(uint8_t(ecur >> (8 * (DX ? (s & 2) + p : (2 * s + p) >> (w.gshift - 5)))));
                     if (DX) {
                         // row rr of 128 codes (64 bytes, 64-byte swizzle): this warp's 64 values are pieces 2 h, 2 h + 1
                         const int rr = s * 64 + (quad & 1) * 32 + lane, h = quad >> 1;
@@ -410,6 +438,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                     if (lane == 0) tc5::mbar_arrive(full_a + 8 * slot);
                 }
                 if (wt.fail) break;
+                it += cn;
                 __syncwarp();
                 if (lane == 0) tc5::mbar_arrive(empty_c + 8 * cslot);
             }
@@ -437,6 +466,154 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
         tc5::fence_after();
         tc5::tmem_free<C::kTmem>(tmem);
     }
+}
+
+// ----------------------------------------------------------------------------
+// Few rows: bound by reading the codes once.  A block takes 32 weight rows; its
+// eight warps take every eighth step of 256 values of k each and add up in
+// shared memory at the end, so that even a 4096 x 4096 matrix gives every SM
+// 7 warps whose loads are all in flight at once.  The widened codes are operand
+// A of m16n8k16 products straight from registers: the contraction order is free
+// as long as both operands agree, so lane quarter q takes 64 consecutive values
+// of a row (two 16-byte loads) where the instruction says "columns 2 q, 2 q + 1,
+// 2 q + 8, 2 q + 9".  Widening costs the same for 1 row as for 8.
+// ----------------------------------------------------------------------------
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool bf16) {
+    if (bf16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+constexpr int kFewWarps = 8, kFewRows = 32;
+
+// One lane's codes and scales of a step: 4 rows (g, g + 8, g + 16, g + 24) of 64 values.
+struct Step {
+    uint4 c[4][2];
+    uint32_t e;        // two rows' bytes; see load_step
+    uint32_t e2;
+};
+
+__device__ __forceinline__ void load_step(Step &st, const uint8_t *codes, const Weights &w, int64_t mrow, int64_t n0, int64_t k, int64_t groups) {
+    const int g = (threadIdx.x & 31) >> 2;
+    st.e = st.e2 = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t n = n0 + g + 8 * i;
+        const uint8_t *c = codes + ((mrow + n) * w.K + k) / 2;
+        const uint8_t *e = w.scales + (mrow + n) * groups;
+        uint32_t eb = 0;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const bool in = n < w.N && k + 32 * p < w.K;
+            st.c[i][p] = in ? __ldg(reinterpret_cast<const uint4 *>(c) + p) : make_uint4(0, 0, 0, 0);
+            eb |= in ? uint32_t(__ldg(e + ((k + 32 * p) >> w.gshift))) << (8 * p) : 0u;
+        }
+        if (i < 2) st.e |= eb << (16 * i);
+        else st.e2 |= eb << (16 * (i - 2));
+    }
+}
+
+template <bool BF16, int NT>
+__global__ void __launch_bounds__(256, 2)
+q4_few_kernel(const void *x, int64_t ldx, const uint8_t *codes, Runs runs, Weights w, Out o, int section) {
+    using T = typename Halves<BF16>::T;
+    extern __shared__ __align__(16) uint8_t few_smem[];   // the rows of a section of k, then the warps' sums
+    const unsigned sx = tc5::smem_addr(few_smem);
+    float *const sums = reinterpret_cast<float *>(few_smem);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane & 3, tok = lane >> 2;
+    const int64_t groups = w.K >> w.gshift;
+    Finder find;
+    find.start(runs);
+    Tile t;
+    for (int64_t tile = blockIdx.x; find.find(runs, tile, t); tile += gridDim.x) {
+        const int64_t n0 = int64_t(t.wt) * kFewRows, mrow = t.mat * w.N;
+        float acc[2][NT][4] = {};
+        for (int64_t sec = 0; sec < w.K; sec += section) {
+            const int len = int(min(w.K - sec, int64_t(section))), steps = (len + 255) >> 8;
+            Step cur;
+            int s = warp;
+            if (s < steps) load_step(cur, codes, w, mrow, n0, sec + s * 256 + q * 64, groups);
+            // rows into shared memory: 64 values a line, its eight pieces swizzled by the line's place in a step and the row
+            __syncthreads();
+            const int pieces = steps * 32;
+            for (int r = 0; r < t.rows; ++r) {
+                const T *src = static_cast<const T *>(x) + (t.row0 + r) * ldx + sec;
+                for (int p = tid; p < pieces; p += 256) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (p * 8 < len) v = __ldg(reinterpret_cast<const uint4 *>(src + p * 8));
+                    const int line = p >> 3, sw = (line & 3) | ((r & 1) << 2);
+                    sts128(sx + ((r * steps * 4 + line) * 8 + ((p & 7) ^ sw)) * 16, v.x, v.y, v.z, v.w);
+                }
+            }
+            __syncthreads();
+            for (; s < steps; s += kFewWarps) {
+                Step next;
+                if (s + kFewWarps < steps) load_step(next, codes, w, mrow, n0, sec + (s + kFewWarps) * 256 + q * 64, groups);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    uint32_t es[4], ez[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e = e4m3_value(uint8_t((i < 2 ? cur.e : cur.e2) >> (16 * (i & 1) + 8 * p)));
+                        es[i] = Halves<BF16>::pair(e);
+                        ez[i] = Halves<BF16>::pair(-24.0f * e);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 b[NT];
+#pragma unroll
+                        for (int u = 0; u < NT; ++u) {
+                            const int r = tok + 8 * u, sw = q | ((r & 1) << 2);
+                            b[u] = make_uint4(0, 0, 0, 0);
+                            if (r < t.rows) b[u] = lds128(sx + ((r * steps * 4 + s * 4 + q) * 8 + ((4 * p + j) ^ sw)) * 16);
+                        }
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            uint32_t lo[4], hi[4];
+                            const uint4 &c0 = cur.c[2 * m][p], &c1 = cur.c[2 * m + 1][p];
+                            const uint32_t w0 = j == 0 ? c0.x : j == 1 ? c0.y : j == 2 ? c0.z : c0.w;
+                            const uint32_t w1 = j == 0 ? c1.x : j == 1 ? c1.y : j == 2 ? c1.z : c1.w;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                lo[i] = Halves<BF16>::fma(Halves<BF16>::raw(w0, i), es[2 * m], ez[2 * m]);
+                                hi[i] = Halves<BF16>::fma(Halves<BF16>::raw(w1, i), es[2 * m + 1], ez[2 * m + 1]);
+                            }
+                            const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+#pragma unroll
+                            for (int u = 0; u < NT; ++u) {
+                                mma16816(acc[m][u], a0, b[u].x, b[u].y, BF16);
+                                mma16816(acc[m][u], a1, b[u].z, b[u].w, BF16);
+                            }
+                        }
+                    }
+                }
+                cur = next;
+            }
+        }
+        __syncthreads();
+        // sums[warp][row of x][weight row]
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int u = 0; u < NT; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sums[(warp * 8 * NT + 8 * u + 2 * q + (i & 1)) * kFewRows + 16 * m + tok + 8 * (i >> 1)] = acc[m][u][i];
+        __syncthreads();
+        const float scale = __ldg(w.scale + t.mat);
+        for (int i = tid; i < 8 * NT * kFewRows; i += 256) {
+            const int r = i / kFewRows, c = i % kFewRows;
+            float v = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kFewWarps; ++k) v += sums[(k * 8 * NT + r) * kFewRows + c];
+            if (r < t.rows && n0 + c < w.N) static_cast<T *>(o.out)[(t.row0 + r) * o.ld + n0 + c] = from_float<T>(scale * v);
+        }
+        __syncthreads();
+    }
+    if (o.zero_rest && runs.offsets) zero_rows<T>(o, find.begin, find.end(runs));
 }
 
 // The parts of a split contraction, added in their order.
@@ -770,6 +947,26 @@ int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, co
     return uq::check_cuda("q4_product_kernel launch");
 }
 
+// Rows (for several matrices, rows each if even) up to which the kernel for few
+// rows is taken.
+constexpr int64_t kFewMost = 16;
+
+template <bool BF16, int NT>
+int few(const void *x, int64_t ldx, int64_t T, const uint8_t *codes, const Weights &w, int64_t mats, const int32_t *offsets, void *y, int64_t ldy, bool zero,
+        cudaStream_t st) {
+    auto kernel = q4_few_kernel<BF16, NT>;
+    const int64_t rows = std::min<int64_t>(T, 8 * NT), wide = (w.K + 255) / 256 * 256;
+    const int section = int(std::min<int64_t>(wide, 98304 / (2 * rows) / 256 * 256));
+    const int smem = int(std::max<int64_t>(rows * section * 2, kFewWarps * 8 * NT * kFewRows * 4));
+    if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), 98304) != cudaSuccess) return uq::check_cuda("q4_few_kernel attribute");
+    const Runs r{offsets, T, mats, 8 * NT, int((w.N + kFewRows - 1) / kFewRows), 1};
+    const Out o{y, ldy, w.N, T, zero};
+    const int64_t tiles = (offsets ? std::min(T, T / (8 * NT) + mats) : 1) * r.wtiles;
+    uq::ProfScope _p("q4_few", st);
+    kernel<<<unsigned(std::min<int64_t>(tiles, offsets ? int64_t(uq::num_sms()) * 2 : int64_t(1) << 30)), 256, smem, st>>>(x, ldx, codes, r, w, o, section);
+    return uq::check_cuda("q4_few_kernel launch");
+}
+
 template <bool BF16, bool DX>
 int product(const void *rows, int64_t lda, int64_t T, const uint8_t *codes, const Weights &w, int64_t mats, const int32_t *offsets, void *out,
             int64_t ldo, bool zero, void *ws, size_t ws_bytes, cudaStream_t st) {
@@ -829,7 +1026,7 @@ bool mm_take_flags(int *timeout, int *offset) {
 
 extern "C" {
 
-size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K) { return product_workspace(T, mats, N, K); }
+size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K) { return T <= kFewMost ? 0 : product_workspace(T, mats, N, K); }
 
 int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t *codes, const uint8_t *scales, const float *scale,
                  int64_t mats, int64_t N, int64_t K, int group, const int32_t *offsets, void *y, int64_t ldy, int zero_rest,
@@ -839,6 +1036,13 @@ int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear: null pointer");
     const Weights w{scales, scale, N, K, uq::ilog2(group)};
     const cudaStream_t st = UQ_STREAM(stream);
+    if (T <= kFewMost * mats) {
+        if (T <= 8 * mats)
+            return dtype == UQ_BF16 ? few<true, 1>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st)
+                                    : few<false, 1>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st);
+        return dtype == UQ_BF16 ? few<true, 2>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st)
+                                : few<false, 2>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st);
+    }
     return dtype == UQ_BF16 ? product<true, false>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, workspace, workspace_bytes, st)
                             : product<false, false>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, workspace, workspace_bytes, st);
 }

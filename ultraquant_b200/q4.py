@@ -21,6 +21,8 @@ kernels met on the device (a token or offset out of range).  The reference has n
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _device as D
@@ -40,7 +42,7 @@ class Q4:
     with no leading dimension or one (experts).  Contiguous CUDA tensors of one device; the byte order of the codes is
     include/uq_b200.h's."""
 
-    __slots__ = ("codes", "scales", "scale", "mats", "rows", "cols", "group", "device")
+    __slots__ = ("codes", "scales", "scale", "mats", "rows", "cols", "group", "device", "ptrs", "form")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, scale: torch.Tensor):
         cs, ss = codes.shape, scales.shape
@@ -60,7 +62,10 @@ class Q4:
         if codes.data_ptr() & 15 or scales.data_ptr() & 15:
             raise ValueError("Q4: codes and scales have to start on a 16-byte boundary")
         self.codes, self.scales, self.scale = codes, scales, scale
-        self.mats, self.rows, self.cols, self.group, self.device = (cs[0] if len(cs) == 3 else 1), cs[-2], cols, group, codes.device
+        mats = cs[0] if len(cs) == 3 else 1
+        self.mats, self.rows, self.cols, self.group, self.device = mats, cs[-2], cols, group, codes.device
+        self.ptrs = (codes.data_ptr(), scales.data_ptr(), scale.data_ptr())
+        self.form = (mats, cs[-2], cols, group)
 
     @property
     def shape(self):
@@ -101,9 +106,8 @@ def enc_q4(W, group: int = 32) -> Q4:
     codes = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=dev)
     scales = torch.empty((*lead, rows, cols // group), dtype=torch.float8_e4m3fn, device=dev)
     scale = torch.empty(tuple(lead), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().uq_q4_encode(w.data_ptr(), _CODE[w.dtype], mats, rows, cols, cols, group, codes.data_ptr(),
-                                            scales.data_ptr(), scale.data_ptr(), D.stream_handle(dev)), "enc_q4")
+    _run(dev, _lib.load().uq_q4_encode, "enc_q4", w.data_ptr(), _CODE[w.dtype], mats, rows, cols, cols, group, codes.data_ptr(),
+         scales.data_ptr(), scale.data_ptr())
     return Q4(codes, scales, scale)
 
 
@@ -112,10 +116,7 @@ def deq_q4(w: Q4, dtype=torch.float32) -> torch.Tensor:
     if dtype not in _OUT:
         raise TypeError(f"deq_q4: dtype {dtype} is not built (float32, bfloat16, float16)")
     out = torch.empty(w.shape, dtype=dtype, device=w.device)
-    with torch.cuda.device(w.device):
-        _lib.check(_lib.load().uq_q4_decode(w.codes.data_ptr(), w.scales.data_ptr(), w.scale.data_ptr(), w.mats, w.rows,
-                                            w.cols, w.group, out.data_ptr(), _OUT[dtype], D.stream_handle(w.device)),
-                   "deq_q4")
+    _run(w.device, _lib.load().uq_q4_decode, "deq_q4", *w.ptrs, *w.form, out.data_ptr(), _OUT[dtype])
     return out
 
 
@@ -124,9 +125,8 @@ def round_scales(w: Q4, scales: torch.Tensor) -> Q4:
     are shared)."""
     c = _trained(w, scales).detach().contiguous()
     e, s = torch.empty_like(w.scales), torch.empty_like(w.scale)
-    with torch.cuda.device(w.device):
-        _lib.check(_lib.load().uq_q4_round_scales(c.data_ptr(), w.mats, c.numel() // max(w.mats, 1), e.data_ptr(),
-                                                  s.data_ptr(), D.stream_handle(w.device)), "round_scales")
+    _run(w.device, _lib.load().uq_q4_round_scales, "round_scales", c.data_ptr(), w.mats, c.numel() // max(w.mats, 1), e.data_ptr(),
+         s.data_ptr())
     return Q4(w.codes, e, s)
 
 
@@ -134,8 +134,7 @@ def check_errors(device=None) -> None:
     """Waits for the current stream and raises what the operators' kernels have met since the last call: ValueError for a
     token or an offset out of range, UQError for a wait that gave up."""
     dev = torch.device(device) if device is not None else D.device()
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().uq_q4_errors(D.stream_handle(dev)), "q4")
+    _run(dev if dev.index is not None else D.device(), _lib.load().uq_q4_errors, "q4")
 
 
 def _trained(w: Q4, scales) -> torch.Tensor:
@@ -147,14 +146,15 @@ def _trained(w: Q4, scales) -> torch.Tensor:
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """(..., n) as a matrix whose rows the kernels can read: unit inner stride, 16-byte aligned base and row stride."""
-    x = x.reshape(-1, x.shape[-1])
-    if x.shape[0] == 0 or x.shape[1] == 0:
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    T, n = x.shape
+    ld, inner = x.stride()
+    if T <= 1:
+        ld = n
+    if (inner == 1 and not ld & 7 and ld >= n and not x.data_ptr() & 15) or T == 0 or n == 0:
         return x
-    ld = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    if x.stride(1) == 1 and ld % 8 == 0 and ld >= x.shape[1] and not x.data_ptr() & 15:
-        return x
-    n = x.shape[1]
-    pad = torch.empty((x.shape[0], -(-n // 8) * 8), dtype=x.dtype, device=x.device)
+    pad = torch.empty((T, -(-n // 8) * 8), dtype=x.dtype, device=x.device)
     pad[:, :n] = x
     return pad[:, :n]
 
@@ -162,6 +162,32 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def _ld(x: torch.Tensor) -> int:
     """Row stride; of a single row, what the kernels ask of it."""
     return x.stride(0) if x.shape[0] > 1 else -(-x.shape[1] // 8) * 8
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _run(dev: torch.device, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the current stream of ``dev``, raising for its status."""
+    i = dev.index
+    stream = _raw_stream(i) if _raw_stream is not None else D.stream_handle(dev)
+    if torch.cuda.current_device() == i:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, stream)
+    if rc:
+        _lib.check(rc, what)
+
+
+@lru_cache(maxsize=4096)
+def _workspace_bytes(name: str, *sizes) -> int:
+    return getattr(_lib.load(), name + "_workspace_bytes")(*sizes)
+
+
+def _scratch(nbytes: int, dev: torch.device):
+    """Of its own for each call: calls on several streams and captured graphs share nothing."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
 def _checked(x: torch.Tensor, w: Q4, offsets, what: str) -> None:
@@ -185,22 +211,19 @@ def _checked(x: torch.Tensor, w: Q4, offsets, what: str) -> None:
 
 def _call(name: str, T: int, a: torch.Tensor, w: Q4, offsets, out: torch.Tensor, zero_rest: bool) -> None:
     """uq_q4_linear or uq_q4_linear_dx on rows ``a``."""
-    lib = _lib.load()
-    nbytes = getattr(lib, name + "_workspace_bytes")(T, w.mats, w.rows, w.cols)
-    # of its own for each call: calls on several streams and captured graphs share nothing
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
-    with torch.cuda.device(w.device):
-        _lib.check(getattr(lib, name)(a.data_ptr(), _ACT[a.dtype], T, _ld(a), w.codes.data_ptr(), w.scales.data_ptr(),
-                                      w.scale.data_ptr(), w.mats, w.rows, w.cols, w.group, D.ptr(offsets),
-                                      out.data_ptr(), out.stride(0) if T > 1 else out.shape[1], int(zero_rest),
-                                      D.ptr(ws), nbytes, torch.cuda.current_stream(w.device).cuda_stream), name)
+    mats, rows, cols, group = w.form
+    nbytes = _workspace_bytes(name, T, mats, rows, cols) if offsets is None else 0
+    ws = _scratch(nbytes, w.device)
+    _run(w.device, getattr(_lib.load(), name), name, a.data_ptr(), _ACT[a.dtype], T, _ld(a), *w.ptrs, mats, rows, cols, group,
+         offsets.data_ptr() if offsets is not None else None, out.data_ptr(), out.stride(0) if T > 1 else out.shape[1],
+         zero_rest, ws.data_ptr() if nbytes else None, nbytes)
 
 
 def _forward(x2: torch.Tensor, w: Q4, offsets, out=None) -> torch.Tensor:
     T = x2.shape[0]
     zero_rest = out is None
     if out is None:
-        out = torch.empty((T, w.rows), dtype=x2.dtype, device=w.device)
+        out = x2.new_empty((T, w.rows))
     if T and w.rows:
         _call("uq_q4_linear", T, x2, w, offsets, out, zero_rest)
     return out
@@ -212,7 +235,7 @@ class _Product(torch.autograd.Function):
         x2 = _rows(x)
         ctx.w, ctx.shape = w, x.shape
         ctx.save_for_backward(x2 if scales is not None else None, offsets, w.codes, w.scales, w.scale)
-        return _forward(x2, w, offsets).reshape(*x.shape[:-1], w.rows)
+        return _shaped(_forward(x2, w, offsets), x, w)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -232,15 +255,15 @@ class _Product(torch.autograd.Function):
         if ctx.needs_input_grad[1]:
             dc = torch.empty(w.scales.shape, dtype=torch.float32, device=w.device)
             if dc.numel():
-                lib = _lib.load()
-                nbytes = lib.uq_q4_linear_dscale_workspace_bytes(T, w.mats, w.rows, w.cols, w.group)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
-                with torch.cuda.device(w.device):
-                    _lib.check(lib.uq_q4_linear_dscale(D.ptr(d2), D.ptr(x2), _ACT[dy.dtype], T, _ld(d2), _ld(x2),
-                                                       w.codes.data_ptr(), w.mats, w.rows, w.cols, w.group, D.ptr(offsets),
-                                                       dc.data_ptr(), D.ptr(ws), nbytes, D.stream_handle(w.device)),
-                               "uq_q4_linear_dscale")
+                nbytes = _workspace_bytes("uq_q4_linear_dscale", T, *w.form)
+                ws = _scratch(nbytes, w.device)
+                _run(w.device, _lib.load().uq_q4_linear_dscale, "uq_q4_linear_dscale", D.ptr(d2), D.ptr(x2), _ACT[dy.dtype], T,
+                     _ld(d2), _ld(x2), w.ptrs[0], *w.form, D.ptr(offsets), dc.data_ptr(), D.ptr(ws), nbytes)
         return dx, dc, None, None
+
+
+def _shaped(y: torch.Tensor, x: torch.Tensor, w: Q4) -> torch.Tensor:
+    return y if x.dim() == 2 else y.reshape(*x.shape[:-1], w.rows)
 
 
 def _wants_grad(*tensors) -> bool:
@@ -255,7 +278,7 @@ def linear(x: torch.Tensor, w: Q4, scales: torch.Tensor | None = None) -> torch.
         _trained(w, scales)
     if _wants_grad(x, scales):
         return _Product.apply(x, scales, w, None)
-    return _forward(_rows(x), w, None).reshape(*x.shape[:-1], w.rows)
+    return _shaped(_forward(_rows(x), w, None), x, w)
 
 
 def grouped_linear(x: torch.Tensor, offsets: torch.Tensor, w: Q4, scales: torch.Tensor | None = None,
@@ -295,25 +318,18 @@ class _Embedding(torch.autograd.Function):
         T = d2.shape[0]
         dc = torch.empty(w.scales.shape, dtype=torch.float32, device=w.device)
         if dc.numel():
-            lib = _lib.load()
-            nbytes = lib.uq_q4_embed_dscale_workspace_bytes(T, w.rows, w.cols, w.group)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None
-            with torch.cuda.device(w.device):
-                _lib.check(lib.uq_q4_embed_dscale(D.ptr(tokens), int(tokens.dtype == torch.int64), T, D.ptr(d2),
-                                                  _OUT[d2.dtype], _ld(d2), w.codes.data_ptr(), w.rows, w.cols, w.group,
-                                                  ctx.alpha, dc.data_ptr(), D.ptr(ws), nbytes, D.stream_handle(w.device)),
-                           "uq_q4_embed_dscale")
+            nbytes = _workspace_bytes("uq_q4_embed_dscale", T, *w.form[1:])
+            ws = _scratch(nbytes, w.device)
+            _run(w.device, _lib.load().uq_q4_embed_dscale, "uq_q4_embed_dscale", D.ptr(tokens), tokens.dtype == torch.int64, T,
+                 D.ptr(d2), _OUT[d2.dtype], _ld(d2), w.ptrs[0], *w.form[1:], ctx.alpha, dc.data_ptr(), D.ptr(ws), nbytes)
         return None, dc, None, None, None
 
 
 def _lookup(tokens, w, alpha, dtype):
     out = torch.empty((*tokens.shape, w.cols), dtype=dtype, device=w.device)
-    if tokens.numel():
-        with torch.cuda.device(w.device):
-            _lib.check(_lib.load().uq_q4_embed(tokens.data_ptr(), int(tokens.dtype == torch.int64), tokens.numel(),
-                                               w.codes.data_ptr(), w.scales.data_ptr(), w.scale.data_ptr(), w.rows, w.cols,
-                                               w.group, alpha, out.data_ptr(), _OUT[dtype],
-                                               torch.cuda.current_stream(w.device).cuda_stream), "embedding")
+    if out.numel():
+        _run(w.device, _lib.load().uq_q4_embed, "embedding", tokens.data_ptr(), tokens.dtype == torch.int64, tokens.numel(), *w.ptrs,
+             *w.form[1:], alpha, out.data_ptr(), _OUT[dtype])
     return out
 
 
