@@ -18,8 +18,8 @@ namespace tma = uq::tma;
 __device__ int g_mm_bad_offset, g_mm_timeout;
 
 // ----------------------------------------------------------------------------
-// Tiles: 128 weight columns of the result by up to `bt` rows of one matrix's
-// run, by one of `splits` parts of the contraction.
+// Tiles: `wtiles` ranges of weight columns of the result by up to `bt` rows of
+// one matrix's run, by one of `splits` parts of the contraction.
 // ----------------------------------------------------------------------------
 struct Runs {
     const int32_t *offsets;   // null: one matrix, all rows
@@ -29,63 +29,59 @@ struct Runs {
 };
 
 struct Tile {
-    int64_t mat, row0;
-    int rows, wt, split;
+    int mat, row0, rows, wt, split;
 };
 
 // Finds a warp's tiles in rising order: the 32 lanes hold 32 matrices' runs at a
 // time.  An offset counts as at least its predecessors and at most T.
 struct Finder {
-    int64_t first, base, lo, hi, incl, top, begin;   // matrices and row tiles before this block of 32; this lane's run
+    int first, lo, incl, top, begin;   // matrices before this block of 32; this lane's run: first row, row tiles up to its end
+    int64_t base;                      // row tiles before this block
     bool loaded;
 
     __device__ __forceinline__ void start(const Runs &r) {
-        first = base = 0;
+        first = 0;
+        base = 0;
         loaded = false;
+        top = 0;
         if (r.offsets) {
-            const int64_t o = r.offsets[0];
-            top = min(max(o, int64_t(0)), r.T);
+            const int o = r.offsets[0];
+            top = min(max(o, 0), int(r.T));
             if (o != top) g_mm_bad_offset = 1;
-        } else {
-            top = 0;
         }
         begin = top;
     }
     __device__ __forceinline__ void load(const Runs &r) {
-        const int lane = threadIdx.x & 31;
-        const int64_t i = first + lane;
-        int64_t o = i < r.mats ? int64_t(r.offsets[i + 1]) : 0;
-        int64_t m = i < r.mats ? min(max(o, int64_t(0)), r.T) : 0;
-        m = max(m, top);
+        const int lane = threadIdx.x & 31, i = first + lane, n = int(r.mats), T = int(r.T);
+        const int o = i < n ? r.offsets[i + 1] : 0;
+        int m = max(i < n ? min(max(o, 0), T) : 0, top);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, m, d);
+            const int v = __shfl_up_sync(0xffffffffu, m, d);
             if (lane >= d) m = max(m, v);
         }
-        if (i < r.mats && o != m) g_mm_bad_offset = 1;
-        hi = m;
+        if (i < n && o != m) g_mm_bad_offset = 1;
         lo = __shfl_up_sync(0xffffffffu, m, 1);
         if (lane == 0) lo = top;
-        incl = (hi - lo + r.bt - 1) / r.bt;
+        incl = (m - lo + r.bt - 1) / r.bt;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, incl, d);
+            const int v = __shfl_up_sync(0xffffffffu, incl, d);
             if (lane >= d) incl += v;
         }
-        top = __shfl_sync(0xffffffffu, hi, 31);
+        top = __shfl_sync(0xffffffffu, m, 31);
         loaded = true;
     }
     // Tile number `t`; false beyond the last.
     __device__ __forceinline__ bool find(const Runs &r, int64_t t, Tile &tile) {
-        tile.split = int(t % r.splits);
-        const int64_t u = t / r.splits;
-        tile.wt = int(u % r.wtiles);
+        const int64_t u = runs_split(r, t, tile.split);
         const int64_t rt = u / r.wtiles;
+        tile.wt = int(u - rt * r.wtiles);
         if (!r.offsets) {
             tile.mat = 0;
-            tile.row0 = rt * r.bt;
-            if (tile.row0 >= r.T) return false;
-            tile.rows = int(min(r.T - tile.row0, int64_t(r.bt)));
+            if (rt * r.bt >= r.T) return false;
+            tile.row0 = int(rt) * r.bt;
+            tile.rows = min(int(r.T) - tile.row0, r.bt);
             return true;
         }
         for (;;) {
@@ -93,19 +89,27 @@ struct Finder {
                 if (first >= r.mats) return false;
                 load(r);
             }
-            const int64_t all = __shfl_sync(0xffffffffu, incl, 31);
+            const int all = __shfl_sync(0xffffffffu, incl, 31);
             if (rt < base + all) break;
             base += all;
             first += 32;
             loaded = false;
         }
         const int at = __popc(__ballot_sync(0xffffffffu, base + incl <= rt));   // runs that end before the tile
-        const int64_t before = __shfl_sync(0xffffffffu, incl, at > 0 ? at - 1 : 0);
-        const int64_t l = __shfl_sync(0xffffffffu, lo, at), h = __shfl_sync(0xffffffffu, hi, at);
+        const int before = __shfl_sync(0xffffffffu, incl, at > 0 ? at - 1 : 0);
+        const int l = __shfl_sync(0xffffffffu, lo, at), next = __shfl_sync(0xffffffffu, lo, at < 31 ? at + 1 : 31);
         tile.mat = first + at;
-        tile.row0 = l + (rt - base - (at > 0 ? before : 0)) * r.bt;
-        tile.rows = int(min(h - tile.row0, int64_t(r.bt)));
+        tile.row0 = l + int(rt - base - (at > 0 ? before : 0)) * r.bt;
+        tile.rows = min((at < 31 ? next : top) - tile.row0, r.bt);
         return true;
+    }
+    static __device__ __forceinline__ int64_t runs_split(const Runs &r, int64_t t, int &split) {
+        if (r.splits == 1) {
+            split = 0;
+            return t;
+        }
+        split = int(t % r.splits);
+        return t / r.splits;
     }
     // The end of the last run, once find() has gone beyond the last tile.
     __device__ __forceinline__ int64_t end(const Runs &r) const { return r.offsets ? top : r.T; }
@@ -114,51 +118,65 @@ struct Finder {
 // ----------------------------------------------------------------------------
 // Weights in 16-bit halves
 // ----------------------------------------------------------------------------
-// The pair (2 i, 2 i + 1) of a word as 16 + u in two halves: u moved to the top
-// bits of the significand of 16.0.  Then e (16 + u) - 24 e = e q in one fused
-// multiply-add: 24 e and e q have at most 8 bits, so nothing rounds.
+// The pair (2 i, 2 i + 1) of a word as a + b u in two halves, u in the significand
+// of a power of two, and the factors of one fused multiply-add that makes e q of
+// it.  Nothing rounds or overflows, |e| <= 448 with 4 significant bits:
+//   bfloat16: u in bits 0 .. 3 of 128:  128 + u, times e less 136 e (17 x 15 has 8 bits)
+//   float16:  u in bits 4 .. 7 of 1024: 1024 + 16 u, times e / 16 less 72 e (9 x 15 has
+//             8 bits, 72 x 448 < 65504)
+// Three shifts a word, since one of the four pairs lies in place.
 template <bool BF16> struct Halves;
 template <> struct Halves<true> {
     using T = __nv_bfloat16;
-    static __device__ __forceinline__ uint32_t raw(uint32_t w, int i) {
-        const uint32_t v = i == 0 ? w << 3 : w >> (4 * i - 3);
-        return (v & 0x00780078u) | 0x41804180u;
+    struct Scale { uint32_t e, z; };
+    // e: two E4M3 values as float16; which: 0 or 1
+    static __device__ __forceinline__ Scale scale(uint32_t e, int which) {
+        const float f = __half2float(__ushort_as_half((unsigned short)(which ? e >> 16 : e)));
+        Scale s;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(s.e) : "f"(f));
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(s.z) : "r"(s.e), "r"(0xc308c308u));
+        return s;
     }
-    static __device__ __forceinline__ uint32_t pair(float e) {
-        const __nv_bfloat162 p = __float2bfloat162_rn(e);
-        return *reinterpret_cast<const uint32_t *>(&p);
-    }
-    static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
-        uint32_t d;
-        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-        return d;
+    static __device__ __forceinline__ void widen8(uint32_t w, const Scale &s, uint32_t *out) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+            asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(out[i]) : "r"(v), "r"(s.e), "r"(s.z));
+        }
     }
 };
 template <> struct Halves<false> {
     using T = __half;
-    static __device__ __forceinline__ uint32_t raw(uint32_t w, int i) {
-        const uint32_t v = i == 0 ? w << 6 : i == 1 ? w << 2 : w >> (4 * i - 6);
-        return (v & 0x03c003c0u) | 0x4c004c00u;
+    struct Scale { uint32_t e, z; };
+    static __device__ __forceinline__ Scale scale(uint32_t e, int which) {
+        const uint32_t d = __byte_perm(e, 0, which ? 0x3232 : 0x1010);
+        Scale s;
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.e) : "r"(d), "r"(0x2c002c00u));   // 1 / 16
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.z) : "r"(d), "r"(0xd480d480u));   // -72
+        return s;
     }
-    static __device__ __forceinline__ uint32_t pair(float e) {
-        const __half2 p = __float2half2_rn(e);
-        return *reinterpret_cast<const uint32_t *>(&p);
-    }
-    static __device__ __forceinline__ uint32_t fma(uint32_t a, uint32_t b, uint32_t c) {
-        uint32_t d;
-        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-        return d;
+    static __device__ __forceinline__ void widen8(uint32_t w, const Scale &s, uint32_t *out) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t v = ((i == 0 ? w << 4 : w >> (4 * i - 4)) & 0x00f000f0u) | 0x64006400u;
+            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(out[i]) : "r"(v), "r"(s.e), "r"(s.z));
+        }
     }
 };
 
+// Two E4M3 bytes as two float16 (E4M3 is a subset; NaN stays NaN).
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t b) {
+    uint32_t h;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
+    return h;
+}
+
 // 32 codes of one group -> 16 registers of two halves each, in order.
-template <bool BF16> __device__ __forceinline__ void widen32(const uint4 &c, float e, uint32_t *out) {
-    const uint32_t s = Halves<BF16>::pair(e), z = Halves<BF16>::pair(-24.0f * e);
-    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out[4 * j + i] = Halves<BF16>::fma(Halves<BF16>::raw(w[j], i), s, z);
+template <bool BF16> __device__ __forceinline__ void widen32(const uint4 &c, const typename Halves<BF16>::Scale &s, uint32_t *out) {
+    Halves<BF16>::widen8(c.x, s, out);
+    Halves<BF16>::widen8(c.y, s, out + 4);
+    Halves<BF16>::widen8(c.z, s, out + 8);
+    Halves<BF16>::widen8(c.w, s, out + 12);
 }
 
 __device__ __forceinline__ uint4 lds128(unsigned addr) {
@@ -177,40 +195,15 @@ struct Weights {
     int gshift;       // group = 2^gshift
 };
 
-// The scale bytes that one lane needs for a chunk of four stages, in one word;
-// 0 (e = 0, so that whatever the codes are the weights are 0) beyond the matrix.
-// Forward: byte j is group j of the chunk's 256 values of weight row `row`.
-// DX: bytes 0, 1 and 2, 3 are the two pieces of 32 values in this lane's row of
-// stages `half` and `half` + 2.
-template <bool DX>
-__device__ __forceinline__ uint64_t chunk_scales(const Weights &w, const uint8_t *e0, int64_t groups, int64_t row, int wt, int stage, int half, int quad) {
-    uint64_t v = 0;
-    if (DX) {
-        const int64_t k0 = int64_t(wt) * 128 + (quad >> 1) * 64;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t n = int64_t(stage + half + 2 * i) * 64 + (quad & 1) * 32 + (threadIdx.x & 31);
-            if (n >= w.N) continue;
-            const uint8_t *p = e0 + n * groups;
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (k0 + 32 * j < w.K) v |= uint64_t(__ldg(p + ((k0 + 32 * j) >> w.gshift))) << (16 * i + 8 * j);
-        }
-    } else if (row < w.N) {
-        const int64_t g0 = (int64_t(stage) * 64) >> w.gshift;
-        const int count = 256 >> w.gshift;   // 8, 4, 2 or 1, aligned where rows are whole chunks
-        const uint8_t *p = e0 + g0;
-        if ((w.K & 255) == 0) {
-            if (count == 8) v = __ldg(reinterpret_cast<const unsigned long long *>(p));
-            else if (count == 4) v = __ldg(reinterpret_cast<const unsigned *>(p));
-            else if (count == 2) v = __ldg(reinterpret_cast<const unsigned short *>(p));
-            else v = __ldg(p);
-        } else {
-            for (int j = 0; j < count; ++j)
-                if (g0 + j < groups) v |= uint64_t(__ldg(p + j)) << (8 * j);
-        }
-    }
-    return v;
+// The E4M3 bytes of values k .. k + 31 and k + 32 .. k + 63 of the row whose bytes
+// begin at `p`, in the low 16 bits; 0 (e = 0: the weights are 0 whatever the
+// codes are) beyond K.  k is a multiple of 64.
+__device__ __forceinline__ uint32_t scale_pair(const Weights &w, const uint8_t *p, int64_t k) {
+    if (k >= w.K) return 0;
+    p += k >> w.gshift;
+    if (w.gshift > 5) return uint32_t(__ldg(p)) * 0x101u;
+    if ((w.K & 63) == 0) return __ldg(reinterpret_cast<const unsigned short *>(p));   // rows of an even number of bytes
+    return uint32_t(__ldg(p)) | (k + 32 < w.K ? uint32_t(__ldg(p + 1)) << 8 : 0u);
 }
 
 struct Out {
@@ -220,154 +213,227 @@ struct Out {
 };
 
 // Register j of lane i: row j, column i of a 32 x 32 piece of the result.
-// Rows [0, rows) and columns below J are written; one row's 32 columns are one
-// line of 64 (or 128) bytes.
-template <bool BF16>
-__device__ __forceinline__ void store_piece(const uint32_t (&r)[32], float s, const Out &o, int split, int splits, int64_t row0, int rows, int64_t col) {
+// pack_piece: rows 2 j and 2 j + 1 in the halves of v[j], scaled and rounded.
+template <bool BF16> __device__ __forceinline__ void pack_piece(const uint32_t (&r)[32], float s, uint32_t (&v)[16]) {
     using T = typename Halves<BF16>::T;
-    if (col >= o.J) return;
-    if (splits > 1) {
-        float *p = static_cast<float *>(o.out) + (int64_t(split) * o.T + row0) * o.J + col;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < rows) p[int64_t(j) * o.J] = __uint_as_float(r[j]);
-    } else {
-        T *p = static_cast<T *>(o.out) + row0 * o.ld + col;
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < rows) p[int64_t(j) * o.ld] = from_float<T>(s * __uint_as_float(r[j]));
+    for (int j = 0; j < 16; ++j) {
+        T two[2] = {from_float<T>(s * __uint_as_float(r[2 * j])), from_float<T>(s * __uint_as_float(r[2 * j + 1]))};
+        v[j] = *reinterpret_cast<const uint32_t *>(two);
     }
 }
+// Writes rows [0, rows) and columns below J.  Where two columns share an aligned
+// word (`wide`) neighbouring lanes trade halves, so that each writes both columns
+// of one row: half the store instructions, a row's 32 columns still one line of
+// 64 bytes.
+__device__ __forceinline__ void store_piece(const uint32_t (&v)[16], void *out, int64_t ld, int64_t J, bool wide, int row0, int rows, int64_t col) {
+    const int odd = threadIdx.x & 1;
+    if (wide) {
+        char *p = static_cast<char *>(out) + (int64_t(row0 + odd) * ld + (col - odd)) * 2;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, v[j], 1);
+            const uint32_t word = odd ? __byte_perm(got, v[j], 0x7632) : __byte_perm(v[j], got, 0x5410);
+            if (2 * j + odd < rows && col < J) *reinterpret_cast<uint32_t *>(p) = word;
+            p += ld * 4;
+        }
+    } else if (col < J) {
+        unsigned short *p = static_cast<unsigned short *>(out) + int64_t(row0) * ld + col;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (j < rows) *p = (unsigned short)(v[j >> 1] >> (16 * (j & 1)));
+            p += ld;
+        }
+    }
+}
+// A tile's share of one warp, out of line so that the widening loop keeps its
+// registers: 32 lanes' columns of `pieces` times 32 rows, every 128 rows.  Once
+// the values are in registers the tensor memory is free (`drained`).
+template <bool BF16, int PIECES>
+__device__ __noinline__ void write_tile(unsigned at, unsigned drained, float scale, void *out, int64_t ld, int64_t J, bool wide, int row0, int rows, int64_t col) {
+    uint32_t v[PIECES][16];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        uint32_t r[32];
+        tc5::ld32(at + i * 128, r);   // beyond the tile's rows: whatever is there, not written
+        tc5::wait_ld();
+        pack_piece<BF16>(r, scale, v[i]);
+    }
+    tc5::fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc5::mbar_arrive_remote(drained);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+        if (i * 128 < rows) store_piece(v[i], out, ld, J, wide, row0 + i * 128, rows - i * 128, col);
+}
+// The same for a part of a split contraction: floats, unscaled, J a row.
+__device__ __noinline__ void write_part(unsigned at, unsigned drained, float *out, int64_t J, int rows, int64_t col) {
+    for (int i = 0; i < rows; i += 128) {
+        uint32_t r[32];
+        tc5::ld32(at + i, r);
+        tc5::wait_ld();
+        float *p = out + int64_t(i) * J + col;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+            if (i + j < rows && col < J) *p = __uint_as_float(r[j]);
+            p += J;
+        }
+    }
+    tc5::fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc5::mbar_arrive_remote(drained);
+}
 
-// Rows outside every run, a share of them for each block's eight warps.
-template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int64_t end) {
+// Rows outside every run, a share of them for the first `threads` threads of each block.
+template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int64_t end, int threads) {
     const int64_t rest = o.T - (end - begin);
     for (int64_t i = blockIdx.x; i < rest; i += gridDim.x) {
         T *p = static_cast<T *>(o.out) + (i < begin ? i : end + i - begin) * o.ld;
-        for (int64_t j = threadIdx.x; j < o.J; j += 256) p[j] = from_float<T>(0.0f);
+        for (int64_t j = threadIdx.x; j < o.J; j += threads) p[j] = from_float<T>(0.0f);
     }
 }
 
 // ----------------------------------------------------------------------------
 // The product kernel.  The result is formed transposed, weight columns in the
-// 128 lanes of tensor memory and up to BT rows in its columns, so that few rows
-// make a narrow instruction.  Stages of 64 contraction steps: `full_b` the rows'
-// tile (TMA, 128-byte swizzle), `full_a` the widened weights, `empty` both free
-// again.
+// lanes of tensor memory and up to BT rows in its columns, so that few rows make
+// a narrow instruction.  A pair of CTAs takes 256 weight columns, 128 each, and
+// each CTA brings half of the tile's rows: alone, a CTA needed 64 bytes a clock
+// of rows from L2, and L2 gave 12 TB/s, 43 a clock and SM.  Stages of 64
+// contraction steps: `full_b` this CTA's half of the rows (TMA, 128-byte
+// swizzle), `full_a` (in the first CTA, for both) the widened weights, `empty`
+// both free again.
 //   forward: lane n; the weights go from registers into tensor memory (32
 //            columns a stage), codes by TMA in chunks of 256 steps
 //   DX:      lane k; a stage is 64 rows n of 128 codes, widened into shared
 //            memory with k contiguous
-// Warps 0 .. 7 widen (four a stage, in turn) and write results; warp 8 copies
-// the rows, warp 9 the codes, warp 10 issues the products.
+// Warps 0 .. 15 widen (warps 4 s .. 4 s + 3 stage s of each chunk) and write
+// results, those of a tile after the next tile's first chunk is widened, so that
+// the tensor cores have work meanwhile; warp 16 copies the rows, warp 17 the
+// codes; warp 18 issues the products (first CTA) or tells the first CTA that its
+// rows are there (second).
 // ----------------------------------------------------------------------------
-constexpr int kThreads = 352;
+constexpr int kWiden = 16, kThreads = (kWiden + 3) * 32;
 
 template <int BT, bool DX> struct Cfg {
-    // stages: an even number, so that each slot is always widened by the same four warps
-    static constexpr int NS = DX ? (BT == 256 ? 4 : 6) : BT == 256 ? 4 : BT == 128 ? 6 : 8;
-    static constexpr int kChunks = DX ? (BT == 64 ? 4 : 2) : BT == 256 ? 4 : BT == 128 ? 6 : 8;
-    static constexpr int kB = BT * 128, kA = DX ? 16384 : 0, kC = 16384;
-    static constexpr int kBar = 3 * NS + 2 * kChunks + 2;
+    static constexpr int NS = DX ? (BT == 256 ? 5 : 6) : 8;                  // stages
+    static constexpr int kChunks = DX ? (BT == 64 ? 4 : BT == 128 ? 3 : 3) : BT == 256 ? 5 : 8;
+    static constexpr int kB = BT * 64, kA = DX ? 16384 : 0, kC = 16384;
+    static constexpr int kBar = 4 * NS + 2 * kChunks + 2;
     static constexpr int kSmem = 1024 + NS * (kB + kA) + kChunks * kC + kBar * 8 + 16;
-    static constexpr int kTmem = 512;
     static_assert(kSmem <= 232448, "shared memory of one block");
-    static_assert(DX ? BT <= 512 : BT + 32 * NS <= 512, "tensor memory");
+    static_assert(DX || BT + 32 * NS <= 512, "tensor memory");
 };
 
 template <int BT, bool BF16, bool DX>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_codes, Runs runs, Weights w, Out o) {
     using C = Cfg<BT, DX>;
-    constexpr int NS = C::NS, NC = C::kChunks, kBox = BT / 4;
+    constexpr int NS = C::NS, NC = C::kChunks, kBox = BT / 4;   // rows of one copy: half of a CTA's share
     extern __shared__ uint8_t smem_raw[];
     const unsigned base = (tc5::smem_addr(smem_raw) + 1023u) & ~1023u;
     const unsigned sb = base, sa = sb + NS * C::kB, sc = sa + NS * C::kA, bars = sc + NC * C::kC;
-    const unsigned full_b = bars, full_a = bars + 8 * NS, empty = bars + 16 * NS, full_c = bars + 24 * NS, empty_c = full_c + 8 * NC,
-                   done = empty_c + 8 * NC, drained = done + 8, misc = drained + 8;
+    const unsigned full_b = bars, full_a = bars + 8 * NS, empty = bars + 16 * NS, full_p = bars + 24 * NS, full_c = bars + 32 * NS,
+                   empty_c = full_c + 8 * NC, done = empty_c + 8 * NC, drained = done + 8, misc = drained + 8;
     volatile int *gave_up = reinterpret_cast<volatile int *>(smem_raw + (misc + 4 - tc5::smem_addr(smem_raw)));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == 10) tc5::tmem_alloc<C::kTmem>(misc);
+    const int warp = tc5::warp_id(), lane = threadIdx.x & 31;
+    const unsigned rank = tc5::pair_rank();
+    if (warp == kWiden + 2) tc5::tmem_alloc<512>(misc);
     if (threadIdx.x == 0) {
         *gave_up = 0;
         for (int i = 0; i < NS; ++i) {
             tma::mbar_init(full_b + 8 * i, 1);
-            tma::mbar_init(full_a + 8 * i, 4);
+            tma::mbar_init(full_a + 8 * i, 8);
             tma::mbar_init(empty + 8 * i, 1);
+            tma::mbar_init(full_p + 8 * i, 1);
         }
         for (int i = 0; i < NC; ++i) {
             tma::mbar_init(full_c + 8 * i, 1);
-            tma::mbar_init(empty_c + 8 * i, 8);
+            tma::mbar_init(empty_c + 8 * i, kWiden);
         }
         tma::mbar_init(done, 1);
-        tma::mbar_init(drained, 8);
+        tma::mbar_init(drained, 2 * kWiden);
         tma::mbar_init(misc + 8, 1);   // products in flight, where a wait gave up
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     tc5::fence_before();
     __syncthreads();
+    tc5::pair_sync();
     tc5::fence_after();
     unsigned tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(misc));
+    tmem = __shfl_sync(0xffffffffu, tmem, 0);
     const unsigned tmem_a = tmem + BT;
 
     tc5::Waiter wt{gave_up, &g_mm_timeout};
     Finder find;
     find.start(runs);
     Tile t;
+    const int64_t step = gridDim.x >> 1, first = blockIdx.x >> 1;                 // pairs
     const int64_t depth = DX ? w.N : w.K;
     const int all = int((depth + 63) / 64);                                       // stages of the whole contraction
     const int per = runs.splits > 1 ? ((all + 4 * runs.splits - 1) / (4 * runs.splits)) * 4 : all;   // of one part, whole chunks
     unsigned it = 0, ct = 0, tiles = 0;                                           // stages, chunks, tiles so far
 
-    if (warp == 8) {
-        // rows
-        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, t); tile += gridDim.x) {
-            const int s0 = t.split * per, n = max(0, min(per, all - s0));
-            const int boxes = (((t.rows + 15) & ~15) + kBox - 1) / kBox;
+    if (warp == kWiden) {
+        // rows: this CTA's half of the product's N
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step) {
+            const int s0 = t.split * per, n = min(per, all - s0);
+            const int half = ((t.rows + 31) & ~31) >> 1, boxes = (half + kBox - 1) / kBox, row = int(t.row0) + int(rank) * half;
             for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS;
                 if (!wt.wait(empty + 8 * slot, ((it / NS) & 1) ^ 1)) break;
                 if (lane == 0) {
                     tma::mbar_arrive_expect_tx(full_b + 8 * slot, boxes * kBox * 128);
                     for (int b = 0; b < boxes; ++b)
-                        tma::load2d(sb + slot * C::kB + b * kBox * 128, &map_rows, (s0 + s) * 64, int(t.row0) + b * kBox, full_b + 8 * slot);
+                        tma::load2d(sb + slot * C::kB + b * kBox * 128, &map_rows, (s0 + s) * 64, row + b * kBox, full_b + 8 * slot);
                 }
+                __syncwarp();
             }
         }
         if (wt.fail)   // copies in flight land before the block ends
             for (unsigned i = it > NS ? it - NS : 0; i < it; ++i) tc5::Waiter::drain(full_b + 8 * (i % NS), (i / NS) & 1);
-    } else if (warp == 9) {
+    } else if (warp == kWiden + 1) {
         // codes: 128 rows of 256 codes, or 256 rows of 128
-        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, t); tile += gridDim.x) {
-            const int s0 = t.split * per, n = max(0, min(per, all - s0));
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step) {
+            const int s0 = t.split * per, n = min(per, all - s0);
+            const int64_t row = t.mat * w.N;
+            const int wtile = t.wt * 2 + int(rank);
             for (int s = 0; s < n; s += 4, ++ct) {
                 const int slot = ct % NC;
                 if (!wt.wait(empty_c + 8 * slot, ((ct / NC) & 1) ^ 1)) break;
                 if (lane == 0) {
                     tma::mbar_arrive_expect_tx(full_c + 8 * slot, C::kC);
-                    const int64_t row = t.mat * w.N;
-                    if (DX) tma::load2d(sc + slot * C::kC, &map_codes, t.wt * 64, int(row + (s0 + s) * 64), full_c + 8 * slot);
-                    else tma::load2d(sc + slot * C::kC, &map_codes, (s0 + s) * 32, int(row + t.wt * 128), full_c + 8 * slot);
+                    if (DX) tma::load2d(sc + slot * C::kC, &map_codes, wtile * 64, int(row + (s0 + s) * 64), full_c + 8 * slot);
+                    else tma::load2d(sc + slot * C::kC, &map_codes, (s0 + s) * 32, int(row + int64_t(wtile) * 128), full_c + 8 * slot);
                 }
+                __syncwarp();
             }
         }
         if (wt.fail)
             for (unsigned i = ct > NC ? ct - NC : 0; i < ct; ++i) tc5::Waiter::drain(full_c + 8 * (i % NC), (i / NC) & 1);
-    } else if (warp == 10) {
+    } else if (warp == kWiden + 2 && rank == 1) {
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step) {
+            const int s0 = t.split * per, n = min(per, all - s0);
+            for (int s = 0; s < n; ++s, ++it) {
+                const int slot = it % NS;
+                if (!wt.wait(full_b + 8 * slot, (it / NS) & 1)) break;
+                if (lane == 0) tc5::mbar_arrive_remote(tc5::leader_addr(full_p + 8 * slot));
+                __syncwarp();
+            }
+        }
+    } else if (warp == kWiden + 2) {
         // products
-        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, t); tile += gridDim.x, ++tiles) {
-            const int s0 = t.split * per, n = max(0, min(per, all - s0));
-            const uint32_t idesc = tc5::idesc_f16(BF16, (t.rows + 15) & ~15, DX, false);
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step, ++tiles) {
+            const int s0 = t.split * per, n = min(per, all - s0);
+            const uint32_t idesc = tc5::idesc_f16(BF16, (t.rows + 31) & ~31, DX, false);
             if (!wt.wait(drained, (tiles & 1) ^ 1)) break;
             for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS;
                 const unsigned par = (it / NS) & 1;
-                if (!wt.wait(full_b + 8 * slot, par) || !wt.wait(full_a + 8 * slot, par)) break;
+                if (!wt.wait(full_b + 8 * slot, par) || !wt.wait(full_p + 8 * slot, par) || !wt.wait(full_a + 8 * slot, par)) break;
                 tc5::fence_after();
-                if (lane == 0) {
-                    const uint64_t b = tc5::desc128(sb + slot * C::kB, 16, 1024);
-                    const uint64_t a = tc5::desc128(sa + slot * C::kA, 8192, 1024);
+                const uint64_t b = tc5::desc128(sb + slot * C::kB, 16, 1024), a = tc5::desc128(sa + slot * C::kA, 8192, 1024);
+                if (tc5::elect()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         if (DX) tc5::mma_ss(tmem, a + k * 128, b + k * 2, idesc, s > 0 || k > 0);
@@ -377,47 +443,73 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                 }
                 __syncwarp();
             }
-            if (!wt.fail && lane == 0) tc5::commit(done);
+            if (!wt.fail && tc5::elect()) tc5::commit(done);
             __syncwarp();
         }
         if (wt.fail) {   // products in flight end before the block does
-            if (lane == 0) tc5::commit(misc + 8);
+            if (tc5::elect()) tc5::commit(misc + 8);
             __syncwarp();
             tc5::Waiter::drain(misc + 8, 0);
         }
     } else {
         // widen, then write the result
-        const int half = warp >> 2, quad = warp & 3;
+        const int stage = warp >> 2, quad = warp & 3;      // of each chunk; lanes of tensor memory
         const int64_t groups = w.K >> w.gshift;
-        bool more;
-        for (int64_t tile = blockIdx.x; (more = find.find(runs, tile, t)) && !wt.fail; tile += gridDim.x, ++tiles) {
-            const int s0 = t.split * per, n = max(0, min(per, all - s0));
-            const float scale = __ldg(w.scale + t.mat);
-            const int64_t row = int64_t(t.wt) * 128 + quad * 32 + lane;   // forward: this lane's weight row
-            const uint8_t *const e0 = w.scales + (t.mat * w.N + (DX ? 0 : min(row, w.N - 1))) * groups;
-            uint64_t eraw = chunk_scales<DX>(w, e0, groups, row, t.wt, s0, half, quad);
-            for (int c = 0; c < n; c += 4, ++ct) {
-                const int cslot = ct % NC, cn = min(4, n - c);
-                const unsigned cpar = (ct / NC) & 1;
-                const uint64_t ecur = eraw;
-                if (c + 4 < n) eraw = chunk_scales<DX>(w, e0, groups, row, t.wt, s0 + c + 4, half, quad);   // a chunk ahead
-                bool seen = false;
-                for (int s = half; s < cn; s += 2) {
-                    const int slot = (it + s) % NS;
-                    if (!seen && !wt.wait(full_c + 8 * cslot, cpar)) break;
-                    seen = true;
-                    if (!wt.wait(empty + 8 * slot, (((it + s) / NS) & 1) ^ 1)) break;
-                    float e[2];
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) e[p] = e4m3_value(uint8_t(ecur >> (8 * (DX ? (s & 2) + p : (2 * s + p) >> (w.gshift - 5)))));
+        unsigned cslot = 0, cpar = 0, slot0 = 0, par0 = 1;   // chunk slot and parity; the chunk's first stage and its parity of `empty`
+        const unsigned full_a0 = tc5::leader_addr(full_a), drained0 = tc5::leader_addr(drained);
+        const bool wide = runs.splits == 1 && !((o.ld | o.J) & 1) && !(reinterpret_cast<uintptr_t>(o.out) & 3);
+        Tile prev = {}, next = {};
+        bool have = false, more = find.find(runs, first, next);   // `prev` has still to be written
+        for (int64_t tile = first; !wt.fail; tile += step) {
+            const bool live = more;
+            int n = 0;
+            bool in = false;
+            const uint8_t *e0 = nullptr;
+            uint32_t eraw = 0;
+            const int s0 = next.split * per, wtile = next.wt * 2 + int(rank);
+            // scale bytes of this warp's stage of the chunk at stage c (which begins before the contraction's end)
+            auto scales_at = [&](int c) -> uint32_t {
+                if (DX) {
+                    const int nn = (s0 + c + stage) * 64 + (quad & 1) * 32 + lane;
+                    return nn < w.N ? scale_pair(w, e0 + nn * groups, int64_t(wtile) * 128 + (quad >> 1) * 64) : 0u;
+                }
+                return in ? scale_pair(w, e0, int64_t(s0 + c + stage) * 64) : 0u;
+            };
+            if (live) {
+                t = next;
+                more = find.find(runs, tile + step, next);
+                n = min(per, all - s0);
+                const int64_t row = int64_t(wtile) * 128 + quad * 32 + lane;   // forward: this lane's weight row
+                in = row < w.N;
+                e0 = w.scales + (t.mat * w.N + (DX || !in ? 0 : row)) * groups;
+                eraw = scales_at(0);
+                if (!DX && more && stage == 0) {   // the next tile's scales on their way to L2
+                    const int64_t r = next.mat * w.N + min(int64_t(next.wt * 2 + int(rank)) * 128 + quad * 32 + lane, w.N - 1);
+                    asm volatile("prefetch.global.L2 [%0];" :: "l"(w.scales + r * groups + ((int64_t(next.split) * per * 64) >> w.gshift)));
+                }
+            }
+            int c = 0;
+            do {
+                const int cn = min(4, n - c);
+                const uint32_t ecur = eraw;
+                if (c + 4 < n) eraw = scales_at(c + 4);   // a chunk ahead
+                if (stage < cn) {
+                    const unsigned wrap = slot0 + stage >= NS, slot = slot0 + stage - (wrap ? NS : 0);
+                    const uint32_t ep = e4m3_pair(ecur);
+                    const typename Halves<BF16>::Scale e[2] = {Halves<BF16>::scale(ep, 0), Halves<BF16>::scale(ep, 1)};
+                    if (!wt.wait(full_c + 8 * cslot, cpar)) break;
                     if (DX) {
                         // row rr of 128 codes (64 bytes, 64-byte swizzle): this warp's 64 values are pieces 2 h, 2 h + 1
-                        const int rr = s * 64 + (quad & 1) * 32 + lane, h = quad >> 1;
+                        const int rr = stage * 64 + (quad & 1) * 32 + lane, h = quad >> 1;
                         const unsigned line = sa + slot * C::kA + h * 8192 + ((quad & 1) * 32 + lane) * 128;
+                        uint4 code[2];
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) code[p] = lds128(sc + cslot * C::kC + rr * 64 + (((2 * h + p) ^ ((rr >> 1) & 3)) << 4));
+                        if (!wt.wait(empty + 8 * slot, par0 ^ wrap)) break;
 #pragma unroll
                         for (int p = 0; p < 2; ++p) {
                             uint32_t v[16];
-                            widen32<BF16>(lds128(sc + cslot * C::kC + rr * 64 + (((2 * h + p) ^ ((rr >> 1) & 3)) << 4)), e[p], v);
+                            widen32<BF16>(code[p], e[p], v);
 #pragma unroll
                             for (int q = 0; q < 4; ++q)
                                 sts128(line + (((4 * p + q) ^ (lane & 7)) << 4), v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
@@ -427,52 +519,63 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                         const int rr = quad * 32 + lane;
                         uint32_t v[32];
 #pragma unroll
-                        for (int p = 0; p < 2; ++p)
-                            widen32<BF16>(lds128(sc + cslot * C::kC + rr * 128 + (((2 * s + p) ^ (rr & 7)) << 4)), e[p], v + 16 * p);
+                        for (int p = 0; p < 2; ++p) widen32<BF16>(lds128(sc + cslot * C::kC + rr * 128 + (((2 * stage + p) ^ (rr & 7)) << 4)), e[p], v + 16 * p);
+                        if (!wt.wait(empty + 8 * slot, par0 ^ wrap)) break;
                         tc5::fence_after();
                         tc5::st32(tmem_a + slot * 32 + (unsigned(quad * 32) << 16), v);
                         tc5::wait_st();
                         tc5::fence_before();
                     }
                     __syncwarp();
-                    if (lane == 0) tc5::mbar_arrive(full_a + 8 * slot);
+                    if (lane == 0) tc5::mbar_arrive_remote(full_a0 + 8 * slot);
+                } else if (live) {
+                    // no stage in a short last chunk: still see its barriers, so that no wait of this warp meets a phase two
+                    // behind the one it means (a parity cannot tell them apart)
+                    const unsigned last = slot0 + cn - 1, wrap = last >= NS;
+                    if (!wt.wait(full_c + 8 * cslot, cpar) || !wt.wait(empty + 8 * (last - (wrap ? NS : 0)), par0 ^ wrap)) break;
                 }
-                if (wt.fail) break;
-                it += cn;
-                __syncwarp();
-                if (lane == 0) tc5::mbar_arrive(empty_c + 8 * cslot);
-            }
-            if (!wt.wait(done, tiles & 1)) break;
-            tc5::fence_after();
-            const int64_t col = int64_t(t.wt) * 128 + quad * 32 + lane;
-            for (int c = half; c * 32 < t.rows; c += 2) {
-                uint32_t r[32];
-                tc5::ld32(tmem + c * 32 + (unsigned(quad * 32) << 16), r);
-                tc5::wait_ld();
-                if (n == 0) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) r[j] = 0;
+                if (live) {
+                    __syncwarp();
+                    if (lane == 0) tc5::mbar_arrive(empty_c + 8 * cslot);
+                    slot0 += cn;
+                    if (slot0 >= NS) { slot0 -= NS; par0 ^= 1; }
+                    if (++cslot == NC) { cslot = 0; cpar ^= 1; }
                 }
-                store_piece<BF16>(r, scale, o, t.split, runs.splits, t.row0 + c * 32, t.rows - c * 32, col);
-            }
-            tc5::fence_before();
-            __syncwarp();
-            if (lane == 0) tc5::mbar_arrive(drained);
+                if (have) {
+                    // the tile before: its products are done; once its values are in registers the next tile's may begin
+                    have = false;
+                    if (!wt.wait(done, tiles & 1)) break;
+                    ++tiles;
+                    tc5::fence_after();
+                    const int64_t col = (int64_t(prev.wt) * 2 + rank) * 128 + quad * 32 + lane;
+                    const unsigned at = tmem + stage * 32 + (unsigned(quad * 32) << 16);
+                    const int r0 = prev.row0 + stage * 32, rows = prev.rows - stage * 32;
+                    if (runs.splits > 1)
+                        write_part(at, drained0, static_cast<float *>(o.out) + (int64_t(prev.split) * o.T + r0) * o.J, o.J, rows, col);
+                    else
+                        write_tile<BF16, BT == 256 ? 2 : 1>(at, drained0, __ldg(w.scale + prev.mat), o.out, o.ld, o.J, wide, r0, rows, col);
+                }
+                c += 4;
+            } while (c < n);
+            if (!live || wt.fail) break;
+            prev = t;
+            have = true;
         }
-        if (o.zero_rest && runs.offsets && !wt.fail) zero_rows<typename Halves<BF16>::T>(o, find.begin, find.end(runs));
+        if (o.zero_rest && runs.offsets && !wt.fail) zero_rows<typename Halves<BF16>::T>(o, find.begin, find.end(runs), kWiden * 32);
     }
+    tc5::fence_before();
     __syncthreads();
-    if (warp == 10) {
+    tc5::pair_sync();   // the other CTA's products read this one's memory, its warps arrive here
+    if (warp == kWiden + 2) {
         tc5::fence_after();
-        tc5::tmem_free<C::kTmem>(tmem);
+        tc5::tmem_free<512>(tmem);
     }
 }
 
 // ----------------------------------------------------------------------------
 // Few rows: bound by reading the codes once.  A block takes 32 weight rows; its
-// eight warps take every eighth step of 256 values of k each and add up in
-// shared memory at the end, so that even a 4096 x 4096 matrix gives every SM
-// 7 warps whose loads are all in flight at once.  The widened codes are operand
+// eight warps take 16 rows and every fourth step of 256 values of k each, two
+// steps' loads ahead, and add up in shared memory at the end.  The widened codes are operand
 // A of m16n8k16 products straight from registers: the contraction order is free
 // as long as both operands agree, so lane quarter q takes 64 consecutive values
 // of a row (two 16-byte loads) where the instruction says "columns 2 q, 2 q + 1,
@@ -487,55 +590,54 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-constexpr int kFewWarps = 8, kFewRows = 32;
+constexpr int kFewParts = 4, kFewRows = 32;
 
-// One lane's codes and scales of a step: 4 rows (g, g + 8, g + 16, g + 24) of 64 values.
+// One lane's codes and scales of a step: 64 values of 2 rows (g, g + 8).
 struct Step {
-    uint4 c[4][2];
-    uint32_t e;        // two rows' bytes; see load_step
-    uint32_t e2;
+    uint4 c[2][2];
+    uint32_t e[2];
 };
 
-__device__ __forceinline__ void load_step(Step &st, const uint8_t *codes, const Weights &w, int64_t mrow, int64_t n0, int64_t k, int64_t groups) {
-    const int g = (threadIdx.x & 31) >> 2;
-    st.e = st.e2 = 0;
+// code[i], e[i]: the lane's rows (code null beyond N); k: its first value in this step.
+__device__ __forceinline__ void load_step(Step &st, const Weights &w, const uint8_t *const (&code)[2], const uint8_t *const (&e)[2], int64_t k) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t n = n0 + g + 8 * i;
-        const uint8_t *c = codes + ((mrow + n) * w.K + k) / 2;
-        const uint8_t *e = w.scales + (mrow + n) * groups;
-        uint32_t eb = 0;
+    for (int i = 0; i < 2; ++i) {
+        const bool in = code[i] != nullptr;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const bool in = n < w.N && k + 32 * p < w.K;
-            st.c[i][p] = in ? __ldg(reinterpret_cast<const uint4 *>(c) + p) : make_uint4(0, 0, 0, 0);
-            eb |= in ? uint32_t(__ldg(e + ((k + 32 * p) >> w.gshift))) << (8 * p) : 0u;
-        }
-        if (i < 2) st.e |= eb << (16 * i);
-        else st.e2 |= eb << (16 * (i - 2));
+        for (int p = 0; p < 2; ++p)
+            st.c[i][p] = in && k + 32 * p < w.K ? __ldg(reinterpret_cast<const uint4 *>(code[i] + (k >> 1)) + p) : make_uint4(0, 0, 0, 0);
+        st.e[i] = in ? scale_pair(w, e[i], k) : 0u;
     }
 }
 
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2)
 q4_few_kernel(const void *x, int64_t ldx, const uint8_t *codes, Runs runs, Weights w, Out o, int section) {
     using T = typename Halves<BF16>::T;
     extern __shared__ __align__(16) uint8_t few_smem[];   // the rows of a section of k, then the warps' sums
     const unsigned sx = tc5::smem_addr(few_smem);
     float *const sums = reinterpret_cast<float *>(few_smem);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane & 3, tok = lane >> 2;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane & 3, tok = lane >> 2, m = warp & 1, part = warp >> 1;
     const int64_t groups = w.K >> w.gshift;
     Finder find;
     find.start(runs);
     Tile t;
     for (int64_t tile = blockIdx.x; find.find(runs, tile, t); tile += gridDim.x) {
         const int64_t n0 = int64_t(t.wt) * kFewRows, mrow = t.mat * w.N;
-        float acc[2][NT][4] = {};
+        float acc[NT][4] = {};
+        const uint8_t *code[2], *ebase[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int64_t n = n0 + 16 * m + tok + 8 * i;
+            code[i] = n < w.N ? codes + ((mrow + n) * w.K) / 2 : nullptr;
+            ebase[i] = w.scales + (mrow + min(n, w.N - 1)) * groups;
+        }
         for (int64_t sec = 0; sec < w.K; sec += section) {
             const int len = int(min(w.K - sec, int64_t(section))), steps = (len + 255) >> 8;
-            Step cur;
-            int s = warp;
-            if (s < steps) load_step(cur, codes, w, mrow, n0, sec + s * 256 + q * 64, groups);
+            Step cur, next;
+            int s = part;
+            if (s < steps) load_step(cur, w, code, ebase, sec + s * 256 + q * 64);
+            if (s + kFewParts < steps) load_step(next, w, code, ebase, sec + (s + kFewParts) * 256 + q * 64);
             // rows into shared memory: 64 values a line, its eight pieces swizzled by the line's place in a step and the row
             __syncthreads();
             const int pieces = steps * 32;
@@ -549,71 +651,60 @@ q4_few_kernel(const void *x, int64_t ldx, const uint8_t *codes, Runs runs, Weigh
                 }
             }
             __syncthreads();
-            for (; s < steps; s += kFewWarps) {
-                Step next;
-                if (s + kFewWarps < steps) load_step(next, codes, w, mrow, n0, sec + (s + kFewWarps) * 256 + q * 64, groups);
+            unsigned at[NT];      // this lane's line of its rows, at step s
+            bool on[NT];
+#pragma unroll
+            for (int u = 0; u < NT; ++u) {
+                on[u] = tok + 8 * u < t.rows;
+                at[u] = sx + (((tok + 8 * u) * steps + s) * 4 + q) * 128;
+            }
+            const unsigned sw = (q | ((tok & 1) << 2)) << 4;
+            for (; s < steps; s += kFewParts) {
+                const uint32_t eh[2] = {e4m3_pair(cur.e[0]), e4m3_pair(cur.e[1])};
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    uint32_t es[4], ez[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = e4m3_value(uint8_t((i < 2 ? cur.e : cur.e2) >> (16 * (i & 1) + 8 * p)));
-                        es[i] = Halves<BF16>::pair(e);
-                        ez[i] = Halves<BF16>::pair(-24.0f * e);
-                    }
+                    const typename Halves<BF16>::Scale e0 = Halves<BF16>::scale(eh[0], p), e1 = Halves<BF16>::scale(eh[1], p);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        uint4 b[NT];
+                        const uint4 &c0 = cur.c[0][p], &c1 = cur.c[1][p];
+                        uint32_t lo[4], hi[4];
+                        Halves<BF16>::widen8(j == 0 ? c0.x : j == 1 ? c0.y : j == 2 ? c0.z : c0.w, e0, lo);
+                        Halves<BF16>::widen8(j == 0 ? c1.x : j == 1 ? c1.y : j == 2 ? c1.z : c1.w, e1, hi);
+                        const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
                         for (int u = 0; u < NT; ++u) {
-                            const int r = tok + 8 * u, sw = q | ((r & 1) << 2);
-                            b[u] = make_uint4(0, 0, 0, 0);
-                            if (r < t.rows) b[u] = lds128(sx + ((r * steps * 4 + s * 4 + q) * 8 + ((4 * p + j) ^ sw)) * 16);
-                        }
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            uint32_t lo[4], hi[4];
-                            const uint4 &c0 = cur.c[2 * m][p], &c1 = cur.c[2 * m + 1][p];
-                            const uint32_t w0 = j == 0 ? c0.x : j == 1 ? c0.y : j == 2 ? c0.z : c0.w;
-                            const uint32_t w1 = j == 0 ? c1.x : j == 1 ? c1.y : j == 2 ? c1.z : c1.w;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                lo[i] = Halves<BF16>::fma(Halves<BF16>::raw(w0, i), es[2 * m], ez[2 * m]);
-                                hi[i] = Halves<BF16>::fma(Halves<BF16>::raw(w1, i), es[2 * m + 1], ez[2 * m + 1]);
-                            }
-                            const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
-#pragma unroll
-                            for (int u = 0; u < NT; ++u) {
-                                mma16816(acc[m][u], a0, b[u].x, b[u].y, BF16);
-                                mma16816(acc[m][u], a1, b[u].z, b[u].w, BF16);
-                            }
+                            uint4 b = make_uint4(0, 0, 0, 0);
+                            if (on[u]) b = lds128(at[u] + (((4 * p + j) << 4) ^ sw));
+                            mma16816(acc[u], a0, b.x, b.y, BF16);
+                            mma16816(acc[u], a1, b.z, b.w, BF16);
                         }
                     }
                 }
                 cur = next;
+                if (s + 2 * kFewParts < steps) load_step(next, w, code, ebase, sec + (s + 2 * kFewParts) * 256 + q * 64);
+#pragma unroll
+                for (int u = 0; u < NT; ++u) at[u] += kFewParts * 512;
             }
         }
         __syncthreads();
-        // sums[warp][row of x][weight row]
+        // sums[part][row of x][weight row]
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int u = 0; u < NT; ++u)
 #pragma unroll
-            for (int u = 0; u < NT; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    sums[(warp * 8 * NT + 8 * u + 2 * q + (i & 1)) * kFewRows + 16 * m + tok + 8 * (i >> 1)] = acc[m][u][i];
+            for (int i = 0; i < 4; ++i)
+                sums[(part * 8 * NT + 8 * u + 2 * q + (i & 1)) * kFewRows + 16 * m + tok + 8 * (i >> 1)] = acc[u][i];
         __syncthreads();
         const float scale = __ldg(w.scale + t.mat);
         for (int i = tid; i < 8 * NT * kFewRows; i += 256) {
             const int r = i / kFewRows, c = i % kFewRows;
             float v = 0.0f;
 #pragma unroll
-            for (int k = 0; k < kFewWarps; ++k) v += sums[(k * 8 * NT + r) * kFewRows + c];
+            for (int k = 0; k < kFewParts; ++k) v += sums[(k * 8 * NT + r) * kFewRows + c];
             if (r < t.rows && n0 + c < w.N) static_cast<T *>(o.out)[(t.row0 + r) * o.ld + n0 + c] = from_float<T>(scale * v);
         }
         __syncthreads();
     }
-    if (o.zero_rest && runs.offsets) zero_rows<T>(o, find.begin, find.end(runs));
+    if (o.zero_rest && runs.offsets) zero_rows<T>(o, find.begin, find.end(runs), 256);
 }
 
 // The parts of a split contraction, added in their order.
@@ -631,17 +722,19 @@ __global__ void __launch_bounds__(256) q4_join_parts_kernel(const float *part, i
 // ----------------------------------------------------------------------------
 // Gradient of the group scales: dW = dy^T x over the rows of a matrix, reduced
 // with the codes before it leaves the chip (a 32nd to a 256th of dW is written).
-// One tile: 128 rows n by 256 columns k; both operands come as lines of 64
-// columns, one line per row t, in stages of 64 rows.  The sums of kPromote
+// One tile of a pair of CTAs: 256 rows n (128 each) by 256 columns k (each brings
+// half); both operands come as lines of 64 columns, one line per row t, in stages
+// of 64 rows.  The sums of kPromote
 // stages are taken from tensor memory (two accumulators in turn), multiplied by
 // q and added in float32 registers, so that no long sum runs in the tensor core.
-// Warps 0 .. 7 reduce, warp 8 copies, warp 9 issues, warp 10 clears the rows
-// behind the last one of a run (they are another matrix's, and may be NaN).
+// Warps 0 .. 7 reduce, warp 8 copies, warp 9 issues (first CTA), warp 10 clears the
+// rows behind the last one of a run (they are another matrix's, and may be NaN)
+// and tells the first CTA that the stage is there.
 // ----------------------------------------------------------------------------
-constexpr int kPromote = 8, kBand = 12;
+constexpr int kPromote = 8, kBand = 8, kDsThreads = 352;
 
 struct DsCfg {
-    static constexpr int NS = 4, kA = 16384, kB = 32768, kBar = 3 * NS + 4;
+    static constexpr int NS = 6, kA = 16384, kB = 16384, kBar = 3 * NS + 4;
     static constexpr int kSmem = 1024 + NS * (kA + kB) + kBar * 8 + 32 + 512;
 };
 
@@ -695,7 +788,7 @@ struct DsFinder {
 };
 
 template <bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kDsThreads, 1)
 q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_constant__ CUtensorMap map_x, Runs runs, const uint8_t *codes, int64_t N,
                  int64_t K, int gshift, int ntiles, int ktiles, float *dc) {
     using C = DsCfg;
@@ -703,23 +796,25 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     extern __shared__ uint8_t smem_raw[];
     const unsigned base = (tc5::smem_addr(smem_raw) + 1023u) & ~1023u;
     const unsigned sa = base, sb = sa + NS * C::kA, bars = sb + NS * C::kB;
-    const unsigned full = bars, fixed = full + 8 * NS, empty = fixed + 8 * NS, done = empty + 8 * NS, drained = done + 16, misc = drained + 16;
+    const unsigned full = bars, ready = full + 8 * NS, empty = ready + 8 * NS, done = empty + 8 * NS, drained = done + 16, misc = drained + 16;
     uint8_t *const misc_ptr = smem_raw + (misc - tc5::smem_addr(smem_raw));
     volatile int *gave_up = reinterpret_cast<volatile int *>(misc_ptr + 4);
     const unsigned sums_full = misc + 16, sums_empty = misc + 24;
     float *const other = reinterpret_cast<float *>(misc_ptr + 32);   // 128 sums of the second half
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = tc5::warp_id(), lane = threadIdx.x & 31;
+    const unsigned rank = tc5::pair_rank();
+    const int64_t step = gridDim.x >> 1, first = blockIdx.x >> 1;   // pairs
     if (warp == 9) tc5::tmem_alloc<512>(misc);
     if (threadIdx.x == 0) {
         *gave_up = 0;
         for (int i = 0; i < NS; ++i) {
             tma::mbar_init(full + 8 * i, 1);
-            tma::mbar_init(fixed + 8 * i, 1);
-            tma::mbar_init(empty + 8 * i, 2);
+            tma::mbar_init(ready + 8 * i, 2);
+            tma::mbar_init(empty + 8 * i, 1);
         }
         for (int i = 0; i < 2; ++i) {
             tma::mbar_init(done + 8 * i, 1);
-            tma::mbar_init(drained + 8 * i, 8);
+            tma::mbar_init(drained + 8 * i, 16);
         }
         tma::mbar_init(misc + 8, 1);
         tma::mbar_init(sums_full, 4);
@@ -728,9 +823,11 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     }
     tc5::fence_before();
     __syncthreads();
+    tc5::pair_sync();
     tc5::fence_after();
     unsigned tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(misc));
+    tmem = __shfl_sync(0xffffffffu, tmem, 0);
 
     tc5::Waiter wt{gave_up, &g_mm_timeout};
     DsFinder find;
@@ -738,7 +835,7 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     unsigned it = 0, part = 0;   // stages, promoted parts so far
 
     if (warp == 8) {
-        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x) {
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += step) {
             const int n = int((t.rows + 63) / 64);
             for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS;
@@ -747,56 +844,54 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
                     tma::mbar_arrive_expect_tx(full + 8 * slot, C::kA + C::kB);
                     const int row = int(t.lo) + s * 64;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) tma::load2d(sa + slot * C::kA + c * 8192, &map_dy, t.nt * 128 + c * 64, row, full + 8 * slot);
+                    for (int c = 0; c < 2; ++c) tma::load2d(sa + slot * C::kA + c * 8192, &map_dy, t.nt * 256 + int(rank) * 128 + c * 64, row, full + 8 * slot);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tma::load2d(sb + slot * C::kB + c * 8192, &map_x, t.kt * 256 + c * 64, row, full + 8 * slot);
+                    for (int c = 0; c < 2; ++c) tma::load2d(sb + slot * C::kB + c * 8192, &map_x, t.kt * 256 + int(rank) * 128 + c * 64, row, full + 8 * slot);
                 }
             }
         }
         if (wt.fail)
             for (unsigned i = it > NS ? it - NS : 0; i < it; ++i) tc5::Waiter::drain(full + 8 * (i % NS), (i / NS) & 1);
     } else if (warp == 10) {
-        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x) {
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += step) {
             const int n = int((t.rows + 63) / 64);
-            for (int s = 0; s < n; ++s, ++it) {   // every stage, so that no phase of `full` goes by unseen
+            for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS, left = int(min(t.rows - int64_t(s) * 64, int64_t(64)));
                 if (!wt.wait(full + 8 * slot, (it / NS) & 1)) break;
                 if (left & 15) {
                     const int rows = 16 - (left & 15);
-                    for (int i = lane; i < rows * 48; i += 32) {   // 6 blocks of lines, 8 pieces a line
-                        const int l = left + i / 48, b = i % 48;
+                    for (int i = lane; i < rows * 32; i += 32) {   // 4 blocks of lines, 8 pieces a line
+                        const int l = left + i / 32, b = i % 32;
                         const unsigned at = b < 16 ? sa + slot * C::kA + (b >> 3) * 8192 : sb + slot * C::kB + ((b - 16) >> 3) * 8192;
                         sts128(at + l * 128 + (b & 7) * 16, 0, 0, 0, 0);
                     }
                     tma::fence_proxy_async();
                 }
                 __syncwarp();
-                if (lane == 0) {
-                    if (left & 15) tc5::mbar_arrive(fixed + 8 * slot);
-                    tc5::mbar_arrive(empty + 8 * slot);
-                }
+                if (lane == 0) tc5::mbar_arrive_remote(tc5::leader_addr(ready + 8 * slot));
+                __syncwarp();
             }
         }
+    } else if (warp == 9 && rank == 1) {
+        // the first CTA issues for both
     } else if (warp == 9) {
-        unsigned parity = 0;   // bit per slot: of its next clearing
         constexpr uint32_t idesc = tc5::idesc_f16(BF16, 256, true, true);
-        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x) {
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += step) {
             const int n = int((t.rows + 63) / 64);
             for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS;
                 const bool begin = s % kPromote == 0, end = s % kPromote == kPromote - 1 || s + 1 == n;
                 if (begin && !wt.wait(drained + 8 * (part & 1), ((part >> 1) & 1) ^ 1)) break;
-                if (!wt.wait(full + 8 * slot, (it / NS) & 1)) break;
+                if (!wt.wait(ready + 8 * slot, (it / NS) & 1)) break;
                 const int left = int(min(t.rows - int64_t(s) * 64, int64_t(64)));
-                if (left & 15) {
-                    if (!wt.wait(fixed + 8 * slot, (parity >> slot) & 1)) break;
-                    parity ^= 1u << slot;
-                }
                 tc5::fence_after();
-                if (lane == 0) {
-                    const uint64_t a = tc5::desc128(sa + slot * C::kA, 8192, 1024), b = tc5::desc128(sb + slot * C::kB, 8192, 1024);
-                    const int steps = (left + 15) >> 4;
-                    for (int k = 0; k < steps; ++k) tc5::mma_ss(tmem + (part & 1) * 256, a + k * 128, b + k * 128, idesc, !begin || k > 0);
+                const uint64_t a = tc5::desc128(sa + slot * C::kA, 8192, 1024), b = tc5::desc128(sb + slot * C::kB, 8192, 1024);
+                const int steps = (left + 15) >> 4;
+                const unsigned d = tmem + (part & 1) * 256;
+                if (tc5::elect()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (k < steps) tc5::mma_ss(d, a + k * 128, b + k * 128, idesc, !begin || k > 0);
                     tc5::commit(empty + 8 * slot);
                     if (end) tc5::commit(done + 8 * (part & 1));
                 }
@@ -805,7 +900,7 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
             }
         }
         if (wt.fail) {
-            if (lane == 0) tc5::commit(misc + 8);
+            if (tc5::elect()) tc5::commit(misc + 8);
             __syncwarp();
             tc5::Waiter::drain(misc + 8, 0);
         }
@@ -813,9 +908,9 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
         const int half = warp >> 2, quad = warp & 3;
         const int64_t groups = K >> gshift;
         unsigned tiles = 0;
-        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += gridDim.x, ++tiles) {
+        for (int64_t tile = first; !wt.fail && find.find(runs, tile, ntiles, ktiles, t); tile += step, ++tiles) {
             const int parts = int((t.rows + 64 * kPromote - 1) / (64 * kPromote));
-            const int64_t n = int64_t(t.nt) * 128 + quad * 32 + lane, k0 = int64_t(t.kt) * 256 + half * 128;
+            const int64_t n = int64_t(t.nt) * 256 + rank * 128 + quad * 32 + lane, k0 = int64_t(t.kt) * 256 + half * 128;
             uint4 code[4];
             float sum[4] = {};
 #pragma unroll
@@ -843,7 +938,7 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
                 }
                 tc5::fence_before();
                 __syncwarp();
-                if (lane == 0) tc5::mbar_arrive(drained + 8 * (part & 1));
+                if (lane == 0) tc5::mbar_arrive_remote(tc5::leader_addr(drained + 8 * (part & 1)));
             }
             if (wt.fail) break;
             float *const row = dc + (t.mat * N + n) * groups;
@@ -873,7 +968,9 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
             }
         }
     }
+    tc5::fence_before();
     __syncthreads();
+    tc5::pair_sync();   // the other CTA's products read this one's memory, its warps arrive here
     if (warp == 9) {
         tc5::fence_after();
         tc5::tmem_free<512>(tmem);
@@ -905,7 +1002,7 @@ struct Plan {
     int width;        // BT of the kernel
     int bt;           // rows of a tile
     int splits;
-    int64_t tiles;    // at most
+    int64_t tiles;    // at most, of a pair of CTAs
 };
 
 // J result columns, `depth` contraction steps.
@@ -915,13 +1012,15 @@ Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
     p.width = each <= 64 ? 64 : each <= 128 ? 128 : 256;
     p.bt = p.width;
     p.splits = 1;
-    const int64_t wt = (J + 127) / 128;
+    const int64_t wt = (J + 255) / 256;
     const int64_t rt = runs ? std::min(T, T / p.bt + mats) : (T + p.bt - 1) / p.bt;
     p.tiles = rt * wt;
-    const int sms = uq::num_sms();
-    if (!runs && p.tiles * 2 <= sms) {
+    const int pairs = uq::num_sms() / 2;
+    if (!runs && p.tiles * 2 <= pairs) {
         const int64_t chunks = (depth + 255) / 256;
-        p.splits = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(sms / p.tiles, chunks / 2), 16)));
+        p.splits = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(pairs / p.tiles, chunks / 2), 16)));
+        const int64_t each_part = (chunks + p.splits - 1) / p.splits;
+        p.splits = int((chunks + each_part - 1) / each_part);   // no part is empty
         p.tiles *= p.splits;
     }
     return p;
@@ -941,7 +1040,7 @@ int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, co
         !tc5::encode2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, uint64_t(w.K / 2), uint64_t(mats * w.N), uint64_t(w.K / 2), DX ? 64 : 128,
                        DX ? 256 : 128, DX ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B))
         return uq::fail(UQ_ERR_CUDA, "tensor map of a 4-bit product");
-    const int grid = int(std::min<int64_t>(tiles, uq::num_sms()));
+    const int grid = 2 * int(std::min<int64_t>(tiles, uq::num_sms() / 2));
     uq::ProfScope _p(DX ? "q4_dx" : "q4_linear", st);
     kernel<<<grid, kThreads, C::kSmem, st>>>(mr, mc, r, w, o);
     return uq::check_cuda("q4_product_kernel launch");
@@ -957,7 +1056,7 @@ int few(const void *x, int64_t ldx, int64_t T, const uint8_t *codes, const Weigh
     auto kernel = q4_few_kernel<BF16, NT>;
     const int64_t rows = std::min<int64_t>(T, 8 * NT), wide = (w.K + 255) / 256 * 256;
     const int section = int(std::min<int64_t>(wide, 98304 / (2 * rows) / 256 * 256));
-    const int smem = int(std::max<int64_t>(rows * section * 2, kFewWarps * 8 * NT * kFewRows * 4));
+    const int smem = int(std::max<int64_t>(rows * section * 2, kFewParts * 8 * NT * kFewRows * 4));
     if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), 98304) != cudaSuccess) return uq::check_cuda("q4_few_kernel attribute");
     const Runs r{offsets, T, mats, 8 * NT, int((w.N + kFewRows - 1) / kFewRows), 1};
     const Out o{y, ldy, w.N, T, zero};
@@ -974,7 +1073,7 @@ int product(const void *rows, int64_t lda, int64_t T, const uint8_t *codes, cons
     const Plan p = plan_for(T, mats, offsets != nullptr, J, depth);
     if (p.splits > 1 && (!ws || ws_bytes < size_t(p.splits) * T * J * 4))
         return uq::fail(UQ_ERR_WORKSPACE, "4-bit product: workspace of %zu bytes, %zu needed", ws_bytes, size_t(p.splits) * T * J * 4);
-    const Runs r{offsets, T, mats, p.bt, int((J + 127) / 128), p.splits};
+    const Runs r{offsets, T, mats, p.bt, int((J + 255) / 256), p.splits};
     const Out o{p.splits > 1 ? ws : out, ldo, J, T, zero};
     int rc = p.width == 64    ? launch<64, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st)
              : p.width == 128 ? launch<128, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st)
@@ -997,10 +1096,10 @@ int dscale(const void *dy, const void *x, int64_t T, int64_t lddy, int64_t ldx, 
         !tc5::encode2d(&mx, ty, x, uint64_t(K), uint64_t(T), uint64_t(ldx) * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B))
         return uq::fail(UQ_ERR_CUDA, "tensor map of the scales' gradient");
     const Runs r{offsets, T, mats, 0, 0, 1};
-    const int ntiles = int((N + 127) / 128), ktiles = int((K + 255) / 256);
-    const int grid = int(std::min<int64_t>(mats * ntiles * int64_t(ktiles), uq::num_sms()));
+    const int ntiles = int((N + 255) / 256), ktiles = int((K + 255) / 256);
+    const int grid = 2 * int(std::min<int64_t>(mats * ntiles * int64_t(ktiles), uq::num_sms() / 2));
     uq::ProfScope _p("q4_dscale", st);
-    kernel<<<grid, kThreads, DsCfg::kSmem, st>>>(md, mx, r, codes, N, K, uq::ilog2(group), ntiles, ktiles, dc);
+    kernel<<<grid, kDsThreads, DsCfg::kSmem, st>>>(md, mx, r, codes, N, K, uq::ilog2(group), ntiles, ktiles, dc);
     return uq::check_cuda("q4_dscale_kernel launch");
 }
 

@@ -10,13 +10,45 @@ namespace tc5 {
 
 __device__ __forceinline__ unsigned smem_addr(const void *p) { return unsigned(__cvta_generic_to_shared(p)); }
 
-// ---- tensor memory -----------------------------------------------------------
-template <int COLS> __device__ __forceinline__ void tmem_alloc(unsigned dst) {   // one whole warp
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(dst), "n"(COLS) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// Everything here works on pairs of CTAs (cta_group::2): one product of M = 256
+// takes 128 rows of A from each CTA and half of B's N columns from each, and
+// leaves 128 rows of D in each, so that every byte of B crosses from L2 once for
+// 256 rows.
+
+// ---- the pair --------------------------------------------------------------------
+__device__ __forceinline__ unsigned pair_rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
-template <int COLS> __device__ __forceinline__ void tmem_free(unsigned addr) {   // the warp that allocated
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "n"(COLS));
+// The first CTA's address of a place in shared memory (for mbarrier arrivals).
+__device__ __forceinline__ unsigned leader_addr(unsigned addr) {
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Warp number, the same in all lanes in a way that the compiler sees: a product's
+// operands are uniform registers, and in code that it takes for divergent every
+// one of them is fetched by a loop over lanes (115 cycles a product).
+__device__ __forceinline__ int warp_id() { return __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0); }
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect() {
+    unsigned r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// ---- tensor memory -----------------------------------------------------------
+template <int COLS> __device__ __forceinline__ void tmem_alloc(unsigned dst) {   // one whole warp of each CTA
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(dst), "n"(COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+template <int COLS> __device__ __forceinline__ void tmem_free(unsigned addr) {   // the warps that allocated
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(addr), "n"(COLS));
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -44,10 +76,10 @@ __device__ __forceinline__ void st32(unsigned addr, const uint32_t (&r)[32]) {
 
 // ---- products ------------------------------------------------------------------
 // Instruction descriptor of kind::f16: float32 sums, both operands of one type,
-// M = 128.  `amn`, `bmn`: the operand's M (N) index is the contiguous one.
+// M = 256, n a multiple of 32.  `amn`, `bmn`: the operand's M (N) index is the contiguous one.
 __device__ __forceinline__ constexpr uint32_t idesc_f16(bool bf16, int n, bool amn, bool bmn) {
     return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(amn) << 15) | (uint32_t(bmn) << 16) |
-           (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+           (uint32_t(n >> 3) << 17) | (uint32_t(256 >> 4) << 24);
 }
 // Shared-memory descriptor with the 128-byte swizzle.  Contraction index
 // contiguous: rows of 128 bytes, 8 rows (1024 bytes) apart by `stride`.  M / N
@@ -61,17 +93,19 @@ __device__ __forceinline__ uint64_t desc128(unsigned addr, unsigned lead, unsign
 // tensor memory or in shared memory.
 __device__ __forceinline__ void mma_ts(unsigned d, unsigned a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
 }
 __device__ __forceinline__ void mma_ss(unsigned d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
 }
-// Arrives on an mbarrier once every product issued so far by this thread is done.
+// Arrives on the mbarrier at this place in both CTAs once every product issued so
+// far by this thread is done.
 __device__ __forceinline__ void commit(unsigned mbar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(mbar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                 :: "r"(mbar), "h"((unsigned short)3) : "memory");
 }
 
 // ---- waits ---------------------------------------------------------------------
@@ -83,6 +117,15 @@ __device__ __forceinline__ bool mbar_test(unsigned addr, unsigned parity) {
 }
 __device__ __forceinline__ void mbar_arrive(unsigned addr) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(addr) : "memory");
+}
+
+// At a barrier of either CTA.  What it announces is read by the tensor cores, not
+// by the waiting thread: tensor memory (after fence_before) or shared memory
+// (after fence.proxy.async), complete in the CTA that wrote it.  So the default,
+// block-scope order is enough; release.cluster here and acquire.cluster at every
+// wait halved the rate of all three products.
+__device__ __forceinline__ void mbar_arrive_remote(unsigned cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
 }
 
 // A block's waits, each by a whole warp and at most 2 s long: the first that
