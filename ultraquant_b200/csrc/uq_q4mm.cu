@@ -179,10 +179,10 @@ template <bool BF16> __device__ __forceinline__ void widen32(const uint4 &c, con
     Halves<BF16>::widen8(c.w, s, out + 12);
 }
 
-__device__ __forceinline__ uint4 lds128(unsigned addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-    return v;
+// A plain load (not asm), so that the compiler may order it among the arithmetic
+// but not across a barrier.
+__device__ __forceinline__ uint4 lds128(const uint8_t *smem, unsigned smem_at, unsigned addr) {
+    return *reinterpret_cast<const uint4 *>(smem + (addr - smem_at));
 }
 __device__ __forceinline__ void sts128(unsigned addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -330,13 +330,13 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     using C = Cfg<BT, DX>;
     constexpr int NS = C::NS, NC = C::kChunks, kBox = BT / 4;   // rows of one copy: half of a CTA's share
     extern __shared__ uint8_t smem_raw[];
-    const unsigned base = (tc5::smem_addr(smem_raw) + 1023u) & ~1023u;
+    const unsigned smem_at = tc5::smem_addr(smem_raw), base = (smem_at + 1023u) & ~1023u;
     const unsigned sb = base, sa = sb + NS * C::kB, sc = sa + NS * C::kA, bars = sc + NC * C::kC;
     const unsigned full_b = bars, full_a = bars + 8 * NS, empty = bars + 16 * NS, full_p = bars + 24 * NS, full_c = bars + 32 * NS,
                    empty_c = full_c + 8 * NC, done = empty_c + 8 * NC, drained = done + 8, misc = drained + 8;
     volatile int *gave_up = reinterpret_cast<volatile int *>(smem_raw + (misc + 4 - tc5::smem_addr(smem_raw)));
     const int warp = tc5::warp_id(), lane = threadIdx.x & 31;
-    const unsigned rank = tc5::pair_rank();
+    const unsigned rank = tc5::cluster_rank();
     if (warp == kWiden + 2) tc5::tmem_alloc<512>(misc);
     if (threadIdx.x == 0) {
         *gave_up = 0;
@@ -357,7 +357,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     }
     tc5::fence_before();
     __syncthreads();
-    tc5::pair_sync();
+    tc5::cluster_sync();
     tc5::fence_after();
     unsigned tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(misc));
@@ -504,7 +504,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                         const unsigned line = sa + slot * C::kA + h * 8192 + ((quad & 1) * 32 + lane) * 128;
                         uint4 code[2];
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) code[p] = lds128(sc + cslot * C::kC + rr * 64 + (((2 * h + p) ^ ((rr >> 1) & 3)) << 4));
+                        for (int p = 0; p < 2; ++p) code[p] = lds128(smem_raw, smem_at, sc + cslot * C::kC + rr * 64 + (((2 * h + p) ^ ((rr >> 1) & 3)) << 4));
                         if (!wt.wait(empty + 8 * slot, par0 ^ wrap)) break;
 #pragma unroll
                         for (int p = 0; p < 2; ++p) {
@@ -519,7 +519,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                         const int rr = quad * 32 + lane;
                         uint32_t v[32];
 #pragma unroll
-                        for (int p = 0; p < 2; ++p) widen32<BF16>(lds128(sc + cslot * C::kC + rr * 128 + (((2 * stage + p) ^ (rr & 7)) << 4)), e[p], v + 16 * p);
+                        for (int p = 0; p < 2; ++p) widen32<BF16>(lds128(smem_raw, smem_at, sc + cslot * C::kC + rr * 128 + (((2 * stage + p) ^ (rr & 7)) << 4)), e[p], v + 16 * p);
                         if (!wt.wait(empty + 8 * slot, par0 ^ wrap)) break;
                         tc5::fence_after();
                         tc5::st32(tmem_a + slot * 32 + (unsigned(quad * 32) << 16), v);
@@ -565,7 +565,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     }
     tc5::fence_before();
     __syncthreads();
-    tc5::pair_sync();   // the other CTA's products read this one's memory, its warps arrive here
+    tc5::cluster_sync();   // the other CTA's products read this one's memory, its warps arrive here
     if (warp == kWiden + 2) {
         tc5::fence_after();
         tc5::tmem_free<512>(tmem);
@@ -573,138 +573,201 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
 }
 
 // ----------------------------------------------------------------------------
-// Few rows: bound by reading the codes once.  A block takes 32 weight rows; its
-// eight warps take 16 rows and every fourth step of 256 values of k each, two
-// steps' loads ahead, and add up in shared memory at the end.  The widened codes are operand
-// A of m16n8k16 products straight from registers: the contraction order is free
-// as long as both operands agree, so lane quarter q takes 64 consecutive values
-// of a row (two 16-byte loads) where the instruction says "columns 2 q, 2 q + 1,
-// 2 q + 8, 2 q + 9".  Widening costs the same for 1 row as for 8.
+// Few rows: bound by reading the codes once, and next to that by the
+// instructions that widen them (11 a word of 8; the integer ones have a half-rate
+// pipe, 14 cycles of the 23 that memory gives a warp's 256 codes).  A block takes
+// 128 weight rows, 16 for each of eight warps; a ninth copies chunks of 256 values
+// of k, codes and rows, into a ring (TMA), so that three blocks an SM keep 144 KB
+// on the way.  Where there are few tiles a cluster of 2, 4 or 8 blocks shares one,
+// each a part of k, and adds up through distributed shared memory.  The widened
+// codes are operand A of m16n8k16 products straight from registers: the
+// contraction order is free as long as both operands agree, so lane quarter q
+// takes 64 consecutive values of a row (two 16-byte pieces) where the instruction
+// says "columns 2 q, 2 q + 1, 2 q + 8, 2 q + 9".  Widening costs the same for 1 row
+// as for 8.  (With A in tensor memory a product of 16 steps takes 118 cycles
+// however few rows there are: 3 times the time that memory needs.)
 // ----------------------------------------------------------------------------
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool bf16) {
     if (bf16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-constexpr int kFewParts = 4, kFewRows = 32;
+constexpr int kFewWarps = 8, kFewRows = 128, kFewThreads = (kFewWarps + 1) * 32;
 
-// One lane's codes and scales of a step: 64 values of 2 rows (g, g + 8).
-struct Step {
-    uint4 c[2][2];
-    uint32_t e[2];
+// NT: blocks of 8 rows.  A quarter of a chunk's rows is one copy of up to 8 NT
+// lines of 64 values; each quarter begins two lines further round the 128-byte
+// swizzle, so that the four lanes of a row read different banks.
+template <int NT> struct FewCfg {
+    static constexpr int NS = NT == 1 ? 3 : 4, kBlocks = NT == 1 ? 3 : 2;     // stages, blocks an SM
+    static constexpr int kC = 16384, kQuarter = 8 * NT * 128 + 256, kX = 4 * kQuarter, kStage = kC + kX;
+    static constexpr int kSums = kFewRows * 8 * NT * 4;                       // of one block, for its cluster
+    static constexpr int kSmem = 1024 + NS * kStage + kSums + NS * 16 + 16;
+    static_assert(kStage % 1024 == 0 && kBlocks * (kSmem + 1024) <= 233472, "shared memory of an SM");
 };
 
-// code[i], e[i]: the lane's rows (code null beyond N); k: its first value in this step.
-__device__ __forceinline__ void load_step(Step &st, const Weights &w, const uint8_t *const (&code)[2], const uint8_t *const (&e)[2], int64_t k) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const bool in = code[i] != nullptr;
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-            st.c[i][p] = in && k + 32 * p < w.K ? __ldg(reinterpret_cast<const uint4 *>(code[i] + (k >> 1)) + p) : make_uint4(0, 0, 0, 0);
-        st.e[i] = in ? scale_pair(w, e[i], k) : 0u;
-    }
-}
-
 template <bool BF16, int NT>
-__global__ void __launch_bounds__(256, NT == 1 ? 3 : 2)
-q4_few_kernel(const void *x, int64_t ldx, const uint8_t *codes, Runs runs, Weights w, Out o, int section) {
+__global__ void __launch_bounds__(kFewThreads, FewCfg<NT>::kBlocks)
+q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_codes, Runs runs, Weights w, Out o, int box) {
     using T = typename Halves<BF16>::T;
-    extern __shared__ __align__(16) uint8_t few_smem[];   // the rows of a section of k, then the warps' sums
-    const unsigned sx = tc5::smem_addr(few_smem);
-    float *const sums = reinterpret_cast<float *>(few_smem);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane & 3, tok = lane >> 2, m = warp & 1, part = warp >> 1;
-    const int64_t groups = w.K >> w.gshift;
+    using C = FewCfg<NT>;
+    constexpr int NS = C::NS;
+    extern __shared__ uint8_t smem_raw[];
+    const unsigned smem_at = tc5::smem_addr(smem_raw), base = (smem_at + 1023u) & ~1023u, sums_at = base + NS * C::kStage, full = sums_at + C::kSums, empty = full + 8 * NS, misc = empty + 8 * NS;
+    volatile int *gave_up = reinterpret_cast<volatile int *>(smem_raw + (misc - smem_at));
+    const int warp = tc5::warp_id(), lane = threadIdx.x & 31;
+    const int parts = runs.splits, part = parts > 1 ? int(tc5::cluster_rank()) : 0;   // blocks of a cluster: parts of k
+    if (threadIdx.x == 0) {
+        *gave_up = 0;
+        for (int i = 0; i < NS; ++i) {
+            tma::mbar_init(full + 8 * i, 1);
+            tma::mbar_init(empty + 8 * i, kFewWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    tc5::Waiter wt{gave_up, &g_mm_timeout};
     Finder find;
     find.start(runs);
     Tile t;
-    for (int64_t tile = blockIdx.x; find.find(runs, tile, t); tile += gridDim.x) {
-        const int64_t n0 = int64_t(t.wt) * kFewRows, mrow = t.mat * w.N;
-        float acc[NT][4] = {};
-        const uint8_t *code[2], *ebase[2];
+    const int chunks = int((w.K + 255) >> 8), c0 = int(int64_t(chunks) * part / parts), c1 = int(int64_t(chunks) * (part + 1) / parts);
+    unsigned slot = 0, phase = 0;
+
+    if (warp == kFewWarps) {
+        unsigned n = 0;
+        for (int64_t tile = blockIdx.x; !wt.fail && find.find(runs, tile, t); tile += gridDim.x) {
+            const int row = int(t.mat * w.N + int64_t(t.wt) * kFewRows);
+            for (int c = c0; c < c1; ++c, ++n) {
+                if (!wt.wait(empty + 8 * slot, phase ^ 1)) break;
+                if (tc5::elect()) {
+                    const unsigned at = base + slot * C::kStage, bar = full + 8 * slot;
+                    tma::mbar_arrive_expect_tx(bar, C::kC + 4 * box * 128);
+                    tma::load2d(at, &map_codes, c * 128, row, bar);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int64_t n = n0 + 16 * m + tok + 8 * i;
-            code[i] = n < w.N ? codes + ((mrow + n) * w.K) / 2 : nullptr;
-            ebase[i] = w.scales + (mrow + min(n, w.N - 1)) * groups;
-        }
-        for (int64_t sec = 0; sec < w.K; sec += section) {
-            const int len = int(min(w.K - sec, int64_t(section))), steps = (len + 255) >> 8;
-            Step cur, next;
-            int s = part;
-            if (s < steps) load_step(cur, w, code, ebase, sec + s * 256 + q * 64);
-            if (s + kFewParts < steps) load_step(next, w, code, ebase, sec + (s + kFewParts) * 256 + q * 64);
-            // rows into shared memory: 64 values a line, its eight pieces swizzled by the line's place in a step and the row
-            __syncthreads();
-            const int pieces = steps * 32;
-            for (int r = 0; r < t.rows; ++r) {
-                const T *src = static_cast<const T *>(x) + (t.row0 + r) * ldx + sec;
-                for (int p = tid; p < pieces; p += 256) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (p * 8 < len) v = __ldg(reinterpret_cast<const uint4 *>(src + p * 8));
-                    const int line = p >> 3, sw = (line & 3) | ((r & 1) << 2);
-                    sts128(sx + ((r * steps * 4 + line) * 8 + ((p & 7) ^ sw)) * 16, v.x, v.y, v.z, v.w);
+                    for (int q = 0; q < 4; ++q) tma::load2d(at + C::kC + q * C::kQuarter, &map_rows, c * 256 + q * 64, t.row0, bar);
                 }
+                __syncwarp();
+                if (++slot == NS) { slot = 0; phase ^= 1; }
             }
-            __syncthreads();
-            unsigned at[NT];      // this lane's line of its rows, at step s
-            bool on[NT];
+        }
+        if (wt.fail)   // copies in flight land before the block ends
+            for (unsigned i = n > NS ? n - NS : 0; i < n; ++i) tc5::Waiter::drain(full + 8 * (i % NS), (i / NS) & 1);
+    } else {
+        const int q = lane & 3, g = lane >> 2;
+        const int64_t groups = w.K >> w.gshift;
+        Tile next;
+        bool more = find.find(runs, blockIdx.x, next);
+        const uint8_t *e0 = nullptr, *e1 = nullptr;      // this lane's two rows of scales; beyond N the last row's, not written
+        uint32_t eraw[2];
+        auto scales_of = [&](const Tile &tt) {
+            const int64_t n = int64_t(tt.wt) * kFewRows + warp * 16 + g;
+            e0 = w.scales + (tt.mat * w.N + min(n, w.N - 1)) * groups;
+            e1 = w.scales + (tt.mat * w.N + min(n + 8, w.N - 1)) * groups;
+        };
+        auto scales_at = [&](int c) {
+            const int64_t k = int64_t(c) * 256 + q * 64;
+            eraw[0] = scale_pair(w, e0, k);
+            eraw[1] = scale_pair(w, e1, k);
+        };
+        if (more) {
+            scales_of(next);
+            scales_at(c0);
+        }
+        for (int64_t tile = blockIdx.x; more && !wt.fail; tile += gridDim.x) {
+            t = next;
+            more = find.find(runs, tile + gridDim.x, next);
+            float acc[2][NT][4] = {};   // two sums each, so that a product need not wait for the one before
+            unsigned tok[NT];           // this lane's row of x (of one that is not there: the last one's)
 #pragma unroll
-            for (int u = 0; u < NT; ++u) {
-                on[u] = tok + 8 * u < t.rows;
-                at[u] = sx + (((tok + 8 * u) * steps + s) * 4 + q) * 128;
-            }
-            const unsigned sw = (q | ((tok & 1) << 2)) << 4;
-            for (; s < steps; s += kFewParts) {
-                const uint32_t eh[2] = {e4m3_pair(cur.e[0]), e4m3_pair(cur.e[1])};
+            for (int u = 0; u < NT; ++u) tok[u] = min(g + 8 * u, t.rows - 1);
+            for (int c = c0; c < c1; ++c) {
+                const uint32_t eh[2] = {e4m3_pair(eraw[0]), e4m3_pair(eraw[1])};
+                if (c + 1 < c1) {
+                    scales_at(c + 1);
+                } else if (more) {   // the next tile's
+                    scales_of(next);
+                    scales_at(c0);
+                }
+                if (!wt.wait(full + 8 * slot, phase)) break;
+                const uint8_t *const stage = smem_raw + (base + slot * C::kStage - smem_at);
+                // rows g and g + 8 of the warp's 16 (the same swizzle): pieces 2 q, 2 q + 1
+                const uint8_t *const code = stage + (warp * 16 + g) * 128;
+                const uint8_t *xs[NT];
+#pragma unroll
+                for (int u = 0; u < NT; ++u) xs[u] = stage + C::kC + q * C::kQuarter + tok[u] * 128;
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    const typename Halves<BF16>::Scale e0 = Halves<BF16>::scale(eh[0], p), e1 = Halves<BF16>::scale(eh[1], p);
+                    const int at = ((2 * q + p) ^ g) << 4;
+                    const uint4 w0 = *reinterpret_cast<const uint4 *>(code + at), w1 = *reinterpret_cast<const uint4 *>(code + 1024 + at);
+                    const typename Halves<BF16>::Scale s0 = Halves<BF16>::scale(eh[0], p), s1 = Halves<BF16>::scale(eh[1], p);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 &c0 = cur.c[0][p], &c1 = cur.c[1][p];
                         uint32_t lo[4], hi[4];
-                        Halves<BF16>::widen8(j == 0 ? c0.x : j == 1 ? c0.y : j == 2 ? c0.z : c0.w, e0, lo);
-                        Halves<BF16>::widen8(j == 0 ? c1.x : j == 1 ? c1.y : j == 2 ? c1.z : c1.w, e1, hi);
+                        Halves<BF16>::widen8(j == 0 ? w0.x : j == 1 ? w0.y : j == 2 ? w0.z : w0.w, s0, lo);
+                        Halves<BF16>::widen8(j == 0 ? w1.x : j == 1 ? w1.y : j == 2 ? w1.z : w1.w, s1, hi);
                         const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
 #pragma unroll
                         for (int u = 0; u < NT; ++u) {
-                            uint4 b = make_uint4(0, 0, 0, 0);
-                            if (on[u]) b = lds128(at[u] + (((4 * p + j) << 4) ^ sw));
-                            mma16816(acc[u], a0, b.x, b.y, BF16);
-                            mma16816(acc[u], a1, b.z, b.w, BF16);
+                            const uint4 b = *reinterpret_cast<const uint4 *>(xs[u] + (((4 * p + j) ^ ((tok[u] + 2 * q) & 7)) << 4));
+                            mma16816(acc[0][u], a0, b.x, b.y, BF16);
+                            mma16816(acc[1][u], a1, b.z, b.w, BF16);
                         }
                     }
                 }
-                cur = next;
-                if (s + 2 * kFewParts < steps) load_step(next, w, code, ebase, sec + (s + 2 * kFewParts) * 256 + q * 64);
+                __syncwarp();
+                if (lane == 0) tc5::mbar_arrive(empty + 8 * slot);
+                if (++slot == NS) { slot = 0; phase ^= 1; }
+            }
+            if (wt.fail) break;
+            // element i of a lane: row of x 8 u + 2 q + (i & 1), weight row g + 8 (i >> 1)
+            if (parts == 1) {
+                const float scale = __ldg(w.scale + t.mat);
 #pragma unroll
-                for (int u = 0; u < NT; ++u) at[u] += kFewParts * 512;
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int r = 8 * u + 2 * q + (i & 1);
+                        const int64_t n = int64_t(t.wt) * kFewRows + warp * 16 + g + 8 * (i >> 1);
+                        if (r < t.rows && n < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + n] = from_float<T>(scale * (acc[0][u][i] + acc[1][u][i]));
+                    }
+            } else {
+                // sums [row of x][weight row]; one tile a block
+                float *const sums = reinterpret_cast<float *>(smem_raw + (sums_at - smem_at));
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sums[(8 * u + 2 * q + (i & 1)) * kFewRows + warp * 16 + g + 8 * (i >> 1)] = acc[0][u][i] + acc[1][u][i];
             }
         }
-        __syncthreads();
-        // sums[part][row of x][weight row]
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                sums[(part * 8 * NT + 8 * u + 2 * q + (i & 1)) * kFewRows + 16 * m + tok + 8 * (i >> 1)] = acc[u][i];
-        __syncthreads();
-        const float scale = __ldg(w.scale + t.mat);
-        for (int i = tid; i < 8 * NT * kFewRows; i += 256) {
-            const int r = i / kFewRows, c = i % kFewRows;
-            float v = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kFewParts; ++k) v += sums[(k * 8 * NT + r) * kFewRows + c];
-            if (r < t.rows && n0 + c < w.N) static_cast<T *>(o.out)[(t.row0 + r) * o.ld + n0 + c] = from_float<T>(scale * v);
-        }
-        __syncthreads();
+        if (parts == 1 && o.zero_rest && runs.offsets && !wt.fail) zero_rows<T>(o, find.begin, find.end(runs), kFewWarps * 32);
     }
-    if (o.zero_rest && runs.offsets) zero_rows<T>(o, find.begin, find.end(runs), 256);
+    if (parts > 1) {
+        tc5::cluster_sync();
+        // this block's share of the tile's weight rows, the parts added in their order
+        find.start(runs);
+        if (find.find(runs, blockIdx.x, t)) {
+            const float scale = __ldg(w.scale);
+            const int share = kFewRows / parts;
+            for (int i = threadIdx.x; i < share * t.rows; i += kFewThreads) {
+                const int r = i / share, n = part * share + i % share;
+                float v = 0.0f;
+                for (int p = 0; p < parts; ++p) {
+                    unsigned from;
+                    float f;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(sums_at + (r * kFewRows + n) * 4), "r"(p));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(from) : "memory");
+                    v += f;
+                }
+                const int64_t col = int64_t(t.wt) * kFewRows + n;
+                if (col < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + col] = from_float<T>(scale * v);
+            }
+        }
+        tc5::cluster_sync();   // no block leaves while another reads its sums
+    }
 }
 
 // The parts of a split contraction, added in their order.
@@ -802,7 +865,7 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     const unsigned sums_full = misc + 16, sums_empty = misc + 24;
     float *const other = reinterpret_cast<float *>(misc_ptr + 32);   // 128 sums of the second half
     const int warp = tc5::warp_id(), lane = threadIdx.x & 31;
-    const unsigned rank = tc5::pair_rank();
+    const unsigned rank = tc5::cluster_rank();
     const int64_t step = gridDim.x >> 1, first = blockIdx.x >> 1;   // pairs
     if (warp == 9) tc5::tmem_alloc<512>(misc);
     if (threadIdx.x == 0) {
@@ -823,7 +886,7 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     }
     tc5::fence_before();
     __syncthreads();
-    tc5::pair_sync();
+    tc5::cluster_sync();
     tc5::fence_after();
     unsigned tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(misc));
@@ -970,7 +1033,7 @@ q4_dscale_kernel(const __grid_constant__ CUtensorMap map_dy, const __grid_consta
     }
     tc5::fence_before();
     __syncthreads();
-    tc5::pair_sync();   // the other CTA's products read this one's memory, its warps arrive here
+    tc5::cluster_sync();   // the other CTA's products read this one's memory, its warps arrive here
     if (warp == 9) {
         tc5::fence_after();
         tc5::tmem_free<512>(tmem);
@@ -1053,16 +1116,41 @@ constexpr int64_t kFewMost = 16;
 template <bool BF16, int NT>
 int few(const void *x, int64_t ldx, int64_t T, const uint8_t *codes, const Weights &w, int64_t mats, const int32_t *offsets, void *y, int64_t ldy, bool zero,
         cudaStream_t st) {
+    using C = FewCfg<NT>;
     auto kernel = q4_few_kernel<BF16, NT>;
-    const int64_t rows = std::min<int64_t>(T, 8 * NT), wide = (w.K + 255) / 256 * 256;
-    const int section = int(std::min<int64_t>(wide, 98304 / (2 * rows) / 256 * 256));
-    const int smem = int(std::max<int64_t>(rows * section * 2, kFewParts * 8 * NT * kFewRows * 4));
-    if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), 98304) != cudaSuccess) return uq::check_cuda("q4_few_kernel attribute");
-    const Runs r{offsets, T, mats, 8 * NT, int((w.N + kFewRows - 1) / kFewRows), 1};
+    if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), C::kSmem) != cudaSuccess) return uq::check_cuda("q4_few_kernel attribute");
+    int box = 1;   // rows of a copy
+    while (box < std::min<int64_t>(T, 8 * NT)) box *= 2;
+    CUtensorMap mr, mc;
+    if (!tc5::encode2d(&mr, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, x, uint64_t(w.K), uint64_t(T), uint64_t(ldx) * 2, 64,
+                       box, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !tc5::encode2d(&mc, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, uint64_t(w.K / 2), uint64_t(mats * w.N), uint64_t(w.K / 2), 128, kFewRows,
+                       CU_TENSOR_MAP_SWIZZLE_128B))
+        return uq::fail(UQ_ERR_CUDA, "tensor map of a 4-bit product");
+    const int64_t wtiles = (w.N + kFewRows - 1) / kFewRows, tiles = (offsets ? std::min(T, T / (8 * NT) + mats) : 1) * wtiles;
+    const int64_t slots = int64_t(uq::num_sms()) * C::kBlocks, chunks = (w.K + 255) / 256;
+    // parts of k: least (rounds of blocks) x (chunks of a block, and about three for its start and end)
+    int parts = 1;
+    int64_t best = (tiles + slots - 1) / slots * (chunks + 3);
+    for (int p = 2; p <= 8 && !offsets && p <= chunks; p *= 2) {
+        const int64_t cost = (tiles * p + slots - 1) / slots * ((chunks + p - 1) / p + 3);
+        if (cost < best) { best = cost; parts = p; }
+    }
+    const Runs r{offsets, T, mats, 8 * NT, int(wtiles), parts};
     const Out o{y, ldy, w.N, T, zero};
-    const int64_t tiles = (offsets ? std::min(T, T / (8 * NT) + mats) : 1) * r.wtiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = unsigned(parts > 1 ? tiles * parts : std::min(tiles, slots));
+    cfg.blockDim = kFewThreads;
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = unsigned(parts);
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
     uq::ProfScope _p("q4_few", st);
-    kernel<<<unsigned(std::min<int64_t>(tiles, offsets ? int64_t(uq::num_sms()) * 2 : int64_t(1) << 30)), 256, smem, st>>>(x, ldx, codes, r, w, o, section);
+    if (cudaLaunchKernelEx(&cfg, kernel, mr, mc, r, w, o, box) != cudaSuccess) return uq::check_cuda("q4_few_kernel launch");
     return uq::check_cuda("q4_few_kernel launch");
 }
 

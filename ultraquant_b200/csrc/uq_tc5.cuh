@@ -15,8 +15,8 @@ __device__ __forceinline__ unsigned smem_addr(const void *p) { return unsigned(_
 // leaves 128 rows of D in each, so that every byte of B crosses from L2 once for
 // 256 rows.
 
-// ---- the pair --------------------------------------------------------------------
-__device__ __forceinline__ unsigned pair_rank() {
+// ---- the cluster -----------------------------------------------------------------
+__device__ __forceinline__ unsigned cluster_rank() {
     unsigned r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
@@ -27,7 +27,7 @@ __device__ __forceinline__ unsigned leader_addr(unsigned addr) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
-__device__ __forceinline__ void pair_sync() {
+__device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
