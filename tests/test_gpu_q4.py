@@ -22,6 +22,13 @@ def q4():
     return m
 
 
+@pytest.fixture(autouse=True)
+def no_device_errors():
+    """No test leaves a wait that gave up, or another error that it did not ask for."""
+    yield
+    q4().check_errors()
+
+
 def make(shape, group, seed, s=None):
     """Q4 of random codes and signed scales, and its parts in float64."""
     g = torch.Generator(device="cuda").manual_seed(seed)
@@ -144,6 +151,32 @@ def test_linear_values(T, N, K, group, dt):
     xd = x.double()
     close(y, xd @ wd.T, xd.abs() @ wd.abs().T, K)
     assert torch.equal(y, q4().linear(x, w))                # the same bits again
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,N,K", [(1, 4096, 14336), (8, 2048, 16384), (12, 1024, 8192), (40, 2048, 8192), (300, 1024, 8192)])
+def test_linear_from_a_cold_cache(T, N, K, dt):
+    """Copies that come late and out of step, through rings that are filled several times: always the same bits."""
+    w, q, c, wd = make((N, K), 32, K)
+    x = acts(T, K, DT[dt], T)
+    dy = acts(T, N, DT[dt], T)
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    first = None
+    for i in range(60):
+        flush.fill_(i)
+        y = q4().linear(x, w)
+        if first is None:
+            first = y
+            close(y, x.double() @ wd.T, x.double().abs() @ wd.abs().T, K)
+        assert torch.equal(y, first), i
+    xg, s = x.clone().requires_grad_(), w.group_scales().requires_grad_()
+    ref = None
+    for i in range(20):
+        y = q4().linear(xg, w, s)
+        flush.fill_(i)
+        got = torch.autograd.grad(y, (xg, s), dy)
+        ref = ref or got
+        assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1]), i
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])

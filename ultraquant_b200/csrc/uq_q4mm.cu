@@ -118,48 +118,61 @@ struct Finder {
 // ----------------------------------------------------------------------------
 // Weights in 16-bit halves
 // ----------------------------------------------------------------------------
-// The pair (2 i, 2 i + 1) of a word as a + b u in two halves, u in the significand
-// of a power of two, and the factors of one fused multiply-add that makes e q of
-// it.  Nothing rounds or overflows, |e| <= 448 with 4 significant bits:
-//   bfloat16: u in bits 0 .. 3 of 128:  128 + u, times e less 136 e (17 x 15 has 8 bits)
-//   float16:  u in bits 4 .. 7 of 1024: 1024 + 16 u, times e / 16 less 72 e (9 x 15 has
-//             8 bits, 72 x 448 < 65504)
-// Three shifts a word, since one of the four pairs lies in place.
+// Eight codes become four words of two halves with one shift: nibbles 0, 4 and
+// 1, 5 of the word and of the word shifted by 8 are masked in place and read as
+// numbers that are linear in u; one fused multiply-add each makes e q of them,
+// times kUnit, a power of two that is taken back from the finished sum.  Nothing
+// rounds or overflows (|e| <= 448 with 4 significant bits, 9 x 15 and 17 x 15 have
+// 8 bits, 129 x 15 has 11):
+//   bfloat16, kUnit 2^-14: the masked bits are 2^-133 u and 2^-129 u, subnormal or
+//     of the least exponent, which continues them; times e 2^119 and e 2^115, less
+//     8 e 2^-14
+//   float16, kUnit 1/8: under the significand of 1024, 1024 + u and 1024 + 16 u;
+//     times e / 8 and e / 128, less 129 e and 9 e
 template <bool BF16> struct Halves;
 template <> struct Halves<true> {
     using T = __nv_bfloat16;
-    struct Scale { uint32_t e, z; };
+    static constexpr float kBack = 16384.0f;   // 1 / kUnit
+    struct Scale { uint32_t e, e16, z; };
     // e: two E4M3 values as float16; which: 0 or 1
     static __device__ __forceinline__ Scale scale(uint32_t e, int which) {
         const float f = __half2float(__ushort_as_half((unsigned short)(which ? e >> 16 : e)));
+        uint32_t d;
         Scale s;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(s.e) : "f"(f));
-        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(s.z) : "r"(s.e), "r"(0xc308c308u));
+        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(d) : "f"(f));
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(s.e) : "r"(d), "r"(0x7b007b00u));     // 2^119
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(s.e16) : "r"(d), "r"(0x79007900u));   // 2^115
+        asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(s.z) : "r"(d), "r"(0xba00ba00u));     // -2^-11
         return s;
     }
     static __device__ __forceinline__ void widen8(uint32_t w, const Scale &s, uint32_t *out) {
+        const uint32_t h = w >> 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t v = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
-            asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(out[i]) : "r"(v), "r"(s.e), "r"(s.z));
+            const uint32_t v = (i < 2 ? w : h) & (i & 1 ? 0x00f000f0u : 0x000f000fu);
+            asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(out[i]) : "r"(v), "r"(i & 1 ? s.e16 : s.e), "r"(s.z));
         }
     }
 };
 template <> struct Halves<false> {
     using T = __half;
-    struct Scale { uint32_t e, z; };
+    static constexpr float kBack = 8.0f;
+    struct Scale { uint32_t e, e16, z, z16; };
     static __device__ __forceinline__ Scale scale(uint32_t e, int which) {
         const uint32_t d = __byte_perm(e, 0, which ? 0x3232 : 0x1010);
         Scale s;
-        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.e) : "r"(d), "r"(0x2c002c00u));   // 1 / 16
-        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.z) : "r"(d), "r"(0xd480d480u));   // -72
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.e) : "r"(d), "r"(0x30003000u));     // 1 / 8
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.e16) : "r"(d), "r"(0x20002000u));   // 1 / 128
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.z) : "r"(d), "r"(0xd808d808u));     // -129
+        asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(s.z16) : "r"(d), "r"(0xc880c880u));   // -9
         return s;
     }
     static __device__ __forceinline__ void widen8(uint32_t w, const Scale &s, uint32_t *out) {
+        const uint32_t h = w >> 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t v = ((i == 0 ? w << 4 : w >> (4 * i - 4)) & 0x00f000f0u) | 0x64006400u;
-            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(out[i]) : "r"(v), "r"(s.e), "r"(s.z));
+            const uint32_t v = ((i < 2 ? w : h) & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+            asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(out[i]) : "r"(v), "r"(i & 1 ? s.e16 : s.e), "r"(i & 1 ? s.z16 : s.z));
         }
     }
 };
@@ -218,7 +231,7 @@ template <bool BF16> __device__ __forceinline__ void pack_piece(const uint32_t (
     using T = typename Halves<BF16>::T;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-        T two[2] = {from_float<T>(s * __uint_as_float(r[2 * j])), from_float<T>(s * __uint_as_float(r[2 * j + 1]))};
+        T two[2] = {from_float<T>(s * (Halves<BF16>::kBack * __uint_as_float(r[2 * j]))), from_float<T>(s * (Halves<BF16>::kBack * __uint_as_float(r[2 * j + 1])))};
         v[j] = *reinterpret_cast<const uint32_t *>(two);
     }
 }
@@ -370,8 +383,9 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     Tile t;
     const int64_t step = gridDim.x >> 1, first = blockIdx.x >> 1;                 // pairs
     const int64_t depth = DX ? w.N : w.K;
-    const int all = int((depth + 63) / 64);                                       // stages of the whole contraction
-    const int per = runs.splits > 1 ? ((all + 4 * runs.splits - 1) / (4 * runs.splits)) * 4 : all;   // of one part, whole chunks
+    // stages of the whole contraction and of one part of it, whole chunks of four: what lies beyond the end is zero, and every
+    // warp takes part in every chunk, so that no barrier goes by two phases unseen by one that will wait for it
+    const int all = int((depth + 255) / 256) * 4, per = (all / 4 + runs.splits - 1) / runs.splits * 4;
     unsigned it = 0, ct = 0, tiles = 0;                                           // stages, chunks, tiles so far
 
     if (warp == kWiden) {
@@ -467,7 +481,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
             const uint8_t *e0 = nullptr;
             uint32_t eraw = 0;
             const int s0 = next.split * per, wtile = next.wt * 2 + int(rank);
-            // scale bytes of this warp's stage of the chunk at stage c (which begins before the contraction's end)
+            // scale bytes of this warp's stage of the chunk at stage c
             auto scales_at = [&](int c) -> uint32_t {
                 if (DX) {
                     const int nn = (s0 + c + stage) * 64 + (quad & 1) * 32 + lane;
@@ -490,10 +504,9 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
             }
             int c = 0;
             do {
-                const int cn = min(4, n - c);
-                const uint32_t ecur = eraw;
-                if (c + 4 < n) eraw = scales_at(c + 4);   // a chunk ahead
-                if (stage < cn) {
+                if (live) {
+                    const uint32_t ecur = eraw;
+                    if (c + 4 < n) eraw = scales_at(c + 4);   // a chunk ahead
                     const unsigned wrap = slot0 + stage >= NS, slot = slot0 + stage - (wrap ? NS : 0);
                     const uint32_t ep = e4m3_pair(ecur);
                     const typename Halves<BF16>::Scale e[2] = {Halves<BF16>::scale(ep, 0), Halves<BF16>::scale(ep, 1)};
@@ -528,16 +541,9 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                     }
                     __syncwarp();
                     if (lane == 0) tc5::mbar_arrive_remote(full_a0 + 8 * slot);
-                } else if (live) {
-                    // no stage in a short last chunk: still see its barriers, so that no wait of this warp meets a phase two
-                    // behind the one it means (a parity cannot tell them apart)
-                    const unsigned last = slot0 + cn - 1, wrap = last >= NS;
-                    if (!wt.wait(full_c + 8 * cslot, cpar) || !wt.wait(empty + 8 * (last - (wrap ? NS : 0)), par0 ^ wrap)) break;
-                }
-                if (live) {
                     __syncwarp();
                     if (lane == 0) tc5::mbar_arrive(empty_c + 8 * cslot);
-                    slot0 += cn;
+                    slot0 += 4;
                     if (slot0 >= NS) { slot0 -= NS; par0 ^= 1; }
                     if (++cslot == NC) { cslot = 0; cpar ^= 1; }
                 }
@@ -660,17 +666,34 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
         const int64_t groups = w.K >> w.gshift;
         Tile next;
         bool more = find.find(runs, blockIdx.x, next);
+        const int per_chunk = 256 >> w.gshift;
+        const bool pairs = w.gshift == 5, even = (w.K & 63) == 0;
         const uint8_t *e0 = nullptr, *e1 = nullptr;      // this lane's two rows of scales; beyond N the last row's, not written
         uint32_t eraw[2];
         auto scales_of = [&](const Tile &tt) {
-            const int64_t n = int64_t(tt.wt) * kFewRows + warp * 16 + g;
-            e0 = w.scales + (tt.mat * w.N + min(n, w.N - 1)) * groups;
-            e1 = w.scales + (tt.mat * w.N + min(n + 8, w.N - 1)) * groups;
+            const int64_t n = int64_t(tt.wt) * kFewRows + warp * 16 + g, at = (int64_t(c0) * 256 + q * 64) >> w.gshift;
+            e0 = w.scales + (tt.mat * w.N + min(n, w.N - 1)) * groups + at;
+            e1 = w.scales + (tt.mat * w.N + min(n + 8, w.N - 1)) * groups + at;
         };
+        // the two rows' bytes for this lane's 64 values of chunk c (see scale_pair), then on to the next chunk
         auto scales_at = [&](int c) {
-            const int64_t k = int64_t(c) * 256 + q * 64;
-            eraw[0] = scale_pair(w, e0, k);
-            eraw[1] = scale_pair(w, e1, k);
+            if (c * 256 + q * 64 < w.K) {
+                if (!pairs) {
+                    eraw[0] = __ldg(e0) * 0x101u;
+                    eraw[1] = __ldg(e1) * 0x101u;
+                } else if (even) {
+                    eraw[0] = __ldg(reinterpret_cast<const unsigned short *>(e0));
+                    eraw[1] = __ldg(reinterpret_cast<const unsigned short *>(e1));
+                } else {
+                    const bool two = c * 256 + q * 64 + 32 < w.K;
+                    eraw[0] = __ldg(e0) | (two ? uint32_t(__ldg(e0 + 1)) << 8 : 0u);
+                    eraw[1] = __ldg(e1) | (two ? uint32_t(__ldg(e1 + 1)) << 8 : 0u);
+                }
+            } else {
+                eraw[0] = eraw[1] = 0;
+            }
+            e0 += per_chunk;
+            e1 += per_chunk;
         };
         if (more) {
             scales_of(next);
@@ -717,6 +740,9 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
                         }
                     }
                 }
+                // the copies into this stage come after the reads above, which may still be on their way: the arrival alone
+                // does not wait for them (cold, with 7 chunks a block, one call in 8 read a part of a later chunk)
+                tma::fence_proxy_async();
                 __syncwarp();
                 if (lane == 0) tc5::mbar_arrive(empty + 8 * slot);
                 if (++slot == NS) { slot = 0; phase ^= 1; }
@@ -731,7 +757,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
                     for (int i = 0; i < 4; ++i) {
                         const int r = 8 * u + 2 * q + (i & 1);
                         const int64_t n = int64_t(t.wt) * kFewRows + warp * 16 + g + 8 * (i >> 1);
-                        if (r < t.rows && n < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + n] = from_float<T>(scale * (acc[0][u][i] + acc[1][u][i]));
+                        if (r < t.rows && n < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + n] = from_float<T>(scale * (Halves<BF16>::kBack * (acc[0][u][i] + acc[1][u][i])));
                     }
             } else {
                 // sums [row of x][weight row]; one tile a block
@@ -763,7 +789,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
                     v += f;
                 }
                 const int64_t col = int64_t(t.wt) * kFewRows + n;
-                if (col < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + col] = from_float<T>(scale * v);
+                if (col < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + col] = from_float<T>(scale * (Halves<BF16>::kBack * v));
             }
         }
         tc5::cluster_sync();   // no block leaves while another reads its sums
@@ -778,7 +804,7 @@ __global__ void __launch_bounds__(256) q4_join_parts_kernel(const float *part, i
     for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < T * J; i += int64_t(gridDim.x) * 256) {
         float v = part[i];
         for (int p = 1; p < splits; ++p) v += part[int64_t(p) * T * J + i];
-        static_cast<Ty *>(out)[(i / J) * ld + i % J] = from_float<Ty>(s * v);
+        static_cast<Ty *>(out)[(i / J) * ld + i % J] = from_float<Ty>(s * (Halves<BF16>::kBack * v));
     }
 }
 
