@@ -379,7 +379,7 @@ int uq_quant_e8_search(const void *W, int w_dtype, int64_t rows, int64_t n0, int
  *   scale   (mats) floats
  * e q has at most 8 significant bits, so it is exact in bfloat16 and in
  * float16; the products below form e q x exactly and add in float32.
- * All pointers 16-byte aligned. */
+ * All pointers 16-byte aligned; at most 65535 matrices. */
 
 /* W (mats, rows, cols), row stride ldw, matrix stride rows * ldw, any dtype
  * code (converted to float32 first).  s = the least power of two, at least
@@ -389,8 +389,10 @@ int uq_quant_e8_search(const void *W, int w_dtype, int64_t rows, int64_t n0, int
  * to 0; q = x / (s e) rounded to nearest even (exactly), clipped to -8 .. 7.
  * A group with a non-finite value gets e = NaN, q = 0.  Writes every byte of
  * codes, scales and scale. */
+size_t uq_q4_encode_workspace_bytes(int64_t mats, int64_t rows, int64_t cols);
 int uq_q4_encode(const void *W, int w_dtype, int64_t mats, int64_t rows, int64_t cols, int64_t ldw,
-                 int group, uint8_t *codes, uint8_t *scales, float *scale, void *stream);
+                 int group, uint8_t *codes, uint8_t *scales, float *scale, void *workspace,
+                 size_t workspace_bytes, void *stream);
 
 /* out (mats, rows, cols) contiguous, UQ_F32, UQ_BF16 or UQ_F16: s e q, one
  * rounding (none to float32 while nothing underflows). */

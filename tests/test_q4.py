@@ -72,12 +72,14 @@ def test_c_abi_refuses(tmp_path):
     lib = _lib.load()
     bad, err = _lib.UQ_ERR_INVALID, lambda: lib.uq_last_error().decode()
     p = 1 << 20      # never followed: every call below is refused before a launch
-    assert lib.uq_q4_encode(p, 0, 1, 4, 48, 48, 32, p, p, p, None) == bad and "whole groups" in err()
-    assert lib.uq_q4_encode(p, 0, 1, 4, 64, 63, 32, p, p, p, None) == bad
-    assert lib.uq_q4_encode(p, 0, 1, 4, 64, 64, 48, p, p, p, None) == bad
-    assert lib.uq_q4_encode(p, 9, 1, 4, 64, 64, 32, p, p, p, None) == bad and "dtype" in err()
-    assert lib.uq_q4_encode(None, 0, 1, 4, 64, 64, 32, p, p, p, None) == bad and "null" in err()
-    assert lib.uq_q4_encode(p, 0, 1, 4, 64, 64, 32, p + 4, p, p, None) == bad and "aligned" in err()
+    assert lib.uq_q4_encode(p, 0, 1, 4, 48, 48, 32, p, p, p, p, 1 << 20, None) == bad and "whole groups" in err()
+    assert lib.uq_q4_encode(p, 0, 1, 4, 64, 63, 32, p, p, p, p, 1 << 20, None) == bad
+    assert lib.uq_q4_encode(p, 0, 1, 4, 64, 64, 48, p, p, p, p, 1 << 20, None) == bad
+    assert lib.uq_q4_encode(p, 9, 1, 4, 64, 64, 32, p, p, p, p, 1 << 20, None) == bad and "dtype" in err()
+    assert lib.uq_q4_encode(None, 0, 1, 4, 64, 64, 32, p, p, p, p, 1 << 20, None) == bad and "null" in err()
+    assert lib.uq_q4_encode(p, 0, 1, 4, 64, 64, 32, p + 4, p, p, p, 1 << 20, None) == bad and "aligned" in err()
+    assert lib.uq_q4_encode(p, 0, 1, 4, 64, 64, 32, p, p, p, None, 0, None) == _lib.UQ_ERR_WORKSPACE and "workspace" in err()
+    assert lib.uq_q4_encode(p, 0, 65536, 4, 64, 64, 32, p, p, p, p, 1 << 30, None) == bad
     assert lib.uq_q4_decode(p, p, p, 1, 4, 64, 32, p, 1, None) == bad and "dtype" in err()
     assert lib.uq_q4_round_scales(p, -1, 4, p, p, None) == bad
     lin = lambda f, dt=2, T=4, ldx=64, mats=1, N=8, K=64, g=32, off=None, x=p, c=p, ld2=64: f(

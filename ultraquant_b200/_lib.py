@@ -81,7 +81,8 @@ SIGNATURES = {
     "uq_quant_e8": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _f64, _i32, _p, _p, _p, _p, _p, _sz, _p]),
     "uq_quant_e8_b28_workspace_bytes": (_sz, [_i64, _i64]),
     "uq_quant_e8_b28": (_i32, [_p, _i32, _i64, _i64, _i64, _p, _f64, _p, _p, _p, _p, _p, _sz, _p]),
-    "uq_q4_encode": (_i32, [_p, _i32, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _p]),
+    "uq_q4_encode_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "uq_q4_encode": (_i32, [_p, _i32, _i64, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _sz, _p]),
     "uq_q4_decode": (_i32, [_p, _p, _p, _i64, _i64, _i64, _i32, _p, _i32, _p]),
     "uq_q4_round_scales": (_i32, [_p, _i64, _i64, _p, _p, _p]),
     "uq_q4_linear_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),

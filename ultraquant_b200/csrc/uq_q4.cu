@@ -51,30 +51,152 @@ __device__ __forceinline__ uint32_t group_top(const float (&x)[8], int lanes) {
     return m;
 }
 
+// blockIdx.y: matrix.  `words` of eight values a matrix, `wrow` a row; `flat`:
+// rows follow one another, so that a word's place needs no division.
 struct EncArgs {
-    int64_t words, wrow, ldw, per_mat;   // 8-value words: all, per row, (values) row stride, per matrix
-    int group;
-    bool vec;
+    int64_t words, wrow, ldw;
+    int group, blocks;       // blocks: of a matrix in q4_top_kernel
+    bool vec, flat;
 };
+constexpr int kWords = 4;    // a thread's loads in flight
 
-// top[mat] = max |x| bits over the groups without a non-finite value.
-template <typename T> __global__ void __launch_bounds__(256) q4_top_kernel(const T *W, EncArgs a, uint32_t *top) {
+template <typename T> __device__ __forceinline__ void load_word(const T *W, const EncArgs &a, int64_t i, float (&x)[8]) {
+    load_weights(W + (a.flat ? i * 8 : (i / a.wrow) * a.ldw + (i % a.wrow) * 8), a.vec, x);
+}
+
+// top[matrix][block] = max |x| bits over the groups without a non-finite value.
+// Bound by memory; a group is looked at as a whole only where a warp has met such
+// a value.
+template <typename T> __global__ void __launch_bounds__(256) q4_top_kernel(const T *W, EncArgs a, int64_t mat_stride, uint32_t *top) {
+    __shared__ uint32_t warp_top[8];
+    W += blockIdx.y * mat_stride;
+    uint32_t best = 0;
+    for (int64_t base = int64_t(blockIdx.x) * 256 * kWords; base < a.words; base += int64_t(gridDim.x) * 256 * kWords) {
+        float x[kWords][8];
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+            const int64_t i = base + u * 256 + threadIdx.x;
+            if (i < a.words) {
+                load_word(W, a, i, x[u]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[u][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[u][j]) & 0x7fffffffu);
+            if (__any_sync(0xffffffffu, m >= 0x7f800000u)) {
+                m = group_top(x[u], a.group / 8);
+                if (m >= 0x7f800000u) m = 0;
+            }
+            best = max(best, m);
+        }
+    }
+    best = __reduce_max_sync(0xffffffffu, best);
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = best;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < 8; ++i) best = max(best, warp_top[i]);
+        top[int64_t(blockIdx.y) * gridDim.x + blockIdx.x] = best;
+    }
+}
+
+// The second reading goes backwards: what the first read last is still in L2.
+template <typename T>
+__global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, int64_t mat_stride, const uint32_t *top, float *scale, uint32_t *codes, uint8_t *scales) {
+    __shared__ uint32_t warp_top[8];
     const int lanes = a.group / 8;
-    const int64_t step = int64_t(gridDim.x) * 256;
-    for (int64_t base = int64_t(blockIdx.x) * 256; base < a.words; base += step) {
-        const int64_t i = base + threadIdx.x;
-        const bool ok = i < a.words;
-        float x[8] = {};
-        if (ok) load_weights(W + (i / a.wrow) * a.ldw + (i % a.wrow) * 8, a.vec, x);
-        uint32_t m = group_top(x, lanes);
-        if (m >= 0x7f800000u) m = 0;
-        const int64_t mat = ok ? i / a.per_mat : 0, mat0 = base / a.per_mat;
-        const bool same = min(base + 255, a.words - 1) / a.per_mat == mat0;   // one matrix in this block's 256 words
-        if (same) {
-            m = __reduce_max_sync(0xffffffffu, m);
-            if ((threadIdx.x & 31) == 0 && m) atomicMax(top + mat0, m);
-        } else if (ok && m) {
-            atomicMax(top + mat, m);
+    uint32_t best = 0;
+    for (int i = threadIdx.x; i < a.blocks; i += 256) best = max(best, top[int64_t(blockIdx.y) * a.blocks + i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = best;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) best = max(best, warp_top[i]);
+    const float s = scale_for(best, 11);
+    if (blockIdx.x == 0 && threadIdx.x == 0) scale[blockIdx.y] = s;
+    W += blockIdx.y * mat_stride;
+    codes += blockIdx.y * a.words;
+    scales += blockIdx.y * (a.words / lanes);
+    const int64_t spans = (a.words + 256 * kWords - 1) / (256 * kWords);
+    for (int64_t span = spans - 1 - blockIdx.x; span >= 0; span -= gridDim.x) {
+        float xs[kWords][8];
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+            const int64_t i = span * 256 * kWords + u * 256 + threadIdx.x;
+            if (i < a.words) {
+                load_word(W, a, i, xs[u]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) xs[u][j] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+            const int64_t i = span * 256 * kWords + u * 256 + threadIdx.x;
+            const float (&x)[8] = xs[u];
+            const uint32_t m = group_top(x, lanes);
+            // the first value of that size: place in the group and sign, the least of (place, sign)
+            const int sub = int(threadIdx.x) & (lanes - 1);
+            uint32_t first = 0xffffffffu;
+#pragma unroll
+            for (int j = 7; j >= 0; --j)
+                if ((__float_as_uint(x[j]) & 0x7fffffffu) == m) first = uint32_t(sub * 8 + j) * 2 + (__float_as_uint(x[j]) >> 31);
+            for (int o = lanes >> 1; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+            if (i >= a.words) continue;   // whole groups: the shuffles above are over
+            // -m / (8 s): s is a power of two, so the quotient is exact (or underflows, and e4m3_of keeps its sign)
+            const float size = __fdiv_rn(__uint_as_float(m), 8.0f * s);
+            uint8_t e = m >= 0x7f800000u ? uint8_t(0x7f) : e4m3_of(size == 0.0f && m ? 0x1p-20f : size);
+            if (e != 0x7f && m && !(first & 1u)) e |= 0x80;   // a positive m takes a negative scale
+            uint32_t word = 0x88888888u;
+            if (e != 0x7f && m) {
+                const float c = s * e4m3_value(e), rc = __frcp_rn(c), half = 0.5f * fabsf(c);
+                word = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    // q = rint(x / c) exactly: t is within 2^-22 of x / c relatively, so rint(t) is off by at most one and
+                    // only next to a border; the remainder x - q c is exact (q c has 8 bits) and decides, ties to even
+                    float q = rintf(x[j] * rc);
+                    const float r = fmaf(-q, c, x[j]);
+                    if (fabsf(r) > half || (fabsf(r) == half && (int(q) & 1))) q += ((r < 0.0f) != (c < 0.0f)) ? -1.0f : 1.0f;
+                    const int v = int(fminf(fmaxf(q, -8.0f), 7.0f)) + 8;
+                    word |= uint32_t(v) << (4 * ((j >> 1) + 4 * (j & 1)));
+                }
+            }
+            codes[i] = word;
+            if (sub == 0) scales[i / lanes] = e;
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) q4_decode_kernel(const uint32_t *codes, const uint8_t *scales, const float *scale, int64_t words, int lshift, T *out) {
+    const float s = __ldg(scale + blockIdx.y);
+    codes += blockIdx.y * words;
+    scales += blockIdx.y * (words >> lshift);
+    out += blockIdx.y * words * 8;
+    for (int64_t base = int64_t(blockIdx.x) * 256 * kWords + threadIdx.x; base < words; base += int64_t(gridDim.x) * 256 * kWords) {
+        uint32_t w[kWords];
+        uint8_t e[kWords];
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+            const int64_t i = min(base + u * 256, words - 1);
+            w[u] = __ldg(codes + i);
+            e[u] = __ldg(scales + (i >> lshift));
+        }
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) {
+            const int64_t i = base + u * 256;
+            if (i >= words) break;
+            const float c = s * e4m3_value(e[u]);
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = float(nibble(w[u], j) - 8) * c;
+            store8(out + i * 8, x);
         }
     }
 }
@@ -82,63 +204,6 @@ template <typename T> __global__ void __launch_bounds__(256) q4_top_kernel(const
 __global__ void q4_scale_kernel(float *scale, int64_t mats, int p) {
     const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
     if (i < mats) scale[i] = scale_for(__float_as_uint(scale[i]), p);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, const float *scale, uint32_t *codes, uint8_t *scales) {
-    const int lanes = a.group / 8;
-    const int64_t step = int64_t(gridDim.x) * 256;
-    for (int64_t base = int64_t(blockIdx.x) * 256; base < a.words; base += step) {
-        const int64_t i = base + threadIdx.x;
-        const bool ok = i < a.words;
-        float x[8] = {};
-        if (ok) load_weights(W + (i / a.wrow) * a.ldw + (i % a.wrow) * 8, a.vec, x);
-        const uint32_t m = group_top(x, lanes);
-        // the first value of that size: place in the group and sign, the least of (place, sign)
-        const int sub = int(threadIdx.x) & (lanes - 1);
-        uint32_t first = 0xffffffffu;
-#pragma unroll
-        for (int j = 7; j >= 0; --j)
-            if ((__float_as_uint(x[j]) & 0x7fffffffu) == m) first = uint32_t(sub * 8 + j) * 2 + (__float_as_uint(x[j]) >> 31);
-        for (int o = lanes >> 1; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-        if (!ok) continue;   // whole groups: the shuffles above are over
-        const float s = scale[i / a.per_mat];
-        // -m / (8 s): s is a power of two, so the quotient is exact (or underflows, and e4m3_of keeps its sign)
-        const float size = __fdiv_rn(__uint_as_float(m), 8.0f * s);
-        uint8_t e = m >= 0x7f800000u ? uint8_t(0x7f) : e4m3_of(size == 0.0f && m ? 0x1p-20f : size);
-        if (e != 0x7f && m && !(first & 1u)) e |= 0x80;   // a positive m takes a negative scale
-        uint32_t word = 0x88888888u;
-        if (e != 0x7f && m) {
-            const float c = s * e4m3_value(e), rc = __frcp_rn(c), half = 0.5f * fabsf(c);
-            word = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                // q = rint(x / c) exactly: t is within 2^-22 of x / c relatively, so rint(t) is off by at most one and
-                // only next to a border; the remainder x - q c is exact (q c has 8 bits) and decides, ties to even
-                float q = rintf(x[j] * rc);
-                const float r = fmaf(-q, c, x[j]);
-                if (fabsf(r) > half || (fabsf(r) == half && (int(q) & 1))) q += ((r < 0.0f) != (c < 0.0f)) ? -1.0f : 1.0f;
-                const int u = int(fminf(fmaxf(q, -8.0f), 7.0f)) + 8;
-                word |= uint32_t(u) << (4 * ((j >> 1) + 4 * (j & 1)));
-            }
-        }
-        codes[i] = word;
-        if (sub == 0) scales[i / lanes] = e;
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) q4_decode_kernel(const uint32_t *codes, const uint8_t *scales, const float *scale, int64_t words,
-                                                        int64_t per_mat, int lshift, T *out) {
-    const int64_t step = int64_t(gridDim.x) * 256;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < words; i += step) {
-        const uint32_t w = __ldg(codes + i);
-        const float c = __ldg(scale + (per_mat == words ? 0 : i / per_mat)) * e4m3_value(__ldg(scales + (i >> lshift)));
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = float(nibble(w, j) - 8) * c;
-        store8(out + i * 8, x);
-    }
 }
 
 __global__ void __launch_bounds__(256) q4_scales_top_kernel(const float *c, int64_t n, uint32_t *top) {
@@ -169,26 +234,44 @@ template <typename I> __device__ __forceinline__ int64_t token_at(const I *token
     return v >= 0 && v < V ? v : -1;
 }
 
+// A block takes a token's row at a time, two words a thread on the way, the next
+// token already read: 16384 rows of 4096 in 34 us, 4.9 TB/s, bound by the writes.
+// (Four rows on the way a block took more registers, fewer blocks and 49 us.)
 template <typename I, typename T>
 __global__ void __launch_bounds__(256) q4_embed_kernel(const I *tokens, int64_t n, const uint32_t *codes, const uint8_t *scales,
                                                        const float *scale, int64_t V, int wrow, int lshift, float alpha, T *out) {
     const float f = alpha * __ldg(scale);
     const int per = wrow >> lshift;
-    for (int64_t t = blockIdx.x; t < n; t += gridDim.x) {
-        const int64_t v = token_at(tokens, t, V);
-        if (v < 0 && threadIdx.x == 0) atomicExch(&g_q4_bad_token, 1);
-        for (int i = threadIdx.x; i < wrow; i += 256) {
-            float x[8];
-            if (v >= 0) {
-                const uint32_t w = __ldg(codes + v * wrow + i);
-                const float c = f * e4m3_value(__ldg(scales + v * per + (i >> lshift)));
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = float(nibble(w, j) - 8) * c;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = __int_as_float(0x7fc00000);
+    int64_t t = blockIdx.x, v = t < n ? token_at(tokens, t, V) : -1;
+    for (; t < n; t += gridDim.x) {
+        const int64_t now = v;
+        if (t + gridDim.x < n) v = token_at(tokens, t + gridDim.x, V);
+        if (now < 0 && threadIdx.x == 0) atomicExch(&g_q4_bad_token, 1);
+        const uint32_t *const row = codes + now * wrow;
+        const uint8_t *const erow = scales + now * per;
+        for (int i = threadIdx.x; i < wrow; i += 512) {
+            const bool two = i + 256 < wrow;
+            uint32_t w[2] = {0, 0};
+            float c[2] = {__int_as_float(0x7fc00000), __int_as_float(0x7fc00000)};
+            if (now >= 0) {
+                w[0] = __ldg(row + i);
+                const uint8_t e0 = __ldg(erow + (i >> lshift));
+                uint8_t e1 = 0;
+                if (two) {
+                    w[1] = __ldg(row + i + 256);
+                    e1 = __ldg(erow + ((i + 256) >> lshift));
+                }
+                c[0] = f * e4m3_value(e0);
+                c[1] = f * e4m3_value(e1);
             }
-            store8(out + (t * wrow + i) * 8, x);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (u && !two) break;
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = float(nibble(w[u], j) - 8) * c[u];
+                store8(out + (t * wrow + i + 256 * u) * 8, x);
+            }
         }
     }
 }
@@ -315,6 +398,17 @@ __global__ void __launch_bounds__(256) q4_zero_kernel(float *p, int64_t n) {
 // goes to part[piece][head / tail].
 constexpr int kSeg = 32;
 
+// Eight values of a row as loaded, and as floats.
+template <typename T> struct Raw8 {
+    union { uint4 v[sizeof(T) / 2]; T t[8]; };
+    __device__ __forceinline__ Raw8() {}
+    __device__ __forceinline__ void load(const T *p, bool ok) {
+#pragma unroll
+        for (int i = 0; i < int(sizeof(T)) / 2; ++i) v[i] = ok ? __ldg(reinterpret_cast<const uint4 *>(p) + i) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ float at(int j) const { return to_float(t[j]); }
+};
+
 template <typename T>
 __global__ void __launch_bounds__(256) q4_segment_kernel(const uint32_t *keys, const uint32_t *pos, int64_t n, const T *dout, int64_t ld,
                                                          const uint32_t *codes, int64_t V, int wrow, int lshift, float alpha, float *dc,
@@ -334,27 +428,22 @@ __global__ void __launch_bounds__(256) q4_segment_kernel(const uint32_t *keys, c
     const int lanes = 1 << lshift, per = wrow >> lshift;
     float acc[8] = {};
     bool head = skey[0] == skey[1];
-    constexpr int U = 4;
+    constexpr int U = sizeof(T) == 4 ? 4 : 8;      // rows on the way
     for (int b = 0; b < m; b += U) {
-        float d[U][8];
+        Raw8<T> d[U];
         uint32_t w[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool ok = in && b + u < m && skey[b + u + 1] < uint32_t(V);
             w[u] = ok ? __ldg(codes + int64_t(skey[b + u + 1]) * wrow + col) : 0;
-            if (ok) {
-                load8(dout + int64_t(spos[b + u]) * ld + col * 8, d[u]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) d[u][j] = 0.f;
-            }
+            d[u].load(dout + (ok ? int64_t(spos[b + u]) * ld + col * 8 : 0), ok);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (b + u >= m) break;
             const uint32_t key = skey[b + u + 1];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += d[u][j];
+            for (int j = 0; j < 8; ++j) acc[j] += d[u].at(j);
             const bool last = b + u + 1 == m;
             if (key >= uint32_t(V) || (!last && skey[b + u + 2] == key)) continue;
             float sum = 0.f;
@@ -404,25 +493,26 @@ int blocks_for(int64_t work, int per_sm) {
     return int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(uq::num_sms()) * per_sm)));
 }
 
+int top_blocks(int64_t words) { return blocks_for((words + 256 * kWords - 1) / (256 * kWords), 8); }
+
 template <typename T>
-int encode(const T *W, int64_t mats, int64_t rows, int64_t cols, int64_t ldw, int group, uint8_t *codes, uint8_t *scales, float *scale, cudaStream_t st) {
+int encode(const T *W, int64_t mats, int64_t rows, int64_t cols, int64_t ldw, int group, uint8_t *codes, uint8_t *scales, float *scale, uint32_t *top, cudaStream_t st) {
     EncArgs a;
     a.wrow = cols / 8;
-    a.per_mat = rows * a.wrow;
-    a.words = mats * a.per_mat;
+    a.words = rows * a.wrow;
     a.ldw = ldw;
     a.group = group;
+    a.blocks = top_blocks(a.words);
     a.vec = al16(W) && ldw * int64_t(sizeof(T)) % 16 == 0;
-    if (cudaMemsetAsync(scale, 0, size_t(mats) * 4, st) != cudaSuccess) return uq::check_cuda("uq_q4_encode");
-    const int grid = blocks_for((a.words + 255) / 256, 8);
-    if (a.words) { uq::ProfScope _p("q4_top", st); q4_top_kernel<T><<<grid, 256, 0, st>>>(W, a, reinterpret_cast<uint32_t *>(scale)); }
-    { uq::ProfScope _p("q4_scale", st); q4_scale_kernel<<<unsigned((mats + 255) / 256), 256, 0, st>>>(scale, mats, 11); }
-    if (a.words) { uq::ProfScope _p("q4_encode", st); q4_encode_kernel<T><<<grid, 256, 0, st>>>(W, a, scale, reinterpret_cast<uint32_t *>(codes), scales); }
+    a.flat = ldw == cols;
+    const dim3 grid(unsigned(a.blocks), unsigned(mats));
+    { uq::ProfScope _p("q4_top", st); q4_top_kernel<T><<<grid, 256, 0, st>>>(W, a, rows * ldw, top); }
+    { uq::ProfScope _p("q4_encode", st); q4_encode_kernel<T><<<grid, 256, 0, st>>>(W, a, rows * ldw, top, scale, reinterpret_cast<uint32_t *>(codes), scales); }
     return uq::check_cuda("q4_encode_kernel launch");
 }
 
 bool form_ok(int64_t mats, int64_t rows, int64_t cols, int group) {
-    return mats >= 0 && rows >= 0 && group_ok(group) && cols > 0 && cols % group == 0 && cols < (int64_t(1) << 31) &&
+    return mats >= 0 && mats <= 65535 && rows >= 0 && group_ok(group) && cols > 0 && cols % group == 0 && cols < (int64_t(1) << 31) &&
            (rows == 0 || mats < (int64_t(1) << 48) / rows / cols);
 }
 
@@ -463,22 +553,29 @@ int lane_shift(int group) { return uq::ilog2(group) - 3; }
 
 extern "C" {
 
+size_t uq_q4_encode_workspace_bytes(int64_t mats, int64_t rows, int64_t cols) {
+    return mats > 0 && rows >= 0 && cols > 0 ? size_t(mats) * top_blocks(rows * (cols / 8)) * 4 : 0;
+}
+
 int uq_q4_encode(const void *W, int w_dtype, int64_t mats, int64_t rows, int64_t cols, int64_t ldw, int group, uint8_t *codes,
-                 uint8_t *scales, float *scale, void *stream) {
+                 uint8_t *scales, float *scale, void *workspace, size_t workspace_bytes, void *stream) {
     if (!form_ok(mats, rows, cols, group) || ldw < cols)
         return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: bad shape (mats=%lld rows=%lld cols=%lld ld=%lld group=%d; cols must be whole groups of 32, 64, 128 or 256)",
                         (long long)mats, (long long)rows, (long long)cols, (long long)ldw, group);
     if (mats == 0) return UQ_OK;
     if (!scale || (rows && (!W || !codes || !scales))) return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: null pointer");
     if (!al16(codes)) return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: codes not 16-byte aligned");
+    if (w_dtype < UQ_F32 || w_dtype > UQ_F16) return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: unknown dtype code %d", w_dtype);
+    const size_t need = uq_q4_encode_workspace_bytes(mats, rows, cols);
+    if (!workspace || workspace_bytes < need) return uq::fail(UQ_ERR_WORKSPACE, "uq_q4_encode: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const cudaStream_t st = UQ_STREAM(stream);
+    uint32_t *const top = static_cast<uint32_t *>(workspace);
     switch (w_dtype) {
-        case UQ_F32: return encode(static_cast<const float *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
-        case UQ_F64: return encode(static_cast<const double *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
-        case UQ_BF16: return encode(static_cast<const __nv_bfloat16 *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
-        case UQ_F16: return encode(static_cast<const __half *>(W), mats, rows, cols, ldw, group, codes, scales, scale, st);
+        case UQ_F32: return encode(static_cast<const float *>(W), mats, rows, cols, ldw, group, codes, scales, scale, top, st);
+        case UQ_F64: return encode(static_cast<const double *>(W), mats, rows, cols, ldw, group, codes, scales, scale, top, st);
+        case UQ_BF16: return encode(static_cast<const __nv_bfloat16 *>(W), mats, rows, cols, ldw, group, codes, scales, scale, top, st);
+        default: return encode(static_cast<const __half *>(W), mats, rows, cols, ldw, group, codes, scales, scale, top, st);
     }
-    return uq::fail(UQ_ERR_INVALID, "uq_q4_encode: unknown dtype code %d", w_dtype);
 }
 
 int uq_q4_decode(const uint8_t *codes, const uint8_t *scales, const float *scale, int64_t mats, int64_t rows, int64_t cols, int group,
@@ -488,15 +585,16 @@ int uq_q4_decode(const uint8_t *codes, const uint8_t *scales, const float *scale
     if (mats == 0 || rows == 0) return UQ_OK;
     if (!codes || !scales || !scale || !out) return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: null pointer");
     if (!al16(codes) || !al16(out)) return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: codes or out not 16-byte aligned");
-    const int64_t per_mat = rows * cols / 8, words = mats * per_mat;
+    const int64_t words = rows * cols / 8;
     const cudaStream_t st = UQ_STREAM(stream);
-    const int grid = blocks_for((words + 255) / 256, 8), ls = lane_shift(group);
+    const dim3 grid(unsigned(top_blocks(words)), unsigned(mats));
+    const int ls = lane_shift(group);
     const uint32_t *cw = reinterpret_cast<const uint32_t *>(codes);
     uq::ProfScope _p("q4_decode", st);
     switch (out_dtype) {
-        case UQ_F32: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, per_mat, ls, static_cast<float *>(out)); break;
-        case UQ_BF16: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, per_mat, ls, static_cast<__nv_bfloat16 *>(out)); break;
-        case UQ_F16: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, per_mat, ls, static_cast<__half *>(out)); break;
+        case UQ_F32: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, ls, static_cast<float *>(out)); break;
+        case UQ_BF16: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, ls, static_cast<__nv_bfloat16 *>(out)); break;
+        case UQ_F16: q4_decode_kernel<<<grid, 256, 0, st>>>(cw, scales, scale, words, ls, static_cast<__half *>(out)); break;
         default: return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: dtype code %d is not built", out_dtype);
     }
     return uq::check_cuda("q4_decode_kernel launch");

@@ -208,15 +208,48 @@ struct Weights {
     int gshift;       // group = 2^gshift
 };
 
-// The E4M3 bytes of values k .. k + 31 and k + 32 .. k + 63 of the row whose bytes
-// begin at `p`, in the low 16 bits; 0 (e = 0: the weights are 0 whatever the
-// codes are) beyond K.  k is a multiple of 64.
-__device__ __forceinline__ uint32_t scale_pair(const Weights &w, const uint8_t *p, int64_t k) {
-    if (k >= w.K) return 0;
-    p += k >> w.gshift;
-    if (w.gshift > 5) return uint32_t(__ldg(p)) * 0x101u;
-    if ((w.K & 63) == 0) return __ldg(reinterpret_cast<const unsigned short *>(p));   // rows of an even number of bytes
-    return uint32_t(__ldg(p)) | (k + 32 < w.K ? uint32_t(__ldg(p + 1)) << 8 : 0u);
+// A chunk's scales on their way to shared memory, four rows of eight pieces of 32
+// values a lane, or (DX) eight rows of four.  Where a row's bytes of the chunk are
+// one aligned word (`packed`), it is kept as it is; else the pieces' bytes are
+// gathered.  Nothing here waits for a load: the words are taken apart when they
+// are stored.
+struct Scales { uint32_t w[8]; };
+
+__device__ __forceinline__ uint32_t load_bytes(const uint8_t *p, int bytes) {
+    return bytes == 4 ? __ldg(reinterpret_cast<const unsigned *>(p)) : bytes == 2 ? __ldg(reinterpret_cast<const unsigned short *>(p)) : __ldg(p);
+}
+// Bytes of the four pieces from value k on, 0 beyond K.
+__device__ __forceinline__ uint32_t gather4(const Weights &w, const uint8_t *row, int64_t k) {
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k + 32 * i < w.K ? __ldg(row + ((k + 32 * i) >> w.gshift)) : 0u;
+    return v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24;
+}
+// Rows lane + 32 j (below `rows`) from value k on; `p`: the first row's bytes.
+template <bool DX>
+__device__ __forceinline__ void load_scales(Scales &v, const Weights &w, bool packed, const uint8_t *p, int64_t groups, int rows, int64_t k) {
+    constexpr int R = DX ? 8 : 4, W = 8 / R;   // rows, words of each
+    const int lane = threadIdx.x & 31, bytes = max((DX ? 128 : 256) >> w.gshift, 1);
+    if (k >= w.K) rows = 0;                    // DX: columns beyond the matrix
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const bool in = lane + 32 * j < rows;
+        const uint8_t *const row = p + (in ? lane + 32 * j : 0) * groups;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v.w[W * j + i] = 0;
+        if (!in) continue;
+        const uint8_t *const at = row + (k >> w.gshift);
+        if (!packed) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) v.w[W * j + i] = gather4(w, row, k + 128 * i);
+        } else if (W == 2 && bytes == 8) {
+            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(at));
+            v.w[W * j] = u.x;
+            v.w[W * j + W - 1] = u.y;
+        } else {
+            v.w[W * j] = load_bytes(at, bytes);
+        }
+    }
 }
 
 struct Out {
@@ -312,9 +345,10 @@ template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int
 // a narrow instruction.  A pair of CTAs takes 256 weight columns, 128 each, and
 // each CTA brings half of the tile's rows: alone, a CTA needed 64 bytes a clock
 // of rows from L2, and L2 gave 12 TB/s, 43 a clock and SM.  Stages of 64
-// contraction steps: `full_b` this CTA's half of the rows (TMA, 128-byte
-// swizzle), `full_a` (in the first CTA, for both) the widened weights, `empty`
-// both free again.
+// contraction steps: `full` (in the first CTA) its half of the rows (TMA, 128-byte
+// swizzle), the second CTA's word that its half is there, and the widened weights
+// of both, one barrier for all, since the issuing warp's waits bound the rate;
+// `empty` both free again.
 //   forward: lane n; the weights go from registers into tensor memory (32
 //            columns a stage), codes by TMA in chunks of 256 steps
 //   DX:      lane k; a stage is 64 rows n of 128 codes, widened into shared
@@ -323,16 +357,18 @@ template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int
 // results, those of a tile after the next tile's first chunk is widened, so that
 // the tensor cores have work meanwhile; warp 16 copies the rows, warp 17 the
 // codes; warp 18 issues the products (first CTA) or tells the first CTA that its
-// rows are there (second).
+// rows are there (second); warp 19 brings each chunk's scales, an odd few bytes
+// from every row, which loaded by the widening warps a chunk ahead still cost 7 %
+// forward and 30 % of DX (4096 x 4096 x 14336: 460 us, 316 without any scales).
 // ----------------------------------------------------------------------------
-constexpr int kWiden = 16, kThreads = (kWiden + 3) * 32;
+constexpr int kWiden = 16, kThreads = (kWiden + 4) * 32;
 
 template <int BT, bool DX> struct Cfg {
     static constexpr int NS = DX ? (BT == 256 ? 5 : 6) : 8;                  // stages
     static constexpr int kChunks = DX ? (BT == 64 ? 4 : BT == 128 ? 3 : 3) : BT == 256 ? 5 : 8;
-    static constexpr int kB = BT * 64, kA = DX ? 16384 : 0, kC = 16384;
-    static constexpr int kBar = 4 * NS + 2 * kChunks + 2;
-    static constexpr int kSmem = 1024 + NS * (kB + kA) + kChunks * kC + kBar * 8 + 16;
+    static constexpr int kB = BT * 64, kA = DX ? 16384 : 0, kC = 16384, kE = 1024;   // kE: a chunk's scales, 512 pairs
+    static constexpr int kBar = 2 * NS + 2 * kChunks + 2;
+    static constexpr int kSmem = 1024 + NS * (kB + kA) + kChunks * (kC + kE) + kBar * 8 + 16;
     static_assert(kSmem <= 232448, "shared memory of one block");
     static_assert(DX || BT + 32 * NS <= 512, "tensor memory");
 };
@@ -344,9 +380,8 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     constexpr int NS = C::NS, NC = C::kChunks, kBox = BT / 4;   // rows of one copy: half of a CTA's share
     extern __shared__ uint8_t smem_raw[];
     const unsigned smem_at = tc5::smem_addr(smem_raw), base = (smem_at + 1023u) & ~1023u;
-    const unsigned sb = base, sa = sb + NS * C::kB, sc = sa + NS * C::kA, bars = sc + NC * C::kC;
-    const unsigned full_b = bars, full_a = bars + 8 * NS, empty = bars + 16 * NS, full_p = bars + 24 * NS, full_c = bars + 32 * NS,
-                   empty_c = full_c + 8 * NC, done = empty_c + 8 * NC, drained = done + 8, misc = drained + 8;
+    const unsigned sb = base, sa = sb + NS * C::kB, sc = sa + NS * C::kA, se = sc + NC * C::kC, bars = se + NC * C::kE;
+    const unsigned full = bars, empty = bars + 8 * NS, full_c = bars + 16 * NS, empty_c = full_c + 8 * NC, done = empty_c + 8 * NC, drained = done + 8, misc = drained + 8;
     volatile int *gave_up = reinterpret_cast<volatile int *>(smem_raw + (misc + 4 - tc5::smem_addr(smem_raw)));
     const int warp = tc5::warp_id(), lane = threadIdx.x & 31;
     const unsigned rank = tc5::cluster_rank();
@@ -354,13 +389,11 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     if (threadIdx.x == 0) {
         *gave_up = 0;
         for (int i = 0; i < NS; ++i) {
-            tma::mbar_init(full_b + 8 * i, 1);
-            tma::mbar_init(full_a + 8 * i, 8);
+            tma::mbar_init(full + 8 * i, rank == 0 ? 10 : 1);
             tma::mbar_init(empty + 8 * i, 1);
-            tma::mbar_init(full_p + 8 * i, 1);
         }
         for (int i = 0; i < NC; ++i) {
-            tma::mbar_init(full_c + 8 * i, 1);
+            tma::mbar_init(full_c + 8 * i, 2);   // codes, scales
             tma::mbar_init(empty_c + 8 * i, kWiden);
         }
         tma::mbar_init(done, 1);
@@ -397,15 +430,15 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                 const int slot = it % NS;
                 if (!wt.wait(empty + 8 * slot, ((it / NS) & 1) ^ 1)) break;
                 if (lane == 0) {
-                    tma::mbar_arrive_expect_tx(full_b + 8 * slot, boxes * kBox * 128);
+                    tma::mbar_arrive_expect_tx(full + 8 * slot, boxes * kBox * 128);
                     for (int b = 0; b < boxes; ++b)
-                        tma::load2d(sb + slot * C::kB + b * kBox * 128, &map_rows, (s0 + s) * 64, row + b * kBox, full_b + 8 * slot);
+                        tma::load2d(sb + slot * C::kB + b * kBox * 128, &map_rows, (s0 + s) * 64, row + b * kBox, full + 8 * slot);
                 }
                 __syncwarp();
             }
         }
         if (wt.fail)   // copies in flight land before the block ends
-            for (unsigned i = it > NS ? it - NS : 0; i < it; ++i) tc5::Waiter::drain(full_b + 8 * (i % NS), (i / NS) & 1);
+            for (unsigned i = it > NS ? it - NS : 0; i < it; ++i) tc5::Waiter::drain(full + 8 * (i % NS), (i / NS) & 1);
     } else if (warp == kWiden + 1) {
         // codes: 128 rows of 256 codes, or 256 rows of 128
         for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step) {
@@ -430,23 +463,27 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
             const int s0 = t.split * per, n = min(per, all - s0);
             for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS;
-                if (!wt.wait(full_b + 8 * slot, (it / NS) & 1)) break;
-                if (lane == 0) tc5::mbar_arrive_remote(tc5::leader_addr(full_p + 8 * slot));
+                if (!wt.wait(full + 8 * slot, (it / NS) & 1)) break;
+                if (lane == 0) tc5::mbar_arrive_remote(tc5::leader_addr(full + 8 * slot));
                 __syncwarp();
             }
         }
     } else if (warp == kWiden + 2) {
         // products
+        unsigned slot = 0, par = 0;
+        bool ready = false;
         for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step, ++tiles) {
             const int s0 = t.split * per, n = min(per, all - s0);
             const uint32_t idesc = tc5::idesc_f16(BF16, (t.rows + 31) & ~31, DX, false);
             if (!wt.wait(drained, (tiles & 1) ^ 1)) break;
-            for (int s = 0; s < n; ++s, ++it) {
-                const int slot = it % NS;
-                const unsigned par = (it / NS) & 1;
-                if (!wt.wait(full_b + 8 * slot, par) || !wt.wait(full_p + 8 * slot, par) || !wt.wait(full_a + 8 * slot, par)) break;
+            for (int s = 0; s < n; ++s) {
+                if (!ready && !wt.wait(full + 8 * slot, par)) break;
                 tc5::fence_after();
                 const uint64_t b = tc5::desc128(sb + slot * C::kB, 16, 1024), a = tc5::desc128(sa + slot * C::kA, 8192, 1024);
+                // whether the next stage is there: asked for before this one's products are issued, since the answer takes as
+                // long as they do
+                const unsigned next = slot + 1 == NS ? 0 : slot + 1, npar = par ^ (slot + 1 == NS);
+                ready = __all_sync(0xffffffffu, tc5::mbar_test(full + 8 * next, npar));
                 if (tc5::elect()) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -456,6 +493,8 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                     tc5::commit(empty + 8 * slot);
                 }
                 __syncwarp();
+                slot = next;
+                par = npar;
             }
             if (!wt.fail && tc5::elect()) tc5::commit(done);
             __syncwarp();
@@ -465,52 +504,79 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
             __syncwarp();
             tc5::Waiter::drain(misc + 8, 0);
         }
+    } else if (warp == kWiden + 3) {
+        // scales, two chunks' loads ahead of the ring
+        const int64_t groups = w.K >> w.gshift;
+        const bool packed = (w.K & (DX ? 127 : 255)) == 0;
+        // bytes of the kept words that are a pair's: those of pieces 2 i and 2 i + 1
+        const int shift = packed ? w.gshift - 5 : 0;
+        uint32_t pick[DX ? 2 : 4];
+#pragma unroll
+        for (int i = 0; i < (DX ? 2 : 4); ++i) pick[i] = uint32_t((2 * i) >> shift) | uint32_t((2 * i + 1) >> shift) << 4;
+        int64_t tile = first;
+        int c = 0, n = 0;       // chunk's first stage in the tile, its stages
+        bool on = true;
+        Scales a, b;
+        auto fetch = [&](Scales &v) -> bool {   // the next chunk's; false beyond the last
+            if (c >= n) {
+                if (!on || !(on = find.find(runs, tile, t))) return false;
+                tile += step;
+                c = 0;
+                n = min(per, all - t.split * per);
+            }
+            const int64_t k0 = int64_t(t.split * per + c) * 64, mrow = t.mat * w.N, col = (int64_t(t.wt) * 2 + rank) * 128;
+            const int64_t row = DX ? k0 : col;
+            load_scales<DX>(v, w, packed, w.scales + (mrow + row) * groups, groups, int(min(w.N - row, int64_t(DX ? 256 : 128))), DX ? col : k0);
+            c += 4;
+            return true;
+        };
+        unsigned slot = 0, par = 1;
+        auto put = [&](const Scales &v) -> bool {
+            if (!wt.wait(empty_c + 8 * slot, par)) return false;
+            uint8_t *const to = smem_raw + (se + slot * C::kE - smem_at);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int i = DX ? j & 1 : j & 3, r = DX ? j >> 1 : j >> 2, at = i * (DX ? 256 : 128) + r * 32;   // [half][row n] or [stage][row n]
+                reinterpret_cast<unsigned short *>(to)[at + lane] =
+                    (unsigned short)(DX ? __byte_perm(v.w[r], 0, pick[i]) : __byte_perm(v.w[2 * r], v.w[2 * r + 1], pick[i]));
+            }
+            __syncwarp();
+            if (lane == 0) tc5::mbar_arrive(full_c + 8 * slot);
+            if (++slot == NC) { slot = 0; par ^= 1; }
+            return true;
+        };
+        bool more_a = fetch(a), more_b = more_a && fetch(b);
+        while (more_a) {
+            if (!put(a)) break;
+            more_a = more_b && fetch(a);
+            if (!more_b || !put(b)) break;
+            more_b = more_a && fetch(b);
+        }
     } else {
         // widen, then write the result
         const int stage = warp >> 2, quad = warp & 3;      // of each chunk; lanes of tensor memory
-        const int64_t groups = w.K >> w.gshift;
         unsigned cslot = 0, cpar = 0, slot0 = 0, par0 = 1;   // chunk slot and parity; the chunk's first stage and its parity of `empty`
-        const unsigned full_a0 = tc5::leader_addr(full_a), drained0 = tc5::leader_addr(drained);
+        const unsigned full0 = tc5::leader_addr(full), drained0 = tc5::leader_addr(drained);
         const bool wide = runs.splits == 1 && !((o.ld | o.J) & 1) && !(reinterpret_cast<uintptr_t>(o.out) & 3);
+        // this lane's scales in a chunk's table: forward those of its row and stage, DX of its row n and half
+        const int eat = DX ? (quad >> 1) * 256 + stage * 64 + (quad & 1) * 32 + lane : stage * 128 + quad * 32 + lane;
         Tile prev = {}, next = {};
         bool have = false, more = find.find(runs, first, next);   // `prev` has still to be written
         for (int64_t tile = first; !wt.fail; tile += step) {
             const bool live = more;
             int n = 0;
-            bool in = false;
-            const uint8_t *e0 = nullptr;
-            uint32_t eraw = 0;
-            const int s0 = next.split * per, wtile = next.wt * 2 + int(rank);
-            // scale bytes of this warp's stage of the chunk at stage c
-            auto scales_at = [&](int c) -> uint32_t {
-                if (DX) {
-                    const int nn = (s0 + c + stage) * 64 + (quad & 1) * 32 + lane;
-                    return nn < w.N ? scale_pair(w, e0 + nn * groups, int64_t(wtile) * 128 + (quad >> 1) * 64) : 0u;
-                }
-                return in ? scale_pair(w, e0, int64_t(s0 + c + stage) * 64) : 0u;
-            };
             if (live) {
                 t = next;
                 more = find.find(runs, tile + step, next);
-                n = min(per, all - s0);
-                const int64_t row = int64_t(wtile) * 128 + quad * 32 + lane;   // forward: this lane's weight row
-                in = row < w.N;
-                e0 = w.scales + (t.mat * w.N + (DX || !in ? 0 : row)) * groups;
-                eraw = scales_at(0);
-                if (!DX && more && stage == 0) {   // the next tile's scales on their way to L2
-                    const int64_t r = next.mat * w.N + min(int64_t(next.wt * 2 + int(rank)) * 128 + quad * 32 + lane, w.N - 1);
-                    asm volatile("prefetch.global.L2 [%0];" :: "l"(w.scales + r * groups + ((int64_t(next.split) * per * 64) >> w.gshift)));
-                }
+                n = min(per, all - t.split * per);
             }
             int c = 0;
             do {
                 if (live) {
-                    const uint32_t ecur = eraw;
-                    if (c + 4 < n) eraw = scales_at(c + 4);   // a chunk ahead
                     const unsigned wrap = slot0 + stage >= NS, slot = slot0 + stage - (wrap ? NS : 0);
-                    const uint32_t ep = e4m3_pair(ecur);
-                    const typename Halves<BF16>::Scale e[2] = {Halves<BF16>::scale(ep, 0), Halves<BF16>::scale(ep, 1)};
                     if (!wt.wait(full_c + 8 * cslot, cpar)) break;
+                    const uint32_t ep = e4m3_pair(reinterpret_cast<const unsigned short *>(smem_raw + (se + cslot * C::kE - smem_at))[eat]);
+                    const typename Halves<BF16>::Scale e[2] = {Halves<BF16>::scale(ep, 0), Halves<BF16>::scale(ep, 1)};
                     if (DX) {
                         // row rr of 128 codes (64 bytes, 64-byte swizzle): this warp's 64 values are pieces 2 h, 2 h + 1
                         const int rr = stage * 64 + (quad & 1) * 32 + lane, h = quad >> 1;
@@ -540,7 +606,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                         tc5::fence_before();
                     }
                     __syncwarp();
-                    if (lane == 0) tc5::mbar_arrive_remote(full_a0 + 8 * slot);
+                    if (lane == 0) tc5::mbar_arrive_remote(full0 + 8 * slot);
                     __syncwarp();
                     if (lane == 0) tc5::mbar_arrive(empty_c + 8 * cslot);
                     slot0 += 4;

@@ -106,8 +106,10 @@ def enc_q4(W, group: int = 32) -> Q4:
     codes = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=dev)
     scales = torch.empty((*lead, rows, cols // group), dtype=torch.float8_e4m3fn, device=dev)
     scale = torch.empty(tuple(lead), dtype=torch.float32, device=dev)
+    nbytes = _workspace_bytes("uq_q4_encode", mats, rows, cols)
+    ws = _scratch(nbytes, dev)
     _run(dev, _lib.load().uq_q4_encode, "enc_q4", w.data_ptr(), _CODE[w.dtype], mats, rows, cols, cols, group, codes.data_ptr(),
-         scales.data_ptr(), scale.data_ptr())
+         scales.data_ptr(), scale.data_ptr(), D.ptr(ws), nbytes)
     return Q4(codes, scales, scale)
 
 
