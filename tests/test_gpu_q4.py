@@ -598,3 +598,109 @@ def test_streams_and_captured_graphs():
         torch.cuda.synchronize()
         for gr, t, d, out in graphs:
             assert torch.equal(out[0], want[i][0]) and torch.equal(out[1], want[i][1])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows,n0,T,group", [(40, 300, 5, 32), (130, 1024, 40, 64), (24, 14336, 3, 256), (64, 96, 33, 128)])
+def test_recipe_layer(rows, n0, T, group, dt):
+    """pipeline.quant_q4_device: the layer is What x without What, and its error sums are those of What."""
+    from ultraquant_b200 import pipeline
+    rng = np.random.RandomState(n0)
+    W = torch.from_numpy(rng.standard_t(4, size=(rows, n0)) * 0.02).cuda()
+    H = torch.from_numpy(np.exp(rng.standard_normal(n0))).cuda()
+    layer = pipeline.quant_q4_device(W, H, group)
+    What = layer.What()
+    n = layer.signs.numel()
+    sH = torch.maximum(H, H.max() * 1e-3).sqrt()
+    # the codes are the restated encoder's of the rotated matrix
+    import oracle
+    X = oracle.rht_rows((W * sH).cpu().numpy())
+    codes, e, s = O4.encode(X, group)
+    assert np.array_equal(layer.w.codes.cpu().numpy(), codes) and np.array_equal(layer.w.scales.view(torch.uint8).cpu().numpy(), e)
+    Xq = O4.decode(codes, e, s, group)
+    assert abs(layer.wnmse - ((X - Xq) ** 2).sum() / (X ** 2).sum()) <= 1e-12
+    ref = oracle.irht_rows(Xq, n0) / sH.cpu().numpy()
+    assert np.abs(What.double().cpu().numpy() - ref).max() <= 2.0 ** -23 * np.abs(ref).max() + 1e-30      # float32 of a float64 value
+    x = acts(T, n0, DT[dt], 1).requires_grad_()
+    y = layer(x)
+    # rotated activations: float32 transform (log2 n + 3 roundings of values of at most the row's length), one rounding to dt
+    xr = torch.from_numpy(oracle.rht_rows((x.detach().double() / sH).cpu().numpy())).cuda()
+    norm = xr.norm(dim=1, keepdim=True)
+    dxr = HALF[DT[dt]] * xr.abs() + (np.log2(n) + 6) * 2 * U * norm + TINY[DT[dt]]
+    Q = torch.from_numpy(Xq).cuda()
+    exact = xr @ Q.T
+    bound = dxr @ Q.abs().T + 2 * (n + 2) * U * ((xr.abs() + dxr) @ Q.abs().T)
+    off = (y.detach().double() - exact).abs()
+    assert (off <= bound * (1 + HALF[DT[dt]]) + HALF[DT[dt]] * exact.abs() + TINY[DT[dt]]).all()
+    # gradient with respect to x: through the product's dx (rounded to dt) and the transform back
+    dy = acts(T, rows, DT[dt], 2)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    g = dy.double() @ Q
+    dg = HALF[DT[dt]] * g.abs() + 2 * (rows + 2) * U * (dy.double().abs() @ Q.abs()) + TINY[DT[dt]]
+    back = torch.from_numpy(oracle.irht_rows(g.cpu().numpy(), n0)).cuda() / sH
+    tol = ((dg.norm(dim=1, keepdim=True) + (np.log2(n) + 6) * 2 * U * g.norm(dim=1, keepdim=True)) / sH.float().double())
+    assert ((dx.double() - back).abs() <= tol * 1.001 + HALF[DT[dt]] * (back.abs() + tol) + TINY[DT[dt]]).all()
+    with pytest.raises(ValueError):
+        layer(x[:, :-1])
+    with pytest.raises(TypeError):
+        layer(x.float())
+
+
+def test_a_model_of_them():
+    """Lookup, rotated projection, experts and head as a model runs them: a prompt and then single tokens give the same
+    results within counted rounding, and a tuning step on all group scales goes through every operator's gradient."""
+    from ultraquant_b200 import pipeline
+    m = q4()
+    V, d, f, E = 300, 256, 384, 4
+    rng = np.random.RandomState(5)
+    weights = lambda *s: torch.from_numpy(rng.standard_normal(s) / np.sqrt(s[-1])).cuda()
+    table = m.enc_q4(weights(V, d), 32)
+    up = pipeline.quant_q4_device(weights(f, d), torch.from_numpy(np.exp(rng.standard_normal(d))).cuda(), 64)
+    ex = m.enc_q4(weights(E, d, f), 128)
+    head = m.enc_q4(weights(V, d), 64)
+    tok = torch.from_numpy(rng.randint(0, V, 37)).cuda()
+    which = torch.from_numpy(rng.randint(0, E - 1, 37)).cuda()          # the last expert gets nothing
+    order = torch.argsort(which, stable=True)
+    off = torch.cat([torch.zeros(1, dtype=torch.long, device="cuda"), torch.bincount(which, minlength=E).cumsum(0)]).int()
+
+    def run(tok, order, off, p=(None, None, None, None)):
+        h = m.embedding(tok, table, 4.0, p[0])
+        u = up(h, p[1])
+        y = m.grouped_linear(u[order], off, ex, p[2])
+        back = torch.empty_like(y).index_copy(0, order, y) + h
+        return h, u, back, m.linear(back, head, p[3])
+
+    h, u, back, logits = run(tok, order, off)
+    # one token at a time: the same products through the kernels for few rows
+    H = HALF[torch.bfloat16]
+    for t in (0, 20, 36):
+        one = torch.zeros(1, dtype=torch.long, device="cuda")
+        o1 = torch.where(torch.arange(E + 1, device="cuda") > which[t], 1, 0).int()
+        h1, u1, b1, l1 = run(tok[t : t + 1], one, o1)
+        assert torch.equal(h1[0], h[t])
+        # each stage: twice its own rounding, and what the stage before may differ by times the sizes of its weights
+        du = 2 * H * u[t].double().abs() * 1.01 + 1e-5
+        assert ((u1[0].double() - u[t].double()).abs() <= du).all()
+        we = m.deq_q4(ex)[which[t]].double().abs()
+        db = we @ du + 4 * H * (back[t].double().abs() + h[t].double().abs()) * 1.01 + 1e-5
+        assert ((b1[0].double() - back[t].double()).abs() <= db).all()
+        dl = m.deq_q4(head).double().abs() @ db + 2 * H * logits[t].double().abs() * 1.01 + 1e-5
+        assert ((l1[0].double() - logits[t].double()).abs() <= dl).all()
+    # the tuning step: gradients of the whole equal those of the pieces, called one by one
+    p = [w.group_scales().requires_grad_() for w in (table, up.w, ex, head)]
+    g = acts(37, V, torch.bfloat16, 3)
+    h, u, back, logits = run(tok, order, off, p)
+    grads = torch.autograd.grad(logits, p, g, retain_graph=True)
+    gb, gh = torch.autograd.grad(logits, (back, p[3]), g, retain_graph=True)
+    assert torch.equal(gh, grads[3])
+    gu, ge = torch.autograd.grad(back, (u, p[2]), gb, retain_graph=True)
+    assert torch.equal(ge, grads[2])
+    ghh, gup = torch.autograd.grad(u, (h, p[1]), gu, retain_graph=True)
+    assert torch.equal(gup, grads[1])
+    (gt,) = torch.autograd.grad(h, p[0], ghh + gb)
+    assert torch.equal(gt, grads[0])
+    # the new scales are stored and used
+    with torch.no_grad():
+        new = m.round_scales(head, p[3] - 0.1 * grads[3] * p[3].abs().mean() / grads[3].abs().mean())
+    assert not torch.equal(m.linear(back, new), logits)
+    assert torch.equal(new.codes, head.codes)

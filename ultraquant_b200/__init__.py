@@ -6,6 +6,7 @@ Modules mirror the reference's interfaces:
 * ``ultraquant_b200.trellis``  -- codebook, trellis_quant, trellis_quant_fast
 * ``ultraquant_b200.qat``      -- trellis_encode, fwht_torch, irht_torch, recon_torch
 * ``ultraquant_b200.q8``       -- enc_q8 / deq_q8 (Q8_0 blocks of the GGUF container)
+* ``ultraquant_b200.q4``       -- 4-bit weights with group scales: codec, linear, grouped_linear, embedding
 * ``ultraquant_b200.pipeline`` -- the builders' importance-weighted recipes
 * ``ultraquant_b200.shard``    -- row-block sharding over torch.distributed ranks
 

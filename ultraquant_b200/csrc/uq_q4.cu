@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, i
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) best = max(best, warp_top[i]);
-    const float s = scale_for(best, 11);
+    const float s = scale_for(best, 11), inv = __fdiv_rn(0.125f, s);   // s >= 2^-117, and below 2^118: inv is a normal number
     if (blockIdx.x == 0 && threadIdx.x == 0) scale[blockIdx.y] = s;
     W += blockIdx.y * mat_stride;
     codes += blockIdx.y * a.words;
@@ -139,33 +139,61 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, i
         for (int u = 0; u < kWords; ++u) {
             const int64_t i = span * 256 * kWords + u * 256 + threadIdx.x;
             const float (&x)[8] = xs[u];
-            const uint32_t m = group_top(x, lanes);
-            // the first value of that size: place in the group and sign, the least of (place, sign)
             const int sub = int(threadIdx.x) & (lanes - 1);
-            uint32_t first = 0xffffffffu;
+            // the group's largest and smallest value; `odd` is NaN where one is not finite
+            float hi = x[0], lo = x[0], odd = 0.0f;
 #pragma unroll
-            for (int j = 7; j >= 0; --j)
-                if ((__float_as_uint(x[j]) & 0x7fffffffu) == m) first = uint32_t(sub * 8 + j) * 2 + (__float_as_uint(x[j]) >> 31);
-            for (int o = lanes >> 1; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+            for (int j = 0; j < 8; ++j) {
+                hi = fmaxf(hi, x[j]);
+                lo = fminf(lo, x[j]);
+                odd = fmaf(x[j], 0.0f, odd);
+            }
+            for (int o = lanes >> 1; o > 0; o >>= 1) {
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                odd += __shfl_xor_sync(0xffffffffu, odd, o);
+            }
+            const bool finite = odd == 0.0f;
+            bool negative = -lo > hi;     // the first value of largest size
+            if (__any_sync(0xffffffffu, -lo == hi && hi != 0.0f)) {   // both signs: the one that comes first
+                uint32_t first = 0xffffffffu;
+#pragma unroll
+                for (int j = 7; j >= 0; --j)
+                    if (fabsf(x[j]) == hi) first = uint32_t(sub * 8 + j) * 2 + (x[j] < 0.0f ? 1 : 0);
+                for (int o = lanes >> 1; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+                if (-lo == hi) negative = first & 1u;
+            }
             if (i >= a.words) continue;   // whole groups: the shuffles above are over
-            // -m / (8 s): s is a power of two, so the quotient is exact (or underflows, and e4m3_of keeps its sign)
-            const float size = __fdiv_rn(__uint_as_float(m), 8.0f * s);
-            uint8_t e = m >= 0x7f800000u ? uint8_t(0x7f) : e4m3_of(size == 0.0f && m ? 0x1p-20f : size);
-            if (e != 0x7f && m && !(first & 1u)) e |= 0x80;   // a positive m takes a negative scale
+            const float m = fmaxf(hi, -lo);
+            // m / (8 s): s is a power of two, so the quotient is exact (or underflows, and e4m3_of keeps its sign)
+            const float size = m * inv;
+            uint8_t e = finite ? e4m3_of(size == 0.0f && m != 0.0f ? 0x1p-20f : size) : uint8_t(0x7f);
+            if (finite && m != 0.0f && !negative) e |= 0x80;   // a positive largest value takes a negative scale
             uint32_t word = 0x88888888u;
-            if (e != 0x7f && m) {
+            if (finite && m != 0.0f) {
                 const float c = s * e4m3_value(e), rc = __frcp_rn(c), half = 0.5f * fabsf(c);
-                word = 0;
+                constexpr float kMagic = 12582912.0f;   // 1.5 2^23: adding it rounds to a whole number, ties to even
+                float q[8];
+                bool border = false;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     // q = rint(x / c) exactly: t is within 2^-22 of x / c relatively, so rint(t) is off by at most one and
-                    // only next to a border; the remainder x - q c is exact (q c has 8 bits) and decides, ties to even
-                    float q = rintf(x[j] * rc);
-                    const float r = fmaf(-q, c, x[j]);
-                    if (fabsf(r) > half || (fabsf(r) == half && (int(q) & 1))) q += ((r < 0.0f) != (c < 0.0f)) ? -1.0f : 1.0f;
-                    const int v = int(fminf(fmaxf(q, -8.0f), 7.0f)) + 8;
-                    word |= uint32_t(v) << (4 * ((j >> 1) + 4 * (j & 1)));
+                    // only next to a border; the remainder x - q c is exact (q c has 8 bits) and shows it
+                    q[j] = (x[j] * rc + kMagic) - kMagic;
+                    border |= fabsf(fmaf(-q[j], c, x[j])) >= half;
                 }
+                if (border) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float r = fmaf(-q[j], c, x[j]);
+                        if (fabsf(r) > half || (fabsf(r) == half && (int(q[j]) & 1))) q[j] += ((r < 0.0f) != (c < 0.0f)) ? -1.0f : 1.0f;
+                    }
+                }
+                // q + 8 in four bits each, gathered in floats of 16 bits: elements 0 2 4 6 and 1 3 5 7
+                float pack[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int j = 7; j >= 0; --j) pack[j & 1] = fmaf(pack[j & 1], 16.0f, fminf(fmaxf(q[j], -8.0f), 7.0f) + 8.0f);
+                word = __byte_perm(__float_as_uint(pack[0] + 8388608.0f), __float_as_uint(pack[1] + 8388608.0f), 0x5410);
             }
             codes[i] = word;
             if (sub == 0) scales[i / lanes] = e;
@@ -173,31 +201,43 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, i
     }
 }
 
+// A thread writes 16 bytes at a time, so that a warp's store is one run of lines:
+// eight values of 16 bits, or (float32) the four of half a word.
 template <typename T>
 __global__ void __launch_bounds__(256) q4_decode_kernel(const uint32_t *codes, const uint8_t *scales, const float *scale, int64_t words, int lshift, T *out) {
+    constexpr int P = 16 / int(sizeof(T)), H = 8 / P;   // values a store, stores a word
     const float s = __ldg(scale + blockIdx.y);
     codes += blockIdx.y * words;
     scales += blockIdx.y * (words >> lshift);
     out += blockIdx.y * words * 8;
-    for (int64_t base = int64_t(blockIdx.x) * 256 * kWords + threadIdx.x; base < words; base += int64_t(gridDim.x) * 256 * kWords) {
-        uint32_t w[kWords];
-        uint8_t e[kWords];
+    const int64_t n = words * H, step = int64_t(gridDim.x) * 256 * kWords;
+    uint32_t w[kWords];
+    uint8_t e[kWords];
+    auto load = [&](int64_t at) {
 #pragma unroll
         for (int u = 0; u < kWords; ++u) {
-            const int64_t i = min(base + u * 256, words - 1);
+            const int64_t i = min(at + u * 256, n - 1) / H;
             w[u] = __ldg(codes + i);
             e[u] = __ldg(scales + (i >> lshift));
         }
+    };
+    int64_t base = int64_t(blockIdx.x) * 256 * kWords + threadIdx.x;
+    if (base < n) load(base);
+    for (; base < n; base += step) {
+        uint4 r[kWords];
 #pragma unroll
         for (int u = 0; u < kWords; ++u) {
-            const int64_t i = base + u * 256;
-            if (i >= words) break;
             const float c = s * e4m3_value(e[u]);
-            float x[8];
+            const uint32_t v = H == 2 && ((base + u * 256) & 1) ? w[u] >> 8 : w[u];   // elements 4 .. 7 are 8 bits up
+            union { uint4 v4; T t[P]; } t;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = float(nibble(w[u], j) - 8) * c;
-            store8(out + i * 8, x);
+            for (int j = 0; j < P; ++j) t.t[j] = from_float<T>(q_of(v, j) * c);
+            r[u] = t.v4;
         }
+        if (base + step < n) load(base + step);   // on their way during the stores
+#pragma unroll
+        for (int u = 0; u < kWords; ++u)
+            if (base + u * 256 < n) __stcs(reinterpret_cast<uint4 *>(out) + base + u * 256, r[u]);
     }
 }
 
@@ -269,7 +309,7 @@ __global__ void __launch_bounds__(256) q4_embed_kernel(const I *tokens, int64_t 
                 if (u && !two) break;
                 float x[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = float(nibble(w[u], j) - 8) * c[u];
+                for (int j = 0; j < 8; ++j) x[j] = q_of(w[u], j) * c[u];
                 store8(out + (t * wrow + i + 256 * u) * 8, x);
             }
         }
@@ -315,26 +355,41 @@ __device__ __forceinline__ uint32_t key_at(const Keys &k, int64_t i) {
     return v < 0 ? uint32_t(k.V) : uint32_t(v);
 }
 
+// The sort's few blocks leave most SMs free: the blocks behind them clear a share
+// of the gradient, float4 [lo, hi) of it.
+struct Clear {
+    float4 *p;
+    int64_t lo, hi;
+};
+__device__ __forceinline__ bool clear_share(const Clear &z, int sorting) {
+    if (int(blockIdx.x) < sorting) return false;
+    for (int64_t i = z.lo + int64_t(blockIdx.x - sorting) * kTile + threadIdx.x; i < z.hi; i += int64_t(gridDim.x - sorting) * kTile)
+        z.p[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    return true;
+}
+
 // hist[bin * chunks + chunk]
-__global__ void __launch_bounds__(kTile) q4_hist_kernel(Keys k, int64_t T, int64_t chunk, int shift, int bits, int *hist) {
+__global__ void __launch_bounds__(kTile) q4_hist_kernel(Keys k, int64_t T, int64_t chunk, int chunks, int shift, int bits, int *hist, Clear z) {
     __shared__ int h[kMaxBins];
+    if (clear_share(z, chunks)) return;
     const int bins = 1 << bits;
     for (int b = threadIdx.x; b < bins; b += kTile) h[b] = 0;
     __syncthreads();
     const int64_t lo = int64_t(blockIdx.x) * chunk, hi = min(lo + chunk, T);
     for (int64_t i = lo + threadIdx.x; i < hi; i += kTile) atomicAdd(h + ((key_at(k, i) >> shift) & (bins - 1)), 1);
     __syncthreads();
-    for (int b = threadIdx.x; b < bins; b += kTile) hist[b * gridDim.x + blockIdx.x] = h[b];
+    for (int b = threadIdx.x; b < bins; b += kTile) hist[b * chunks + blockIdx.x] = h[b];
 }
 
 // Moves each entry to its place: entries of smaller digits, then those of the
 // same digit in earlier chunks, earlier tiles, earlier warps, earlier lanes.
-__global__ void __launch_bounds__(kTile) q4_scatter_kernel(Keys k, const uint32_t *pos_in, int64_t T, int64_t chunk, int shift, int bits,
-                                                           const int *hist, uint32_t *keys_out, uint32_t *pos_out) {
+__global__ void __launch_bounds__(kTile) q4_scatter_kernel(Keys k, const uint32_t *pos_in, int64_t T, int64_t chunk, int chunks, int shift, int bits,
+                                                           const int *hist, uint32_t *keys_out, uint32_t *pos_out, Clear z) {
     __shared__ int start[kMaxBins];
     __shared__ int wsum[kTile / 32];
     __shared__ unsigned short count[kTile / 32][kMaxBins];
-    const int bins = 1 << bits, chunks = gridDim.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (clear_share(z, chunks)) return;
+    const int bins = 1 << bits, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int total = 0, before = 0;
     if (tid < bins) {
         for (int c = 0; c < chunks; ++c) {
@@ -384,12 +439,6 @@ __global__ void __launch_bounds__(kTile) q4_scatter_kernel(Keys k, const uint32_
         __syncthreads();
         if (tid < bins) start[tid] += sum;
     }
-}
-
-__global__ void __launch_bounds__(256) q4_zero_kernel(float *p, int64_t n) {
-    const int64_t v = n / 4, step = int64_t(gridDim.x) * 256;
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < v; i += step) reinterpret_cast<float4 *>(p)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (blockIdx.x == 0 && threadIdx.x < (n & 3)) p[v * 4 + threadIdx.x] = 0.f;
 }
 
 // A block adds the rows of kSeg consecutive sorted entries, 2048 columns.  A
@@ -449,7 +498,7 @@ __global__ void __launch_bounds__(256) q4_segment_kernel(const uint32_t *keys, c
             float sum = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                sum = fmaf(float(nibble(w[u], j) - 8), acc[j], sum);
+                sum = fmaf(q_of(w[u], j), acc[j], sum);
                 acc[j] = 0.f;
             }
             for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -587,7 +636,7 @@ int uq_q4_decode(const uint8_t *codes, const uint8_t *scales, const float *scale
     if (!al16(codes) || !al16(out)) return uq::fail(UQ_ERR_INVALID, "uq_q4_decode: codes or out not 16-byte aligned");
     const int64_t words = rows * cols / 8;
     const cudaStream_t st = UQ_STREAM(stream);
-    const dim3 grid(unsigned(top_blocks(words)), unsigned(mats));
+    const dim3 grid(unsigned(top_blocks(words * (out_dtype == UQ_F32 ? 2 : 1))), unsigned(mats));
     const int ls = lane_shift(group);
     const uint32_t *cw = reinterpret_cast<const uint32_t *>(codes);
     uq::ProfScope _p("q4_decode", st);
@@ -654,17 +703,23 @@ int uq_q4_embed_dscale(const void *tokens, int tokens64, int64_t T, const void *
     if (!al16(codes) || !al16(dc) || !al16(dout) || ld % 8) return uq::fail(UQ_ERR_INVALID, "uq_q4_embed_dscale: codes, dout and dc have to be 16-byte aligned, ld a multiple of 8");
     const cudaStream_t st = UQ_STREAM(stream);
     const int64_t per = K / group;
-    { uq::ProfScope _p("q4_zero", st); q4_zero_kernel<<<blocks_for((V * per + 1023) / 1024, 8), 256, 0, st>>>(dc, V * per); }
-    if (T) {
+    if (T == 0) return cudaMemsetAsync(dc, 0, size_t(V * per) * 4, st) == cudaSuccess ? UQ_OK : uq::check_cuda("uq_q4_embed_dscale");
+    {
         const SortPlan p = sort_plan(T, V);
         const Carve c = carve(workspace, workspace_bytes, T, p, per);
         if (!workspace || c.bytes > workspace_bytes)
             return uq::fail(UQ_ERR_WORKSPACE, "uq_q4_embed_dscale: workspace of %zu bytes, %zu needed", workspace_bytes, c.bytes);
+        // the gradient is cleared beside the sort, a share in each launch; up to three odd floats at its end before
+        const int64_t vecs = V * per / 4, launches = 2 * p.passes;
+        if (V * per % 4 && cudaMemsetAsync(dc + vecs * 4, 0, size_t(V * per % 4) * 4, st) != cudaSuccess) return uq::check_cuda("uq_q4_embed_dscale");
+        const auto share = [&](int i) { return Clear{reinterpret_cast<float4 *>(dc), vecs * i / launches, vecs * (i + 1) / launches}; };
+        const unsigned grid = unsigned(p.chunks + std::min<int64_t>(uq::num_sms() * 2, (vecs / launches + kTile) / kTile));
         for (int i = 0; i < p.passes; ++i) {
             const Keys k{tokens, tokens64, V, i ? c.key[(i - 1) & 1] : nullptr};
-            { uq::ProfScope _p("q4_hist", st); q4_hist_kernel<<<p.chunks, kTile, 0, st>>>(k, T, p.chunk, i * p.bits, p.bits, c.hist); }
+            { uq::ProfScope _p("q4_hist", st); q4_hist_kernel<<<grid, kTile, 0, st>>>(k, T, p.chunk, p.chunks, i * p.bits, p.bits, c.hist, share(2 * i)); }
             { uq::ProfScope _p("q4_scatter", st);
-              q4_scatter_kernel<<<p.chunks, kTile, 0, st>>>(k, i ? c.pos[(i - 1) & 1] : nullptr, T, p.chunk, i * p.bits, p.bits, c.hist, c.key[i & 1], c.pos[i & 1]); }
+              q4_scatter_kernel<<<grid, kTile, 0, st>>>(k, i ? c.pos[(i - 1) & 1] : nullptr, T, p.chunk, p.chunks, i * p.bits, p.bits, c.hist, c.key[i & 1], c.pos[i & 1],
+                                                        share(2 * i + 1)); }
         }
         const int last = (p.passes - 1) & 1, ls = lane_shift(group);
         switch (dtype) {

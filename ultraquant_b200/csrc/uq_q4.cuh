@@ -28,6 +28,10 @@ __device__ __forceinline__ float e4m3_value(uint8_t b) {
 // Nibble of element i (0 .. 7) of a word.
 __device__ __forceinline__ int nibble(uint32_t w, int i) { return int((w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u); }
 
+// q of element i as a float: u under the significand of 2^23, less 2^23 + 8 (a
+// conversion instruction would have a quarter of the rate).
+__device__ __forceinline__ float q_of(uint32_t w, int i) { return __uint_as_float(0x4b000000u | uint32_t(nibble(w, i))) - 8388616.0f; }
+
 template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
@@ -52,7 +56,7 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float (
 #pragma unroll
     for (int i = 0; i < 8; ++i) u.t[i] = from_float<T>(x[i]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) reinterpret_cast<uint4 *>(p)[i] = u.v[i];
+    for (int i = 0; i < N; ++i) __stcs(reinterpret_cast<uint4 *>(p) + i, u.v[i]);
 }
 #endif
 

@@ -12,9 +12,10 @@ from dataclasses import dataclass
 import torch
 
 from . import _device as D
-from . import _lib
+from . import _lib, q4, qat
 
-__all__ = ["quant_trellis", "quant_step", "QuantResult", "quant_trellis_device", "quant_step_device"]
+__all__ = ["quant_trellis", "quant_step", "QuantResult", "quant_trellis_device", "quant_step_device", "quant_q4_device",
+           "Q4Layer"]
 
 
 @dataclass
@@ -159,3 +160,99 @@ def quant_step(W, H, step, block28=False, scale_search=False):
     w = D.as_device(W)
     h = D.as_device(H, torch.float64)
     return _host_result(quant_step_device(w, h, step, block28=block28, scale_search=scale_search).What, W)
+
+
+class _Rotate(torch.autograd.Function):
+    """The activations' side of the recipe: (x / sH) padded, signs, FWHT / sqrt(n), in float32, rounded to x's dtype."""
+
+    @staticmethod
+    def forward(ctx, x, sH, signs):
+        ctx.save_for_backward(sH, signs)
+        ctx.dtype = x.dtype
+        n = signs.numel()
+        x2 = x.reshape(-1, x.shape[-1]).float().contiguous()
+        # the adjoint of uq_fwht's forward direction (signs and 1 / sH behind the transform)
+        return qat._fwht_call(x2, n, signs, sH, 1, n).to(x.dtype).reshape(*x.shape[:-1], n)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        sH, signs = ctx.saved_tensors
+        n = signs.numel()
+        g2 = g.reshape(-1, n).float().contiguous()
+        return qat._fwht_call(g2, n, signs, sH, 0, sH.numel()).to(ctx.dtype).reshape(*g.shape[:-1], sH.numel()), None, None
+
+
+@dataclass
+class Q4Layer:
+    """A weight matrix quantized in the rotated, whitened domain, as a linear layer: What x = Q (FWHT (d x / sH) / sqrt(n))
+    without What being formed.  ``w``: the 4-bit codes of rht_rows(W * sH); ``scales`` of a call: the trained group scales
+    (see q4.linear)."""
+    w: q4.Q4                      # (rows, n), n = next_pow2(n0)
+    sH: torch.Tensor              # (n0,) float32
+    signs: torch.Tensor           # (n,) float32
+    err: torch.Tensor             # [sum (A - Ah)^2, sum A^2] fp64
+
+    @property
+    def wnmse(self) -> float:
+        e = self.err.double().cpu()
+        return float(e[0] / e[1])
+
+    def rotate(self, x: torch.Tensor) -> torch.Tensor:
+        """(..., n0) bfloat16 or float16 activations -> (..., n), what ``w`` is multiplied with; differentiable in x."""
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"Q4Layer: activations of dtype {x.dtype} are not built (bfloat16, float16)")
+        if x.dim() == 0 or x.shape[-1] != self.sH.numel() or x.device != self.sH.device:
+            raise ValueError(f"Q4Layer: activations {tuple(x.shape)} on {x.device} do not match {self.sH.numel()} columns on {self.sH.device}")
+        return _Rotate.apply(x, self.sH, self.signs)
+
+    def __call__(self, x: torch.Tensor, scales: torch.Tensor | None = None) -> torch.Tensor:
+        return q4.linear(self.rotate(x), self.w, scales)
+
+    def What(self) -> torch.Tensor:
+        """The reconstruction (rows, n0) float32, as the other recipes return it."""
+        return _q4_reconstruction(self.w, self.sH.double(), self.sH.numel(), self.signs.double())
+
+
+def _q4_reconstruction(w, sH, n0, signs):
+    lib = _lib.load()
+    X = q4.deq_q4(w)
+    rows, n = X.shape
+    out = torch.empty((rows, n0), dtype=torch.float64, device=X.device)
+    if out.numel():
+        _lib.check(lib.uq_irht_rows(X.data_ptr(), D.dtype_code(X), rows, n, n, n0, signs.data_ptr(), out.data_ptr(),
+                                    D.stream_handle(X.device)), "uq_irht_rows")
+    return (out / sH).float()
+
+
+def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_errors=True) -> Q4Layer:
+    """The builders' recipe (buildalloc.py:21-24: clamp the imatrix, whiten, rotate, quantize) with 4-bit codes and group
+    scales in place of the lattice (q4.enc_q4; no counterpart in the reference).  W (rows, n0) float32 / float64 and H (n0)
+    on the device; rows of up to 32768 columns.  The layer multiplies with the codes themselves."""
+    lib = _lib.load()
+    dev = W.device
+    if W.dim() != 2 or H.shape != (W.shape[1],) or W.shape[1] == 0:
+        raise ValueError(f"quant_q4: expected W (rows, n0) and H (n0), got {tuple(W.shape)} and {tuple(H.shape)}")
+    rows, n0 = W.shape
+    n = int(lib.uq_next_pow2(n0))
+    if n < group:
+        raise ValueError(f"quant_q4: {n} rotated columns are not whole groups of {group}")
+    H = H.to(device=dev, dtype=torch.float64)
+    sH = torch.maximum(H, H.max() * 1e-3).sqrt()
+    A = (W.double() * sH).contiguous()
+    d = D.signs(n, seed, dev)
+    X = torch.empty((rows, n), dtype=torch.float64, device=dev)
+    if rows:
+        _lib.check(lib.uq_rht_rows(A.data_ptr(), _lib.UQ_F64, rows, n0, n0, d.data_ptr(), X.data_ptr(), D.stream_handle(dev)),
+                   "uq_rht_rows")
+    w = q4.enc_q4(X, group)
+    err = torch.zeros(2, dtype=torch.float64, device=dev)
+    if rows:
+        Q = q4.deq_q4(w)
+        ws = torch.empty(lib.uq_wnmse_workspace_bytes(), dtype=torch.uint8, device=dev)
+        # the rotation keeps lengths: the sums in the rotated domain are the weighted ones (of the padded columns too)
+        _lib.check(lib.uq_wnmse_sums(X.data_ptr(), _lib.UQ_F64, Q.data_ptr(), _lib.UQ_F32, X.numel(), err.data_ptr(),
+                                     ws.data_ptr(), ws.numel(), D.stream_handle(dev)), "uq_wnmse_sums")
+    if check_errors:
+        _device_status(lib, dev, "quant_q4")
+    return Q4Layer(w, sH.float(), d.float(), err)
