@@ -735,28 +735,28 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
         const int per_chunk = 256 >> w.gshift;
         const bool pairs = w.gshift == 5, even = (w.K & 63) == 0;
         const uint8_t *e0 = nullptr, *e1 = nullptr;      // this lane's two rows of scales; beyond N the last row's, not written
-        uint32_t eraw[2];
+        uint32_t elo[2], ehi[2];     // the two bytes of this lane's 64 values, as they come from memory: put together when used
         auto scales_of = [&](const Tile &tt) {
             const int64_t n = int64_t(tt.wt) * kFewRows + warp * 16 + g, at = (int64_t(c0) * 256 + q * 64) >> w.gshift;
             e0 = w.scales + (tt.mat * w.N + min(n, w.N - 1)) * groups + at;
             e1 = w.scales + (tt.mat * w.N + min(n + 8, w.N - 1)) * groups + at;
         };
-        // the two rows' bytes for this lane's 64 values of chunk c (see scale_pair), then on to the next chunk
+        // the two rows' bytes for chunk c, then on to the next chunk
+        const uint32_t both = pairs ? 1u : 0x101u;   // one byte for both halves
         auto scales_at = [&](int c) {
+            elo[0] = elo[1] = ehi[0] = ehi[1] = 0;
             if (c * 256 + q * 64 < w.K) {
-                if (!pairs) {
-                    eraw[0] = __ldg(e0) * 0x101u;
-                    eraw[1] = __ldg(e1) * 0x101u;
-                } else if (even) {
-                    eraw[0] = __ldg(reinterpret_cast<const unsigned short *>(e0));
-                    eraw[1] = __ldg(reinterpret_cast<const unsigned short *>(e1));
+                if (pairs && even) {
+                    elo[0] = __ldg(reinterpret_cast<const unsigned short *>(e0));
+                    elo[1] = __ldg(reinterpret_cast<const unsigned short *>(e1));
                 } else {
-                    const bool two = c * 256 + q * 64 + 32 < w.K;
-                    eraw[0] = __ldg(e0) | (two ? uint32_t(__ldg(e0 + 1)) << 8 : 0u);
-                    eraw[1] = __ldg(e1) | (two ? uint32_t(__ldg(e1 + 1)) << 8 : 0u);
+                    elo[0] = __ldg(e0);
+                    elo[1] = __ldg(e1);
+                    if (pairs && c * 256 + q * 64 + 32 < w.K) {
+                        ehi[0] = __ldg(e0 + 1);
+                        ehi[1] = __ldg(e1 + 1);
+                    }
                 }
-            } else {
-                eraw[0] = eraw[1] = 0;
             }
             e0 += per_chunk;
             e1 += per_chunk;
@@ -773,7 +773,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
 #pragma unroll
             for (int u = 0; u < NT; ++u) tok[u] = min(g + 8 * u, t.rows - 1);
             for (int c = c0; c < c1; ++c) {
-                const uint32_t eh[2] = {e4m3_pair(eraw[0]), e4m3_pair(eraw[1])};
+                const uint32_t eh[2] = {e4m3_pair(elo[0] * both + (ehi[0] << 8)), e4m3_pair(elo[1] * both + (ehi[1] << 8))};
                 if (c + 1 < c1) {
                     scales_at(c + 1);
                 } else if (more) {   // the next tile's

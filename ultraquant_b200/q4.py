@@ -61,11 +61,20 @@ class Q4:
             raise ValueError("Q4: codes, scales and scale have to be contiguous")
         if codes.data_ptr() & 15 or scales.data_ptr() & 15:
             raise ValueError("Q4: codes and scales have to start on a 16-byte boundary")
+        self._set(codes, scales, scale, cs[0] if len(cs) == 3 else 1, cs[-2], cols, group)
+
+    def _set(self, codes, scales, scale, mats, rows, cols, group):
         self.codes, self.scales, self.scale = codes, scales, scale
-        mats = cs[0] if len(cs) == 3 else 1
-        self.mats, self.rows, self.cols, self.group, self.device = mats, cs[-2], cols, group, codes.device
+        self.mats, self.rows, self.cols, self.group, self.device = mats, rows, cols, group, codes.device
         self.ptrs = (codes.data_ptr(), scales.data_ptr(), scale.data_ptr())
-        self.form = (mats, cs[-2], cols, group)
+        self.form = (mats, rows, cols, group)
+
+    @classmethod
+    def _of(cls, codes, scales, scale, mats, rows, cols, group):
+        """Of tensors made here, which need no check."""
+        w = cls.__new__(cls)
+        w._set(codes, scales, scale, mats, rows, cols, group)
+        return w
 
     @property
     def shape(self):
@@ -87,7 +96,7 @@ def _weights(W):
         raise TypeError(f"enc_q4: dtype {W.dtype} is not built (float32, float64, bfloat16, float16)")
     if not W.is_cuda:
         W = W.to(D.device())
-    return W.contiguous()
+    return W if W.is_contiguous() else W.contiguous()
 
 
 def enc_q4(W, group: int = 32) -> Q4:
@@ -103,22 +112,22 @@ def enc_q4(W, group: int = 32) -> Q4:
         raise ValueError(f"enc_q4: {cols} columns are not whole groups of {group}")
     dev = w.device
     mats = lead[0] if lead else 1
-    codes = torch.empty((*lead, rows, cols // 2), dtype=torch.uint8, device=dev)
-    scales = torch.empty((*lead, rows, cols // group), dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty(tuple(lead), dtype=torch.float32, device=dev)
+    codes = w.new_empty((*lead, rows, cols // 2), dtype=torch.uint8)
+    scales = w.new_empty((*lead, rows, cols // group), dtype=torch.float8_e4m3fn)
+    scale = w.new_empty(tuple(lead), dtype=torch.float32)
     nbytes = _workspace_bytes("uq_q4_encode", mats, rows, cols)
     ws = _scratch(nbytes, dev)
-    _run(dev, _lib.load().uq_q4_encode, "enc_q4", w.data_ptr(), _CODE[w.dtype], mats, rows, cols, cols, group, codes.data_ptr(),
+    _run(dev, "uq_q4_encode", w.data_ptr(), _CODE[w.dtype], mats, rows, cols, cols, group, codes.data_ptr(),
          scales.data_ptr(), scale.data_ptr(), D.ptr(ws), nbytes)
-    return Q4(codes, scales, scale)
+    return Q4._of(codes, scales, scale, mats, rows, cols, group)
 
 
 def deq_q4(w: Q4, dtype=torch.float32) -> torch.Tensor:
     """The values: scale * scales * q, rounded once to ``dtype`` (float32 holds them exactly)."""
     if dtype not in _OUT:
         raise TypeError(f"deq_q4: dtype {dtype} is not built (float32, bfloat16, float16)")
-    out = torch.empty(w.shape, dtype=dtype, device=w.device)
-    _run(w.device, _lib.load().uq_q4_decode, "deq_q4", *w.ptrs, *w.form, out.data_ptr(), _OUT[dtype])
+    out = w.codes.new_empty(w.shape, dtype=dtype)
+    _run(w.device, "uq_q4_decode", *w.ptrs, *w.form, out.data_ptr(), _OUT[dtype])
     return out
 
 
@@ -127,16 +136,16 @@ def round_scales(w: Q4, scales: torch.Tensor) -> Q4:
     are shared)."""
     c = _trained(w, scales).detach().contiguous()
     e, s = torch.empty_like(w.scales), torch.empty_like(w.scale)
-    _run(w.device, _lib.load().uq_q4_round_scales, "round_scales", c.data_ptr(), w.mats, c.numel() // max(w.mats, 1), e.data_ptr(),
+    _run(w.device, "uq_q4_round_scales", c.data_ptr(), w.mats, c.numel() // max(w.mats, 1), e.data_ptr(),
          s.data_ptr())
-    return Q4(w.codes, e, s)
+    return Q4._of(w.codes, e, s, *w.form)
 
 
 def check_errors(device=None) -> None:
     """Waits for the current stream and raises what the operators' kernels have met since the last call: ValueError for a
     token or an offset out of range, UQError for a wait that gave up."""
     dev = torch.device(device) if device is not None else D.device()
-    _run(dev if dev.index is not None else D.device(), _lib.load().uq_q4_errors, "q4")
+    _run(dev if dev.index is not None else D.device(), "uq_q4_errors")
 
 
 def _trained(w: Q4, scales) -> torch.Tensor:
@@ -169,9 +178,14 @@ def _ld(x: torch.Tensor) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _run(dev: torch.device, fn, what: str, *args) -> None:
-    """fn(*args, stream) on the current stream of ``dev``, raising for its status."""
-    i = dev.index
+@lru_cache(maxsize=None)
+def _fn(name: str):
+    return getattr(_lib.load(), name)
+
+
+def _run(dev: torch.device, name: str, *args) -> None:
+    """The entry point ``name`` on the current stream of ``dev``, raising for its status."""
+    fn, i = _fn(name), dev.index
     stream = _raw_stream(i) if _raw_stream is not None else D.stream_handle(dev)
     if torch.cuda.current_device() == i:
         rc = fn(*args, stream)
@@ -179,12 +193,12 @@ def _run(dev: torch.device, fn, what: str, *args) -> None:
         with torch.cuda.device(i):
             rc = fn(*args, stream)
     if rc:
-        _lib.check(rc, what)
+        _lib.check(rc, name)
 
 
 @lru_cache(maxsize=4096)
 def _workspace_bytes(name: str, *sizes) -> int:
-    return getattr(_lib.load(), name + "_workspace_bytes")(*sizes)
+    return _fn(name + "_workspace_bytes")(*sizes)
 
 
 def _scratch(nbytes: int, dev: torch.device):
@@ -216,7 +230,7 @@ def _call(name: str, T: int, a: torch.Tensor, w: Q4, offsets, out: torch.Tensor,
     mats, rows, cols, group = w.form
     nbytes = _workspace_bytes(name, T, mats, rows, cols) if offsets is None else 0
     ws = _scratch(nbytes, w.device)
-    _run(w.device, getattr(_lib.load(), name), name, a.data_ptr(), _ACT[a.dtype], T, _ld(a), *w.ptrs, mats, rows, cols, group,
+    _run(w.device, name, a.data_ptr(), _ACT[a.dtype], T, _ld(a), *w.ptrs, mats, rows, cols, group,
          offsets.data_ptr() if offsets is not None else None, out.data_ptr(), out.stride(0) if T > 1 else out.shape[1],
          zero_rest, ws.data_ptr() if nbytes else None, nbytes)
 
@@ -259,7 +273,7 @@ class _Product(torch.autograd.Function):
             if dc.numel():
                 nbytes = _workspace_bytes("uq_q4_linear_dscale", T, *w.form)
                 ws = _scratch(nbytes, w.device)
-                _run(w.device, _lib.load().uq_q4_linear_dscale, "uq_q4_linear_dscale", D.ptr(d2), D.ptr(x2), _ACT[dy.dtype], T,
+                _run(w.device, "uq_q4_linear_dscale", D.ptr(d2), D.ptr(x2), _ACT[dy.dtype], T,
                      _ld(d2), _ld(x2), w.ptrs[0], *w.form, D.ptr(offsets), dc.data_ptr(), D.ptr(ws), nbytes)
         return dx, dc, None, None
 
@@ -322,15 +336,15 @@ class _Embedding(torch.autograd.Function):
         if dc.numel():
             nbytes = _workspace_bytes("uq_q4_embed_dscale", T, *w.form[1:])
             ws = _scratch(nbytes, w.device)
-            _run(w.device, _lib.load().uq_q4_embed_dscale, "uq_q4_embed_dscale", D.ptr(tokens), tokens.dtype == torch.int64, T,
+            _run(w.device, "uq_q4_embed_dscale", D.ptr(tokens), tokens.dtype == torch.int64, T,
                  D.ptr(d2), _OUT[d2.dtype], _ld(d2), w.ptrs[0], *w.form[1:], ctx.alpha, dc.data_ptr(), D.ptr(ws), nbytes)
         return None, dc, None, None, None
 
 
 def _lookup(tokens, w, alpha, dtype):
-    out = torch.empty((*tokens.shape, w.cols), dtype=dtype, device=w.device)
+    out = w.codes.new_empty((*tokens.shape, w.cols), dtype=dtype)
     if out.numel():
-        _run(w.device, _lib.load().uq_q4_embed, "embedding", tokens.data_ptr(), tokens.dtype == torch.int64, tokens.numel(), *w.ptrs,
+        _run(w.device, "uq_q4_embed", tokens.data_ptr(), tokens.dtype == torch.int64, tokens.numel(), *w.ptrs,
              *w.form[1:], alpha, out.data_ptr(), _OUT[dtype])
     return out
 
