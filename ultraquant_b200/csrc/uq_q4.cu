@@ -105,11 +105,11 @@ template <typename T> __global__ void __launch_bounds__(256) q4_top_kernel(const
     }
 }
 
+// `lanes`: threads of a group, eight values each (a constant: the reductions unroll).
 // The second reading goes backwards: what the first read last is still in L2.
-template <typename T>
+template <typename T, int lanes>
 __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, int64_t mat_stride, const uint32_t *top, float *scale, uint32_t *codes, uint8_t *scales) {
     __shared__ uint32_t warp_top[8];
-    const int lanes = a.group / 8;
     uint32_t best = 0;
     for (int i = threadIdx.x; i < a.blocks; i += 256) best = max(best, top[int64_t(blockIdx.y) * a.blocks + i]);
     best = __reduce_max_sync(0xffffffffu, best);
@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, i
                 lo = fminf(lo, x[j]);
                 odd = fmaf(x[j], 0.0f, odd);
             }
+#pragma unroll
             for (int o = lanes >> 1; o > 0; o >>= 1) {
                 hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
                 lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, i
                 word = __byte_perm(__float_as_uint(pack[0] + 8388608.0f), __float_as_uint(pack[1] + 8388608.0f), 0x5410);
             }
             codes[i] = word;
-            if (sub == 0) scales[i / lanes] = e;
+            if (sub == 0) scales[uint64_t(i) / lanes] = e;
         }
     }
 }
@@ -556,7 +557,16 @@ int encode(const T *W, int64_t mats, int64_t rows, int64_t cols, int64_t ldw, in
     a.flat = ldw == cols;
     const dim3 grid(unsigned(a.blocks), unsigned(mats));
     { uq::ProfScope _p("q4_top", st); q4_top_kernel<T><<<grid, 256, 0, st>>>(W, a, rows * ldw, top); }
-    { uq::ProfScope _p("q4_encode", st); q4_encode_kernel<T><<<grid, 256, 0, st>>>(W, a, rows * ldw, top, scale, reinterpret_cast<uint32_t *>(codes), scales); }
+    {
+        uq::ProfScope _p("q4_encode", st);
+        uint32_t *const cw = reinterpret_cast<uint32_t *>(codes);
+        switch (group) {
+            case 32: q4_encode_kernel<T, 4><<<grid, 256, 0, st>>>(W, a, rows * ldw, top, scale, cw, scales); break;
+            case 64: q4_encode_kernel<T, 8><<<grid, 256, 0, st>>>(W, a, rows * ldw, top, scale, cw, scales); break;
+            case 128: q4_encode_kernel<T, 16><<<grid, 256, 0, st>>>(W, a, rows * ldw, top, scale, cw, scales); break;
+            default: q4_encode_kernel<T, 32><<<grid, 256, 0, st>>>(W, a, rows * ldw, top, scale, cw, scales); break;
+        }
+    }
     return uq::check_cuda("q4_encode_kernel launch");
 }
 

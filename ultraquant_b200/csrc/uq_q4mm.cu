@@ -215,9 +215,6 @@ struct Weights {
 // are stored.
 struct Scales { uint32_t w[8]; };
 
-__device__ __forceinline__ uint32_t load_bytes(const uint8_t *p, int bytes) {
-    return bytes == 4 ? __ldg(reinterpret_cast<const unsigned *>(p)) : bytes == 2 ? __ldg(reinterpret_cast<const unsigned short *>(p)) : __ldg(p);
-}
 // Bytes of the four pieces from value k on, 0 beyond K.
 __device__ __forceinline__ uint32_t gather4(const Weights &w, const uint8_t *row, int64_t k) {
     uint32_t v[4];
@@ -225,30 +222,43 @@ __device__ __forceinline__ uint32_t gather4(const Weights &w, const uint8_t *row
     for (int i = 0; i < 4; ++i) v[i] = k + 32 * i < w.K ? __ldg(row + ((k + 32 * i) >> w.gshift)) : 0u;
     return v[0] | v[1] << 8 | v[2] << 16 | v[3] << 24;
 }
-// Rows lane + 32 j (below `rows`) from value k on; `p`: the first row's bytes.
+// Rows lane + 32 j (below `rows`) of `groups` bytes each, from `p` on: a word of
+// WORD's size of each, 0 for a row that is not there.
+template <typename WORD, int R> __device__ __forceinline__ void load_rows(uint32_t (&w)[8], const uint8_t *p, int64_t groups, int rows) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        WORD v = {};
+        if (lane + 32 * j < rows) v = __ldg(reinterpret_cast<const WORD *>(p + (lane + 32 * j) * groups));
+        if constexpr (sizeof(WORD) == 8) {
+            w[2 * j] = v.x;
+            w[2 * j + 1] = v.y;
+        } else {
+            w[8 / R * j] = v;
+        }
+    }
+}
+// The scales from value k on; `p`: the first row's bytes.
 template <bool DX>
 __device__ __forceinline__ void load_scales(Scales &v, const Weights &w, bool packed, const uint8_t *p, int64_t groups, int rows, int64_t k) {
     constexpr int R = DX ? 8 : 4, W = 8 / R;   // rows, words of each
-    const int lane = threadIdx.x & 31, bytes = max((DX ? 128 : 256) >> w.gshift, 1);
+    const int bytes = (DX ? 128 : 256) >> w.gshift;
     if (k >= w.K) rows = 0;                    // DX: columns beyond the matrix
+    const uint8_t *const at = p + (k >> w.gshift);
+    if (!packed) {
+        const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-        const bool in = lane + 32 * j < rows;
-        const uint8_t *const row = p + (in ? lane + 32 * j : 0) * groups;
+        for (int j = 0; j < R; ++j)
 #pragma unroll
-        for (int i = 0; i < W; ++i) v.w[W * j + i] = 0;
-        if (!in) continue;
-        const uint8_t *const at = row + (k >> w.gshift);
-        if (!packed) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) v.w[W * j + i] = gather4(w, row, k + 128 * i);
-        } else if (W == 2 && bytes == 8) {
-            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(at));
-            v.w[W * j] = u.x;
-            v.w[W * j + W - 1] = u.y;
-        } else {
-            v.w[W * j] = load_bytes(at, bytes);
-        }
+            for (int i = 0; i < W; ++i) v.w[W * j + i] = lane + 32 * j < rows ? gather4(w, p + (lane + 32 * j) * groups, k + 128 * i) : 0u;
+    } else if (W == 2 && bytes == 8) {
+        if constexpr (W == 2) load_rows<uint2, R>(v.w, at, groups, rows);
+    } else if (bytes == 4) {
+        load_rows<unsigned, R>(v.w, at, groups, rows);
+    } else if (bytes == 2) {
+        load_rows<unsigned short, R>(v.w, at, groups, rows);
+    } else {
+        load_rows<unsigned char, R>(v.w, at, groups, rows);
     }
 }
 
