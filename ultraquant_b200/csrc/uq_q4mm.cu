@@ -34,7 +34,8 @@ struct Tile {
 
 // Finds a warp's tiles in rising order: the 32 lanes hold 32 matrices' runs at a
 // time.  An offset counts as at least its predecessors and at most T.
-struct Finder {
+// RUNS: whether there are offsets; without them none of the state is kept.
+template <bool RUNS> struct Finder {
     int first, lo, incl, top, begin;   // matrices before this block of 32; this lane's run: first row, row tiles up to its end
     int64_t base;                      // row tiles before this block
     bool loaded;
@@ -44,7 +45,7 @@ struct Finder {
         base = 0;
         loaded = false;
         top = 0;
-        if (r.offsets) {
+        if (RUNS) {
             const int o = r.offsets[0];
             top = min(max(o, 0), int(r.T));
             if (o != top) g_mm_bad_offset = 1;
@@ -77,30 +78,30 @@ struct Finder {
         const int64_t u = runs_split(r, t, tile.split);
         const int64_t rt = u / r.wtiles;
         tile.wt = int(u - rt * r.wtiles);
-        if (!r.offsets) {
+        if constexpr (!RUNS) {
             tile.mat = 0;
             if (rt * r.bt >= r.T) return false;
             tile.row0 = int(rt) * r.bt;
             tile.rows = min(int(r.T) - tile.row0, r.bt);
-            return true;
-        }
-        for (;;) {
-            if (!loaded) {
-                if (first >= r.mats) return false;
-                load(r);
+        } else {
+            for (;;) {
+                if (!loaded) {
+                    if (first >= r.mats) return false;
+                    load(r);
+                }
+                const int all = __shfl_sync(0xffffffffu, incl, 31);
+                if (rt < base + all) break;
+                base += all;
+                first += 32;
+                loaded = false;
             }
-            const int all = __shfl_sync(0xffffffffu, incl, 31);
-            if (rt < base + all) break;
-            base += all;
-            first += 32;
-            loaded = false;
+            const int at = __popc(__ballot_sync(0xffffffffu, base + incl <= rt));   // runs that end before the tile
+            const int before = __shfl_sync(0xffffffffu, incl, at > 0 ? at - 1 : 0);
+            const int l = __shfl_sync(0xffffffffu, lo, at), next = __shfl_sync(0xffffffffu, lo, at < 31 ? at + 1 : 31);
+            tile.mat = first + at;
+            tile.row0 = l + int(rt - base - (at > 0 ? before : 0)) * r.bt;
+            tile.rows = min((at < 31 ? next : top) - tile.row0, r.bt);
         }
-        const int at = __popc(__ballot_sync(0xffffffffu, base + incl <= rt));   // runs that end before the tile
-        const int before = __shfl_sync(0xffffffffu, incl, at > 0 ? at - 1 : 0);
-        const int l = __shfl_sync(0xffffffffu, lo, at), next = __shfl_sync(0xffffffffu, lo, at < 31 ? at + 1 : 31);
-        tile.mat = first + at;
-        tile.row0 = l + int(rt - base - (at > 0 ? before : 0)) * r.bt;
-        tile.rows = min((at < 31 ? next : top) - tile.row0, r.bt);
         return true;
     }
     static __device__ __forceinline__ int64_t runs_split(const Runs &r, int64_t t, int &split) {
@@ -112,7 +113,7 @@ struct Finder {
         return t / r.splits;
     }
     // The end of the last run, once find() has gone beyond the last tile.
-    __device__ __forceinline__ int64_t end(const Runs &r) const { return r.offsets ? top : r.T; }
+    __device__ __forceinline__ int64_t end(const Runs &r) const { return RUNS ? top : r.T; }
 };
 
 // ----------------------------------------------------------------------------
@@ -383,7 +384,7 @@ template <int BT, bool DX> struct Cfg {
     static_assert(DX || BT + 32 * NS <= 512, "tensor memory");
 };
 
-template <int BT, bool BF16, bool DX>
+template <int BT, bool BF16, bool DX, bool RUNS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_codes, Runs runs, Weights w, Out o) {
     using C = Cfg<BT, DX>;
@@ -421,7 +422,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     const unsigned tmem_a = tmem + BT;
 
     tc5::Waiter wt{gave_up, &g_mm_timeout};
-    Finder find;
+    Finder<RUNS> find;
     find.start(runs);
     Tile t;
     const int64_t step = gridDim.x >> 1, first = blockIdx.x >> 1;                 // pairs
@@ -643,7 +644,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
             prev = t;
             have = true;
         }
-        if (o.zero_rest && runs.offsets && !wt.fail) zero_rows<typename Halves<BF16>::T>(o, find.begin, find.end(runs), kWiden * 32);
+        if (RUNS && o.zero_rest && !wt.fail) zero_rows<typename Halves<BF16>::T>(o, find.begin, find.end(runs), kWiden * 32);
     }
     tc5::fence_before();
     __syncthreads();
@@ -691,7 +692,7 @@ template <int NT> struct FewCfg {
     static_assert(kStage % 1024 == 0 && kBlocks * (kSmem + 1024) <= 233472, "shared memory of an SM");
 };
 
-template <bool BF16, int NT>
+template <bool BF16, int NT, bool RUNS>
 __global__ void __launch_bounds__(kFewThreads, FewCfg<NT>::kBlocks)
 q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_codes, Runs runs, Weights w, Out o, int box) {
     using T = typename Halves<BF16>::T;
@@ -701,7 +702,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
     const unsigned smem_at = tc5::smem_addr(smem_raw), base = (smem_at + 1023u) & ~1023u, sums_at = base + NS * C::kStage, full = sums_at + C::kSums, empty = full + 8 * NS, misc = empty + 8 * NS;
     volatile int *gave_up = reinterpret_cast<volatile int *>(smem_raw + (misc - smem_at));
     const int warp = tc5::warp_id(), lane = threadIdx.x & 31;
-    const int parts = runs.splits, part = parts > 1 ? int(tc5::cluster_rank()) : 0;   // blocks of a cluster: parts of k
+    const int parts = RUNS ? 1 : runs.splits, part = parts > 1 ? int(tc5::cluster_rank()) : 0;   // blocks of a cluster: parts of k
     if (threadIdx.x == 0) {
         *gave_up = 0;
         for (int i = 0; i < NS; ++i) {
@@ -712,7 +713,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
     }
     __syncthreads();
     tc5::Waiter wt{gave_up, &g_mm_timeout};
-    Finder find;
+    Finder<RUNS> find;
     find.start(runs);
     Tile t;
     const int chunks = int((w.K + 255) >> 8), c0 = int(int64_t(chunks) * part / parts), c1 = int(int64_t(chunks) * (part + 1) / parts);
@@ -845,7 +846,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
                         sums[(8 * u + 2 * q + (i & 1)) * kFewRows + warp * 16 + g + 8 * (i >> 1)] = acc[0][u][i] + acc[1][u][i];
             }
         }
-        if (parts == 1 && o.zero_rest && runs.offsets && !wt.fail) zero_rows<T>(o, find.begin, find.end(runs), kFewWarps * 32);
+        if (RUNS && o.zero_rest && !wt.fail) zero_rows<T>(o, find.begin, find.end(runs), kFewWarps * 32);
     }
     if (parts > 1) {
         tc5::cluster_sync();
@@ -1191,11 +1192,11 @@ Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
     return p;
 }
 
-template <int BT, bool BF16, bool DX>
+template <int BT, bool BF16, bool DX, bool RUNS>
 int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, const Runs &r, const Weights &w, const Out &o, int64_t tiles, cudaStream_t st) {
     using C = Cfg<BT, DX>;
     CUtensorMap mr, mc;
-    auto kernel = q4_product_kernel<BT, BF16, DX>;
+    auto kernel = q4_product_kernel<BT, BF16, DX, RUNS>;
     // before the maps: in a thread without a context (autograd's, at its first call) this binds the device's, which the
     // map encoder needs
     if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), C::kSmem) != cudaSuccess) return uq::check_cuda("q4_product_kernel attribute");
@@ -1219,7 +1220,7 @@ template <bool BF16, int NT>
 int few(const void *x, int64_t ldx, int64_t T, const uint8_t *codes, const Weights &w, int64_t mats, const int32_t *offsets, void *y, int64_t ldy, bool zero,
         cudaStream_t st) {
     using C = FewCfg<NT>;
-    auto kernel = q4_few_kernel<BF16, NT>;
+    const auto kernel = offsets ? q4_few_kernel<BF16, NT, true> : q4_few_kernel<BF16, NT, false>;
     if (uq::set_smem_attr(reinterpret_cast<const void *>(kernel), C::kSmem) != cudaSuccess) return uq::check_cuda("q4_few_kernel attribute");
     int box = 1;   // rows of a copy
     while (box < std::min<int64_t>(T, 8 * NT)) box *= 2;
@@ -1265,9 +1266,13 @@ int product(const void *rows, int64_t lda, int64_t T, const uint8_t *codes, cons
         return uq::fail(UQ_ERR_WORKSPACE, "4-bit product: workspace of %zu bytes, %zu needed", ws_bytes, size_t(p.splits) * T * J * 4);
     const Runs r{offsets, T, mats, p.bt, int((J + 255) / 256), p.splits};
     const Out o{p.splits > 1 ? ws : out, ldo, J, T, zero};
-    int rc = p.width == 64    ? launch<64, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st)
-             : p.width == 128 ? launch<128, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st)
-                              : launch<256, BF16, DX>(rows, lda, codes, mats, r, w, o, p.tiles, st);
+    const auto go = offsets ? p.width == 64    ? launch<64, BF16, DX, true>
+                              : p.width == 128 ? launch<128, BF16, DX, true>
+                                               : launch<256, BF16, DX, true>
+                    : p.width == 64  ? launch<64, BF16, DX, false>
+                    : p.width == 128 ? launch<128, BF16, DX, false>
+                                     : launch<256, BF16, DX, false>;
+    const int rc = go(rows, lda, codes, mats, r, w, o, p.tiles, st);
     if (rc || p.splits == 1) return rc;
     uq::ProfScope _p("q4_join_parts", st);
     q4_join_parts_kernel<BF16><<<unsigned(std::min<int64_t>((T * J + 255) / 256, 1184)), 256, 0, st>>>(static_cast<const float *>(ws), p.splits, T, J, w.scale, out, ldo);
