@@ -380,6 +380,40 @@ def test_grouped_takes_falling_and_far_offsets_in_order_and_reports_them():
         q4().check_errors()
 
 
+def test_no_expert_and_many_experts():
+    none = q4().Q4(torch.empty(0, 40, 32, dtype=torch.uint8, device="cuda"), torch.empty(0, 40, 2, device="cuda").to(torch.float8_e4m3fn),
+                   torch.empty(0, device="cuda"))
+    x = acts(5, 64, torch.bfloat16, 1).requires_grad_()
+    s = none.group_scales().requires_grad_()
+    torch.full((5, 40), 3.0, device="cuda", dtype=torch.bfloat16)            # memory that the result may get, not zero
+    y = q4().grouped_linear(x, torch.zeros(1, dtype=torch.int32, device="cuda"), none, s)
+    dx, dc = torch.autograd.grad(y, (x, s), torch.ones_like(y))
+    assert torch.equal(y, torch.zeros_like(y)) and torch.equal(dx, torch.zeros_like(dx)) and dc.shape == (0, 40, 2)
+    # more experts than a warp looks at a time, single rows and gaps between them
+    E, N, K = 131, 24, 64
+    w, q, c, wd = make((E, N, K), 32, 7)
+    counts = [(i * 7) % 3 for i in range(E)]
+    off = experts(counts)
+    T = sum(counts)
+    x = acts(T, K, torch.bfloat16, 3).requires_grad_()
+    s = w.group_scales().requires_grad_()
+    dy = acts(T, N, torch.bfloat16, 4)
+    y = q4().grouped_linear(x, off, w, s)
+    dx, dc = torch.autograd.grad(y, (x, s), dy)
+    which = torch.repeat_interleave(torch.arange(E), torch.tensor(counts)).cuda()
+    xd, d, we = x.detach().double(), dy.double(), wd[which]
+    close(y, torch.einsum("tk,tnk->tn", xd, we), torch.einsum("tk,tnk->tn", xd.abs(), we.abs()), K)
+    close(dx, torch.einsum("tn,tnk->tk", d, we), torch.einsum("tn,tnk->tk", d.abs(), we.abs()), N)
+    outer = torch.zeros(E, N, K, dtype=torch.float64, device="cuda").index_add_(0, which, d[:, :, None] * xd[:, None])
+    size = torch.zeros(E, N, K, dtype=torch.float64, device="cuda").index_add_(0, which, d.abs()[:, :, None] * xd.abs()[:, None])
+    close(dc, (outer * q).view(E, N, 2, 32).sum(-1), (size * q.abs()).view(E, N, 2, 32).sum(-1), 2 + 32)
+    # the same rows in one run, many to the kernels for many rows
+    big = q4().Q4(w.codes[:3].contiguous(), w.scales[:3].contiguous(), w.scale[:3].contiguous())
+    x2 = acts(900, K, torch.bfloat16, 5)
+    y2 = q4().grouped_linear(x2, torch.tensor([0, 0, 900, 900], dtype=torch.int32, device="cuda"), big)
+    close(y2, x2.double() @ wd[1].T, x2.double().abs() @ wd[1].abs().T, K)
+
+
 def test_one_expert_is_linear():
     for T in (3, 70):
         w, *_ = make((1, 200, 320), 64, 2)

@@ -1298,6 +1298,13 @@ int dscale(const void *dy, const void *x, int64_t T, int64_t lddy, int64_t ldx, 
     return uq::check_cuda("q4_dscale_kernel launch");
 }
 
+// No matrix: every row is outside every run.
+int no_matrix(void *out, int64_t ld, int64_t T, int64_t J, bool zero, cudaStream_t st) {
+    if (!zero || T == 0 || J == 0) return UQ_OK;
+    if (!out || (T > 1 && ld < J)) return uq::fail(UQ_ERR_INVALID, "4-bit product: output (null pointer or row stride)");
+    return cudaMemset2DAsync(out, size_t(std::max(ld, J)) * 2, 0, size_t(J) * 2, size_t(T), st) == cudaSuccess ? UQ_OK : uq::check_cuda("4-bit product");
+}
+
 size_t product_workspace(int64_t T, int64_t mats, int64_t J, int64_t depth) {
     if (T <= 0 || mats != 1 || J <= 0 || depth <= 0 || T > kMost || J > kMost || depth > kMost) return 0;
     const Plan p = plan_for(T, mats, false, J, depth);
@@ -1326,7 +1333,8 @@ int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t
                  int64_t mats, int64_t N, int64_t K, int group, const int32_t *offsets, void *y, int64_t ldy, int zero_rest,
                  void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = check_args("uq_q4_linear", dtype, T, mats, N, K, group, offsets, codes, x, ldx, K, y, ldy, N, false)) return rc;
-    if (T == 0 || N == 0 || mats == 0) return UQ_OK;
+    if (mats == 0) return no_matrix(y, ldy, T, N, zero_rest, UQ_STREAM(stream));
+    if (T == 0 || N == 0) return UQ_OK;
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear: null pointer");
     const Weights w{scales, scale, N, K, uq::ilog2(group)};
     const cudaStream_t st = UQ_STREAM(stream);
@@ -1347,7 +1355,8 @@ int uq_q4_linear_dx(const void *dy, int dtype, int64_t T, int64_t lddy, const ui
                     int64_t mats, int64_t N, int64_t K, int group, const int32_t *offsets, void *dx, int64_t lddx, int zero_rest,
                     void *workspace, size_t workspace_bytes, void *stream) {
     if (int rc = check_args("uq_q4_linear_dx", dtype, T, mats, N, K, group, offsets, codes, dy, lddy, N, dx, lddx, K, false)) return rc;
-    if (T == 0 || N == 0 || mats == 0) return UQ_OK;
+    if (mats == 0) return no_matrix(dx, lddx, T, K, zero_rest, UQ_STREAM(stream));
+    if (T == 0 || N == 0) return UQ_OK;
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear_dx: null pointer");
     const Weights w{scales, scale, N, K, uq::ilog2(group)};
     const cudaStream_t st = UQ_STREAM(stream);

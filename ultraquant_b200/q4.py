@@ -42,7 +42,7 @@ class Q4:
     with no leading dimension or one (experts).  Contiguous CUDA tensors of one device; the byte order of the codes is
     include/uq_b200.h's."""
 
-    __slots__ = ("codes", "scales", "scale", "mats", "rows", "cols", "group", "device", "ptrs", "form")
+    __slots__ = ("codes", "scales", "scale", "mats", "rows", "cols", "group", "device", "form")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, scale: torch.Tensor):
         cs, ss = codes.shape, scales.shape
@@ -66,7 +66,6 @@ class Q4:
     def _set(self, codes, scales, scale, mats, rows, cols, group):
         self.codes, self.scales, self.scale = codes, scales, scale
         self.mats, self.rows, self.cols, self.group, self.device = mats, rows, cols, group, codes.device
-        self.ptrs = (codes.data_ptr(), scales.data_ptr(), scale.data_ptr())
         self.form = (mats, rows, cols, group)
 
     @classmethod
@@ -75,6 +74,10 @@ class Q4:
         w = cls.__new__(cls)
         w._set(codes, scales, scale, mats, rows, cols, group)
         return w
+
+    @property
+    def ptrs(self):
+        return self.codes.data_ptr(), self.scales.data_ptr(), self.scale.data_ptr()
 
     @property
     def shape(self):
