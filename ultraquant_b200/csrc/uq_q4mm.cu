@@ -657,12 +657,14 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
 
 // ----------------------------------------------------------------------------
 // Few rows: bound by reading the codes once, and next to that by the
-// instructions that widen them (11 a word of 8; the integer ones have a half-rate
-// pipe, 14 cycles of the 23 that memory gives a warp's 256 codes).  A block takes
-// 128 weight rows, 16 for each of eight warps; a ninth copies chunks of 256 values
-// of k, codes and rows, into a ring (TMA), so that three blocks an SM keep 144 KB
-// on the way.  Where there are few tiles a cluster of 2, 4 or 8 blocks shares one,
-// each a part of k, and adds up through distributed shared memory.  The widened
+// instructions that widen them.  (57344 x 8192, 1 row: 57 us, 4.3 TB/s.  The copies
+// alone take 42 us; the arithmetic alone 52, of which the masks and shifts, on a pipe
+// of half rate, with the products of pairs by their scale are 40.)  A block takes
+// 128 weight rows, 32 for each of four warps (16 of eight for more than 8 rows); one
+// more copies chunks of 256 values of k, codes and rows, into a ring (TMA).  Four
+// blocks an SM with two stages: 57 us; three with three: 63.  Where there are few
+// tiles a cluster of 2, 4 or 8 blocks shares one, each a part of k, and adds up
+// through distributed shared memory.  The widened
 // codes are operand A of m16n8k16 products straight from registers: the
 // contraction order is free as long as both operands agree, so lane quarter q
 // takes 64 consecutive values of a row (two 16-byte pieces) where the instruction
@@ -679,13 +681,15 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-constexpr int kFewWarps = 8, kFewRows = 128, kFewThreads = (kFewWarps + 1) * 32;
+constexpr int kFewRows = 128, kFewParts = 8;   // weight rows of a tile; most parts of k
 
-// NT: blocks of 8 rows.  A quarter of a chunk's rows is one copy of up to 8 NT
+// NT: blocks of 8 rows; MT: blocks of 16 weight rows of a warp.  A quarter of a chunk's rows is one copy of up to 8 NT
 // lines of 64 values; each quarter begins two lines further round the 128-byte
 // swizzle, so that the four lanes of a row read different banks.
 template <int NT> struct FewCfg {
-    static constexpr int NS = NT == 1 ? 3 : 4, kBlocks = NT == 1 ? 3 : 2;     // stages, blocks an SM
+    // two weight blocks a warp share the loads of the rows and the steps of the loop; with more rows the registers do not reach
+    static constexpr int MT = NT == 1 ? 2 : 1, kWarps = 8 / MT, kThreads = (kWarps + 1) * 32;
+    static constexpr int NS = NT == 2 ? 4 : 2, kBlocks = NT == 1 ? 4 : 2;     // stages, blocks an SM
     static constexpr int kC = 16384, kQuarter = 8 * NT * 128 + 256, kX = 4 * kQuarter, kStage = kC + kX;
     static constexpr int kSums = kFewRows * 8 * NT * 4;                       // of one block, for its cluster
     static constexpr int kSmem = 1024 + NS * kStage + kSums + NS * 16 + 16;
@@ -693,11 +697,11 @@ template <int NT> struct FewCfg {
 };
 
 template <bool BF16, int NT, bool RUNS>
-__global__ void __launch_bounds__(kFewThreads, FewCfg<NT>::kBlocks)
+__global__ void __launch_bounds__(FewCfg<NT>::kThreads, FewCfg<NT>::kBlocks)
 q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constant__ CUtensorMap map_codes, Runs runs, Weights w, Out o, int box) {
     using T = typename Halves<BF16>::T;
     using C = FewCfg<NT>;
-    constexpr int NS = C::NS;
+    constexpr int NS = C::NS, MT = C::MT, kFewWarps = C::kWarps;
     extern __shared__ uint8_t smem_raw[];
     const unsigned smem_at = tc5::smem_addr(smem_raw), base = (smem_at + 1023u) & ~1023u, sums_at = base + NS * C::kStage, full = sums_at + C::kSums, empty = full + 8 * NS, misc = empty + 8 * NS;
     volatile int *gave_up = reinterpret_cast<volatile int *>(smem_raw + (misc - smem_at));
@@ -743,34 +747,33 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
         const int64_t groups = w.K >> w.gshift;
         Tile next;
         bool more = find.find(runs, blockIdx.x, next);
-        const int per_chunk = 256 >> w.gshift;
-        const bool pairs = w.gshift == 5, even = (w.K & 63) == 0;
-        const uint8_t *e0 = nullptr, *e1 = nullptr;      // this lane's two rows of scales; beyond N the last row's, not written
-        uint32_t elo[2], ehi[2];     // the two bytes of this lane's 64 values, as they come from memory: put together when used
+        const bool pairs = w.gshift == 5, both = pairs && (groups & 1) == 0;   // two scales a quarter; as one word
+        constexpr int R = 2 * MT;        // this lane's rows: 8 apart
+        const uint8_t *es = nullptr;     // the tile's scales from this part on
+        uint32_t ro[R];                  // the rows' from there; beyond N the last row's, not written
+        uint32_t elo[R], ehi[R];         // the bytes of this lane's 64 values, as they come from memory: put together when used
         auto scales_of = [&](const Tile &tt) {
-            const int64_t n = int64_t(tt.wt) * kFewRows + warp * 16 + g, at = (int64_t(c0) * 256 + q * 64) >> w.gshift;
-            e0 = w.scales + (tt.mat * w.N + min(n, w.N - 1)) * groups + at;
-            e1 = w.scales + (tt.mat * w.N + min(n + 8, w.N - 1)) * groups + at;
+            const int64_t n0 = int64_t(tt.wt) * kFewRows;
+            es = w.scales + (tt.mat * w.N + n0) * groups;
+#pragma unroll
+            for (int i = 0; i < R; ++i) ro[i] = uint32_t(min(int64_t(warp * 16 * MT + g + 8 * i), w.N - 1 - n0)) * uint32_t(groups) + (q * 64 >> w.gshift);
         };
-        // the two rows' bytes for chunk c, then on to the next chunk
-        const uint32_t both = pairs ? 1u : 0x101u;   // one byte for both halves
+        // the rows' bytes for chunk c; of a quarter that begins beyond K the row's last, for values that are zero
         auto scales_at = [&](int c) {
-            elo[0] = elo[1] = ehi[0] = ehi[1] = 0;
-            if (c * 256 + q * 64 < w.K) {
-                if (pairs && even) {
-                    elo[0] = __ldg(reinterpret_cast<const unsigned short *>(e0));
-                    elo[1] = __ldg(reinterpret_cast<const unsigned short *>(e1));
-                } else {
-                    elo[0] = __ldg(e0);
-                    elo[1] = __ldg(e1);
-                    if (pairs && c * 256 + q * 64 + 32 < w.K) {
-                        ehi[0] = __ldg(e0 + 1);
-                        ehi[1] = __ldg(e1 + 1);
-                    }
-                }
+            const int first = c * 256 >> w.gshift;
+            const uint8_t *const p = es + first;
+            uint32_t back = 0, step = 1;
+            if (int64_t(c) * 256 + 256 > w.K) {
+                const int at = q * 64 >> w.gshift, last = int(groups) - 1 - first;
+                back = max(at - (both ? last - 1 : last), 0);
+                step = at < last;
             }
-            e0 += per_chunk;
-            e1 += per_chunk;
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                if (both) elo[i] = __ldg(reinterpret_cast<const unsigned short *>(p + (ro[i] - back)));
+                else elo[i] = __ldg(p + (ro[i] - back));
+                if (pairs && !both) ehi[i] = __ldg(p + (ro[i] - back + step));
+            }
         };
         if (more) {
             scales_of(next);
@@ -779,12 +782,14 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
         for (int64_t tile = blockIdx.x; more && !wt.fail; tile += gridDim.x) {
             t = next;
             more = find.find(runs, tile + gridDim.x, next);
-            float acc[2][NT][4] = {};   // two sums each, so that a product need not wait for the one before
+            float acc[MT][2][NT][4] = {};   // two sums each, so that a product need not wait for the one before
             unsigned tok[NT];           // this lane's row of x (of one that is not there: the last one's)
 #pragma unroll
             for (int u = 0; u < NT; ++u) tok[u] = min(g + 8 * u, t.rows - 1);
             for (int c = c0; c < c1; ++c) {
-                const uint32_t eh[2] = {e4m3_pair(elo[0] * both + (ehi[0] << 8)), e4m3_pair(elo[1] * both + (ehi[1] << 8))};
+                uint32_t eh[R];
+#pragma unroll
+                for (int i = 0; i < R; ++i) eh[i] = e4m3_pair(both ? elo[i] : pairs ? elo[i] | ehi[i] << 8 : elo[i] * 0x101u);
                 if (c + 1 < c1) {
                     scales_at(c + 1);
                 } else if (more) {   // the next tile's
@@ -793,27 +798,38 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
                 }
                 if (!wt.wait(full + 8 * slot, phase)) break;
                 const uint8_t *const stage = smem_raw + (base + slot * C::kStage - smem_at);
-                // rows g and g + 8 of the warp's 16 (the same swizzle): pieces 2 q, 2 q + 1
-                const uint8_t *const code = stage + (warp * 16 + g) * 128;
+                // rows g, g + 8, ... of the warp's (the same swizzle): pieces 2 q, 2 q + 1
+                const uint8_t *const code = stage + (warp * 16 * MT + g) * 128;
                 const uint8_t *xs[NT];
 #pragma unroll
                 for (int u = 0; u < NT; ++u) xs[u] = stage + C::kC + q * C::kQuarter + tok[u] * 128;
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
                     const int at = ((2 * q + p) ^ g) << 4;
-                    const uint4 w0 = *reinterpret_cast<const uint4 *>(code + at), w1 = *reinterpret_cast<const uint4 *>(code + 1024 + at);
-                    const typename Halves<BF16>::Scale s0 = Halves<BF16>::scale(eh[0], p), s1 = Halves<BF16>::scale(eh[1], p);
+                    uint4 cw[R];
+                    typename Halves<BF16>::Scale sc[R];
+#pragma unroll
+                    for (int i = 0; i < R; ++i) {
+                        cw[i] = *reinterpret_cast<const uint4 *>(code + i * 1024 + at);
+                        sc[i] = Halves<BF16>::scale(eh[i], p);
+                    }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        uint32_t lo[4], hi[4];
-                        Halves<BF16>::widen8(j == 0 ? w0.x : j == 1 ? w0.y : j == 2 ? w0.z : w0.w, s0, lo);
-                        Halves<BF16>::widen8(j == 0 ? w1.x : j == 1 ? w1.y : j == 2 ? w1.z : w1.w, s1, hi);
-                        const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+                        uint4 b[NT];
 #pragma unroll
-                        for (int u = 0; u < NT; ++u) {
-                            const uint4 b = *reinterpret_cast<const uint4 *>(xs[u] + (((4 * p + j) ^ ((tok[u] + 2 * q) & 7)) << 4));
-                            mma16816(acc[0][u], a0, b.x, b.y, BF16);
-                            mma16816(acc[1][u], a1, b.z, b.w, BF16);
+                        for (int u = 0; u < NT; ++u) b[u] = *reinterpret_cast<const uint4 *>(xs[u] + (((4 * p + j) ^ ((tok[u] + 2 * q) & 7)) << 4));
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            uint32_t lo[4], hi[4];
+                            const uint4 &w0 = cw[2 * m], &w1 = cw[2 * m + 1];
+                            Halves<BF16>::widen8(j == 0 ? w0.x : j == 1 ? w0.y : j == 2 ? w0.z : w0.w, sc[2 * m], lo);
+                            Halves<BF16>::widen8(j == 0 ? w1.x : j == 1 ? w1.y : j == 2 ? w1.z : w1.w, sc[2 * m + 1], hi);
+                            const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]}, a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+#pragma unroll
+                            for (int u = 0; u < NT; ++u) {
+                                mma16816(acc[m][0][u], a0, b[u].x, b[u].y, BF16);
+                                mma16816(acc[m][1][u], a1, b[u].z, b[u].w, BF16);
+                            }
                         }
                     }
                 }
@@ -825,26 +841,21 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
                 if (++slot == NS) { slot = 0; phase ^= 1; }
             }
             if (wt.fail) break;
-            // element i of a lane: row of x 8 u + 2 q + (i & 1), weight row g + 8 (i >> 1)
-            if (parts == 1) {
-                const float scale = __ldg(w.scale + t.mat);
+            // element i of a lane: row of x 8 u + 2 q + (i & 1), weight row 16 m + g + 8 (i >> 1)
+            const float scale = __ldg(w.scale + t.mat);
+            float *const sums = reinterpret_cast<float *>(smem_raw + (sums_at - smem_at));   // [row of x][weight row]; one tile a block
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int u = 0; u < NT; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int r = 8 * u + 2 * q + (i & 1);
-                        const int64_t n = int64_t(t.wt) * kFewRows + warp * 16 + g + 8 * (i >> 1);
-                        if (r < t.rows && n < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + n] = from_float<T>(scale * (Halves<BF16>::kBack * (acc[0][u][i] + acc[1][u][i])));
+                        const int r = 8 * u + 2 * q + (i & 1), c = (warp * MT + m) * 16 + g + 8 * (i >> 1);
+                        const float v = acc[m][0][u][i] + acc[m][1][u][i];
+                        const int64_t n = int64_t(t.wt) * kFewRows + c;
+                        if (parts > 1) sums[r * kFewRows + c] = v;
+                        else if (r < t.rows && n < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + n] = from_float<T>(scale * (Halves<BF16>::kBack * v));
                     }
-            } else {
-                // sums [row of x][weight row]; one tile a block
-                float *const sums = reinterpret_cast<float *>(smem_raw + (sums_at - smem_at));
-#pragma unroll
-                for (int u = 0; u < NT; ++u)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sums[(8 * u + 2 * q + (i & 1)) * kFewRows + warp * 16 + g + 8 * (i >> 1)] = acc[0][u][i] + acc[1][u][i];
-            }
         }
         if (RUNS && o.zero_rest && !wt.fail) zero_rows<T>(o, find.begin, find.end(runs), kFewWarps * 32);
     }
@@ -854,17 +865,20 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
         find.start(runs);
         if (find.find(runs, blockIdx.x, t)) {
             const float scale = __ldg(w.scale);
-            const int share = kFewRows / parts;
-            for (int i = threadIdx.x; i < share * t.rows; i += kFewThreads) {
-                const int r = i / share, n = part * share + i % share;
-                float v = 0.0f;
-                for (int p = 0; p < parts; ++p) {
+            const int first = kFewRows * part / parts, share = kFewRows * (part + 1) / parts - first;
+            for (int i = threadIdx.x; i < share * t.rows; i += C::kThreads) {
+                const int r = i / share, n = first + i % share;
+                float v = 0.0f, f[kFewParts];   // on their way together
+#pragma unroll
+                for (int p = 0; p < kFewParts; ++p) {
+                    f[p] = 0.0f;
+                    if (p >= parts) continue;
                     unsigned from;
-                    float f;
                     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(from) : "r"(sums_at + (r * kFewRows + n) * 4), "r"(p));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(from) : "memory");
-                    v += f;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f[p]) : "r"(from) : "memory");
                 }
+#pragma unroll
+                for (int p = 0; p < kFewParts; ++p) v += f[p];
                 const int64_t col = int64_t(t.wt) * kFewRows + n;
                 if (col < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + col] = from_float<T>(scale * (Halves<BF16>::kBack * v));
             }
@@ -1171,23 +1185,38 @@ struct Plan {
     int64_t tiles;    // at most, of a pair of CTAs
 };
 
-// J result columns, `depth` contraction steps.
+// J result columns, `depth` contraction steps.  The width and the parts of k with
+// the least estimated cycles: a stage of 64 steps takes 2 cycles a row of the tile
+// in the tensor cores and about 430 to be widened, a tile some 4500 for its start
+// and end, and joining parts a launch (5700) and their way to memory and back.
+// Measured at 4096 x 4096: 512 rows 18 us as 64 tiles of 128 rows, 34 us as two
+// parts of 32 tiles of 256; 64 rows 17 us in four parts, 20 us in one.
 Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
-    Plan p;
-    const int64_t each = std::max<int64_t>(1, T / std::max<int64_t>(mats, 1));   // rows a matrix, if even
-    p.width = each <= 64 ? 64 : each <= 128 ? 128 : 256;
-    p.bt = p.width;
-    p.splits = 1;
-    const int64_t wt = (J + 255) / 256;
-    const int64_t rt = runs ? std::min(T, T / p.bt + mats) : (T + p.bt - 1) / p.bt;
-    p.tiles = rt * wt;
-    const int pairs = uq::num_sms() / 2;
-    if (!runs && p.tiles * 2 <= pairs) {
-        const int64_t chunks = (depth + 255) / 256;
-        p.splits = int(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(pairs / p.tiles, chunks / 2), 16)));
-        const int64_t each_part = (chunks + p.splits - 1) / p.splits;
-        p.splits = int((chunks + each_part - 1) / each_part);   // no part is empty
-        p.tiles *= p.splits;
+    Plan p{};
+    const int64_t wt = (J + 255) / 256, chunks = (depth + 255) / 256, pairs = uq::num_sms() / 2;
+    if (runs) {   // the runs' lengths are not known here: as if they were even
+        const int64_t each = std::max<int64_t>(1, T / std::max<int64_t>(mats, 1));
+        p.width = p.bt = each <= 64 ? 64 : each <= 128 ? 128 : 256;
+        p.splits = 1;
+        p.tiles = std::min(T, T / p.bt + mats) * wt;
+        return p;
+    }
+    double best = 0;
+    for (int width = 64; width <= 256; width *= 2) {
+        const int64_t tiles = (T + width - 1) / width * wt;
+        for (int64_t s = 1; s <= std::min<int64_t>(16, chunks); ++s) {
+            const int64_t part = (chunks + s - 1) / s;
+            if (s > 1 && ((chunks + part - 1) / part != s || tiles * s > pairs)) continue;   // an empty part; more than one round
+            const double rounds = double((tiles * s + pairs - 1) / pairs), rows = double(std::min<int64_t>(T, width));
+            const double cost = rounds * (double(part * 4) * std::max(2.0 * rows, 430.0) + 4500.0) +
+                                (s > 1 ? 5700.0 + double(s) * double(T) * double(J) * 8 / 2100.0 : 0.0);
+            if (p.width == 0 || cost < best) {
+                best = cost;
+                p.width = p.bt = width;
+                p.splits = int(s);
+                p.tiles = tiles * s;
+            }
+        }
     }
     return p;
 }
@@ -1212,9 +1241,14 @@ int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, co
     return uq::check_cuda("q4_product_kernel launch");
 }
 
-// Rows (for several matrices, rows each if even) up to which the kernel for few
-// rows is taken.
-constexpr int64_t kFewMost = 16;
+// Whether the kernel for few rows is taken.  Up to 16 rows (for several matrices:
+// 16 each if they were even): 4096 x 4096 at 16 rows 7.9 us, by pairs 15; 28672 x
+// 8192 43 against 63.  Up to 32 where a single matrix has so few tiles that the
+// pairs would have to split k: 4096 x 4096 at 32 rows 10.6 us against 15.1, but
+// 28672 x 8192 68 against 63.
+bool few_rows(int64_t T, int64_t mats, bool runs, int64_t N) {
+    return T <= 16 * mats || (!runs && T <= 32 && (N + 255) / 256 * 2 <= uq::num_sms() / 2);
+}
 
 template <bool BF16, int NT>
 int few(const void *x, int64_t ldx, int64_t T, const uint8_t *codes, const Weights &w, int64_t mats, const int32_t *offsets, void *y, int64_t ldy, bool zero,
@@ -1232,18 +1266,21 @@ int few(const void *x, int64_t ldx, int64_t T, const uint8_t *codes, const Weigh
         return uq::fail(UQ_ERR_CUDA, "tensor map of a 4-bit product");
     const int64_t wtiles = (w.N + kFewRows - 1) / kFewRows, tiles = (offsets ? std::min(T, T / (8 * NT) + mats) : 1) * wtiles;
     const int64_t slots = int64_t(uq::num_sms()) * C::kBlocks, chunks = (w.K + 255) / 256;
-    // parts of k: least (rounds of blocks) x (chunks of a block, and about three for its start and end)
+    // Parts of k: the least time of the busiest SM, in 0.35 us.  m blocks at a time take m + 1 a chunk between them, and 8 to
+    // start and end; adding up the parts takes 4 a block of 8 rows.  (1 row, parts 1, 2, 4, 8: 4096 x 4096 13.2, 9.5, 7.3,
+    // 7.0 us; 28672 x 8192 34.0, 33.3, 34.0, 37.8.  16 rows of 14336 x 4096 15.4, 17.4, 21.0, 27.4.)
+    const auto cost = [&](int64_t p) {
+        const int64_t blocks = (tiles * p + uq::num_sms() - 1) / uq::num_sms(), c = (chunks + p - 1) / p, rest = blocks % C::kBlocks;
+        return blocks / C::kBlocks * ((C::kBlocks + 1) * c + 8) + (rest ? (rest + 1) * c + 8 : 0) + (p > 1 ? 4 * NT : 0);
+    };
     int parts = 1;
-    int64_t best = (tiles + slots - 1) / slots * (chunks + 3);
-    for (int p = 2; p <= 8 && !offsets && p <= chunks; p *= 2) {
-        const int64_t cost = (tiles * p + slots - 1) / slots * ((chunks + p - 1) / p + 3);
-        if (cost < best) { best = cost; parts = p; }
-    }
+    for (int p = 2; p <= kFewParts && !offsets && p <= chunks; p *= 2)
+        if (cost(p) < cost(parts)) parts = p;
     const Runs r{offsets, T, mats, 8 * NT, int(wtiles), parts};
     const Out o{y, ldy, w.N, T, zero};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = unsigned(parts > 1 ? tiles * parts : std::min(tiles, slots));
-    cfg.blockDim = kFewThreads;
+    cfg.blockDim = C::kThreads;
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute at;
@@ -1327,7 +1364,9 @@ bool mm_take_flags(int *timeout, int *offset) {
 
 extern "C" {
 
-size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K) { return T <= kFewMost ? 0 : product_workspace(T, mats, N, K); }
+size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K) {
+    return T > 0 && mats == 1 && !few_rows(T, 1, false, N) ? product_workspace(T, mats, N, K) : 0;
+}
 
 int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t *codes, const uint8_t *scales, const float *scale,
                  int64_t mats, int64_t N, int64_t K, int group, const int32_t *offsets, void *y, int64_t ldy, int zero_rest,
@@ -1338,12 +1377,12 @@ int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear: null pointer");
     const Weights w{scales, scale, N, K, uq::ilog2(group)};
     const cudaStream_t st = UQ_STREAM(stream);
-    if (T <= kFewMost * mats) {
-        if (T <= 8 * mats)
-            return dtype == UQ_BF16 ? few<true, 1>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st)
-                                    : few<false, 1>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st);
-        return dtype == UQ_BF16 ? few<true, 2>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st)
-                                : few<false, 2>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st);
+    if (few_rows(T, mats, offsets != nullptr, N)) {
+        const auto go = dtype == UQ_BF16 ? T <= 8 * mats ? few<true, 1> : T <= 16 * mats ? few<true, 2> : few<true, 4>
+                        : T <= 8 * mats  ? few<false, 1>
+                        : T <= 16 * mats ? few<false, 2>
+                                         : few<false, 4>;
+        return go(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, st);
     }
     return dtype == UQ_BF16 ? product<true, false>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, workspace, workspace_bytes, st)
                             : product<false, false>(x, ldx, T, codes, w, mats, offsets, y, ldy, zero_rest, workspace, workspace_bytes, st);
