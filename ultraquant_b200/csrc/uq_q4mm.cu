@@ -1203,16 +1203,17 @@ Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
     }
     double best = 0;
     for (int width = 64; width <= 256; width *= 2) {
-        const int64_t tiles = (T + width - 1) / width * wt;
+        const int64_t n = (T + width - 1) / width, tiles = n * wt, bt = ((T + n - 1) / n + 31) / 32 * 32;
         for (int64_t s = 1; s <= std::min<int64_t>(16, chunks); ++s) {
             const int64_t part = (chunks + s - 1) / s;
             if (s > 1 && ((chunks + part - 1) / part != s || tiles * s > pairs)) continue;   // an empty part; more than one round
-            const double rounds = double((tiles * s + pairs - 1) / pairs), rows = double(std::min<int64_t>(T, width));
+            const double rounds = double((tiles * s + pairs - 1) / pairs), rows = double(bt);
             const double cost = rounds * (double(part * 4) * std::max(2.0 * rows, 430.0) + 4500.0) +
                                 (s > 1 ? 5700.0 + double(s) * double(T) * double(J) * 8 / 2100.0 : 0.0);
             if (p.width == 0 || cost < best) {
                 best = cost;
-                p.width = p.bt = width;
+                p.width = width;
+                p.bt = int(bt);
                 p.splits = int(s);
                 p.tiles = tiles * s;
             }
