@@ -13,7 +13,10 @@ Kernels: viterbi (segments of 256, L / R), rht and irht (fp64), e8,
 normalize, fwht (fp32), recon and recon_bwd (the QAT decoder, fp32), q8enc and
 q8dec (Q8_0 blocks, fp32 side), rht28 (opt-in unpadded 28 x P transform, --n0),
 qe8 (finite-codebook E8, fp64, --bpw; all of its kernels), e8search (the opt-in
-per-row search over 16 E8 steps at base step 0.48, fp64; the search kernel).
+per-row search over 16 E8 steps at base step 0.48, fp64; the search kernel),
+q4few, q4linear, q4dx and q4dscale (products with 4-bit weights of --n0 x --n,
+groups of 32, and --rows bfloat16 activations: the kernel for few rows, the one
+by pairs of CTAs, and the two gradients).
 """
 from __future__ import annotations
 
@@ -29,7 +32,7 @@ from . import _lib
 SCOPE = {"viterbi": "viterbi_fwd", "rht": "rht", "irht": "rht", "e8": "e8_quant",
          "normalize": "normalize", "fwht": "fwht", "recon": "qat_recon", "recon_bwd": "qat_recon_bwd",
          "q8enc": "q8_encode", "q8dec": "q8_decode", "rht28": "rht", "qe8": "qe8_search",
-         "e8search": "e8_search"}
+         "e8search": "e8_search", "q4few": "q4_few", "q4linear": "q4_linear", "q4dx": "q4_dx", "q4dscale": "q4_dscale"}
 
 
 def _peaks():
@@ -170,6 +173,22 @@ def build_case(args, lib, st):
             def run():
                 _lib.check(lib.uq_q8_decode(q.data_ptr(), rows, n, W.data_ptr(), n, st), "q8dec")
         return run, rows * n * 4 + rows * n // 32 * 34, "bytes"
+    if k in ("q4few", "q4linear", "q4dx", "q4dscale"):
+        from . import q4
+        w = q4.enc_q4(torch.randn(n0, n, device=dev, generator=g) * 0.02, 32)
+        x = torch.randn(rows, n, device=dev, generator=g).bfloat16().requires_grad_(k == "q4dx")
+        if k in ("q4few", "q4linear"):
+            def run():
+                q4.linear(x, w)
+        else:
+            sc = w.group_scales().requires_grad_(k == "q4dscale")
+            y, dy = q4.linear(x, w, sc), torch.randn(rows, n0, device=dev, generator=g).bfloat16()
+
+            def run():
+                torch.autograd.grad(y, x if k == "q4dx" else sc, dy, retain_graph=True)
+        if k == "q4few":
+            return run, n0 * n * 17 // 32 + 2 * rows * (n + n0), "bytes"
+        return run, 2 * rows * n * n0, "flops"
     raise SystemExit(f"unknown kernel {k}")
 
 
@@ -200,6 +219,8 @@ def measure(kernel: str, rows: int = 4096, n: int = 4096, n0: int = 0, L: int = 
     _lib.check(lib.uq_profile_read(SCOPE[kernel].encode(), _lib.ctypes.byref(tot), _lib.ctypes.byref(cnt)),
                "profile")
     rec = {"kernel": kernel, "rows": rows, "n": n0 or n, "runs": iters, "launches": cnt.value}
+    if kernel.startswith("q4"):
+        rec["k"] = n
     if kernel == "qe8":
         # every kernel of the call, and the call as a whole (events on the stream)
         for scope in ("e8_quant", "qe8_cb_norm", "qe8_classify", "qe8_search", "qe8_exact"):
@@ -225,6 +246,9 @@ def measure(kernel: str, rows: int = 4096, n: int = 4096, n0: int = 0, L: int = 
         peak, kind = (hbm_peak, "given") if hbm_peak else _peaks()
         gbs = units / (ms * 1e-3) / 1e9
         rec.update(algorithmic_bytes=units, achieved_gbs=gbs, peak_gbs=peak, frac=gbs / peak, peak_kind=kind)
+    elif unit == "flops":
+        tf = units / (ms * 1e-3) / 1e12
+        rec.update(flops=units, achieved_tflops=tf)
     else:
         props = torch.cuda.get_device_properties(dev)
         nominal = props.multi_processor_count * 128 * 1965e6
@@ -238,7 +262,7 @@ def main(argv=None):
     ap.add_argument("kernel", choices=sorted(SCOPE))
     ap.add_argument("--rows", type=int, default=4096, help="rows (sequences for viterbi)")
     ap.add_argument("--n", type=int, default=4096, help="row width (power of two)")
-    ap.add_argument("--n0", type=int, default=0, help="unpadded width of rht / irht (default n)")
+    ap.add_argument("--n0", type=int, default=0, help="unpadded width of rht / irht, weight rows of q4 (default n)")
     ap.add_argument("--L", type=int, default=16)
     ap.add_argument("--R", type=int, default=2)
     ap.add_argument("--bpw", type=float, default=2.0, help="rate of the qe8 case")
