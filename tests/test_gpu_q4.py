@@ -180,6 +180,64 @@ def test_linear_from_a_cold_cache(T, N, K, dt):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,N,K,group", [(1, 140, 608, 32), (2, 200, 320, 64), (4, 33, 192, 32), (6, 150, 384, 128), (8, 129, 32, 32),
+                                         (8, 260, 8224, 32), (10, 40, 1120, 32), (15, 131, 448, 64), (24, 100, 4160, 32), (32, 600, 8480, 32)])
+def test_linear_few_rows_at_the_end_of_a_chunk(T, N, K, group, dt):
+    """Few rows, the last chunk of 256 values cut off at each place a group can end; a NaN scale there stays in its row."""
+    w, q, c, wd = make((N, K), group, T * K)
+    x = acts(T, K, DT[dt], K)
+    xd = x.double()
+    close(q4().linear(x, w), xd @ wd.T, xd.abs() @ wd.abs().T, K)
+    bad = w.scales.view(torch.uint8).clone()
+    bad[N // 2, -1] = 0x7F
+    y = q4().linear(x, q4().Q4(w.codes, bad.view(torch.float8_e4m3fn), w.scale))
+    rest = [n for n in range(N) if n != N // 2]
+    assert torch.isnan(y[:, N // 2]).all() and torch.equal(y[:, rest], q4().linear(x, w)[:, rest])
+
+
+def test_offsets_beyond_32_bits():
+    """Codes, activations and results of more than 2^31 elements: the last rows are right."""
+    m = q4()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    E, N, K, group, last = 3, 24576, 65536, 256, 48              # 2.4 GB of codes
+    codes = torch.randint(0, 256, (E, N, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    e = (torch.randn(E, N, K // group, generator=g, device="cuda") * 3).to(torch.float8_e4m3fn)
+    w = m.Q4(codes, e, torch.full((E,), 0.015625, device="cuda"))
+    tail = m.Q4(codes[2, -last:].clone(), e[2, -last:].clone(), w.scale[2:].reshape(()))
+    wt, q = m.deq_q4(tail).double(), torch.from_numpy(O4.unpack(tail.codes.cpu().numpy())).double().cuda()
+    for T in (4, 100):
+        off = torch.tensor([0, 1, 1, T], dtype=torch.int32, device="cuda")
+        x = acts(T, K, torch.bfloat16, T).requires_grad_()
+        s = w.group_scales().requires_grad_()
+        y = m.grouped_linear(x, off, w, s)
+        xd = x.detach()[1:].double()
+        close(y.detach()[1:, -last:], xd @ wt.T, xd.abs() @ wt.abs().T, K)
+        dy = torch.zeros(T, N, device="cuda", dtype=torch.bfloat16)
+        dy[:, -last:] = acts(T, last, torch.bfloat16, 7)
+        dx, dc = torch.autograd.grad(y, (x, s), dy)
+        d = dy[1:, -last:].double()
+        close(dx[1:], d @ wt, d.abs() @ wt.abs(), N)
+        close(dc[2, -last:], ((d.T @ xd) * q).view(last, -1, group).sum(-1), ((d.abs().T @ xd.abs()) * q.abs()).view(last, -1, group).sum(-1), T + group)
+        del x, s, y, dy, dx, dc
+    # the last rows of a table, and a result of more than 2^31 elements
+    table = m.Q4(codes.view(E * N, K // 2), e.view(E * N, K // group), w.scale[0].reshape(()))
+    tok = torch.full((33000,), E * N - last, dtype=torch.int64, device="cuda")
+    tok[-last:] = torch.arange(E * N - last, E * N, device="cuda")
+    assert torch.equal(m.embedding(tok, table)[-last:], m.deq_q4(tail, torch.bfloat16))
+    del codes, e, w, table
+    # many rows of x
+    T, N, K = 70001, 64, 32768
+    w, q, c, wd = make((N, K), 256, 9)
+    x = torch.randn(T, K, generator=g, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    y = m.linear(x, w)
+    dy = acts(T, N, torch.bfloat16, 3)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    xd, d = x.detach()[-200:].double(), dy[-200:].double()
+    close(y[-200:], xd @ wd.T, xd.abs() @ wd.abs().T, K)
+    close(dx[-200:], d @ wd, d.abs() @ wd.abs(), N)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
 @pytest.mark.parametrize("T,N,K,group", SIZES)
 def test_linear_gradients(T, N, K, group, dt):
     w, q, c, wd = make((N, K), group, T * N + K)

@@ -105,6 +105,16 @@ def test_c_abi_refuses(tmp_path):
     assert eb() == _lib.UQ_ERR_WORKSPACE and "workspace" in err()
 
 
+def test_c_abi_refuses_scales_off_their_boundary():
+    from ultraquant_b200 import _lib
+    lib = _lib.load()
+    p = 1 << 20      # never followed
+    for f in (lib.uq_q4_linear, lib.uq_q4_linear_dx):
+        for off in (1, 2, 8):
+            rc = f(p, 2, 4, 64, p, p + off, p, 1, 8, 64, 32, None, p, 64, 1, None, 0, None)
+            assert rc == _lib.UQ_ERR_INVALID and "scales" in lib.uq_last_error().decode()
+
+
 def test_workspace_sizes_grow_with_the_call():
     from ultraquant_b200 import _lib
     lib = _lib.load()

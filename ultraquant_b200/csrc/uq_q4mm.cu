@@ -1376,6 +1376,7 @@ int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t
     if (mats == 0) return no_matrix(y, ldy, T, N, zero_rest, UQ_STREAM(stream));
     if (T == 0 || N == 0) return UQ_OK;
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear: null pointer");
+    if (!al16(scales)) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear: scales have to be 16-byte aligned");
     const Weights w{scales, scale, N, K, uq::ilog2(group)};
     const cudaStream_t st = UQ_STREAM(stream);
     if (few_rows(T, mats, offsets != nullptr, N)) {
@@ -1398,6 +1399,7 @@ int uq_q4_linear_dx(const void *dy, int dtype, int64_t T, int64_t lddy, const ui
     if (mats == 0) return no_matrix(dx, lddx, T, K, zero_rest, UQ_STREAM(stream));
     if (T == 0 || N == 0) return UQ_OK;
     if (!scales || !scale) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear_dx: null pointer");
+    if (!al16(scales)) return uq::fail(UQ_ERR_INVALID, "uq_q4_linear_dx: scales have to be 16-byte aligned");
     const Weights w{scales, scale, N, K, uq::ilog2(group)};
     const cudaStream_t st = UQ_STREAM(stream);
     return dtype == UQ_BF16 ? product<true, true>(dy, lddy, T, codes, w, mats, offsets, dx, lddx, zero_rest, workspace, workspace_bytes, st)
