@@ -65,8 +65,8 @@ template <typename T> __device__ __forceinline__ void load_word(const T *W, cons
 }
 
 // top[matrix][block] = max |x| bits over the groups without a non-finite value.
-// Bound by memory; a group is looked at as a whole only where a warp has met such
-// a value.
+// Bound by memory (4096 x 14336 float32: 49 us, 4.8 TB/s); a group is looked at as a
+// whole only where a warp has met such a value.
 template <typename T> __global__ void __launch_bounds__(256) q4_top_kernel(const T *W, EncArgs a, int64_t mat_stride, uint32_t *top) {
     __shared__ uint32_t warp_top[8];
     W += blockIdx.y * mat_stride;
@@ -106,7 +106,8 @@ template <typename T> __global__ void __launch_bounds__(256) q4_top_kernel(const
 }
 
 // `lanes`: threads of a group, eight values each (a constant: the reductions unroll).
-// The second reading goes backwards: what the first read last is still in L2.
+// The second reading goes backwards: what the first read last is still in L2
+// (4096 x 14336 float32 in 60 us).
 template <typename T, int lanes>
 __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, int64_t mat_stride, const uint32_t *top, float *scale, uint32_t *codes, uint8_t *scales) {
     __shared__ uint32_t warp_top[8];
@@ -203,7 +204,8 @@ __global__ void __launch_bounds__(256) q4_encode_kernel(const T *W, EncArgs a, i
 }
 
 // A thread writes 16 bytes at a time, so that a warp's store is one run of lines:
-// eight values of 16 bits, or (float32) the four of half a word.
+// eight values of 16 bits, or (float32) the four of half a word.  Bound by the writes:
+// 4096 x 14336 to float32 in 45 us, 5.9 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) q4_decode_kernel(const uint32_t *codes, const uint8_t *scales, const float *scale, int64_t words, int lshift, T *out) {
     constexpr int P = 16 / int(sizeof(T)), H = 8 / P;   // values a store, stores a word
@@ -276,7 +278,7 @@ template <typename I> __device__ __forceinline__ int64_t token_at(const I *token
 }
 
 // A block takes a token's row at a time, two words a thread on the way, the next
-// token already read: 16384 rows of 4096 in 34 us, 4.9 TB/s, bound by the writes.
+// token already read: 16384 rows of 4096 in 32 us, 5.2 TB/s, bound by the writes.
 // (Four rows on the way a block took more registers, fewer blocks and 49 us.)
 template <typename I, typename T>
 __global__ void __launch_bounds__(256) q4_embed_kernel(const I *tokens, int64_t n, const uint32_t *codes, const uint8_t *scales,
@@ -445,7 +447,9 @@ __global__ void __launch_bounds__(kTile) q4_scatter_kernel(Keys k, const uint32_
 // A block adds the rows of kSeg consecutive sorted entries, 2048 columns.  A
 // token whose entries all lie in the piece is written out; of one that goes
 // on from the piece before (head) or into the next (tail) the piece's part
-// goes to part[piece][head / tail].
+// goes to part[piece][head / tail].  Bound by the rows that it gathers: 16384 of
+// 4096 values, of 131072 tokens, 49 us, 3.4 TB/s; the sort before it 18 us, the join
+// 7.  (Pieces of 16 with four rows on the way 44 us here, but more to join; of 64, 50.)
 constexpr int kSeg = 32;
 
 // Eight values of a row as loaded, and as floats.

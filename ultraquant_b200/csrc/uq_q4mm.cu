@@ -371,6 +371,9 @@ template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int
 // rows are there (second); warp 19 brings each chunk's scales, an odd few bytes
 // from every row, which loaded by the widening warps a chunk ahead still cost 7 %
 // forward and 30 % of DX (4096 x 4096 x 14336: 460 us, 316 without any scales).
+// Bound by the tensor cores, except that a tile of less than 215 rows is widened no
+// sooner than one of 215.  Forward 2047 x 14336 x 4096 168 us, 1.43 PFLOP/s, in 7
+// rounds of tiles for 6.05; DX 4096 x 4096 x 14336 355 us, 1.36 PFLOP/s, 13 for 12.1.
 // ----------------------------------------------------------------------------
 constexpr int kWiden = 16, kThreads = (kWiden + 4) * 32;
 
@@ -664,9 +667,8 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
 // more copies chunks of 256 values of k, codes and rows, into a ring (TMA).  Four
 // blocks an SM with two stages: 57 us; three with three: 63.  Where there are few
 // tiles a cluster of 2, 4 or 8 blocks shares one, each a part of k, and adds up
-// through distributed shared memory.  The widened
-// codes are operand A of m16n8k16 products straight from registers: the
-// contraction order is free as long as both operands agree, so lane quarter q
+// through distributed shared memory.  The widened codes are operand A of m16n8k16
+// products straight from registers: the contraction order is free as long as both operands agree, so lane quarter q
 // takes 64 consecutive values of a row (two 16-byte pieces) where the instruction
 // says "columns 2 q, 2 q + 1, 2 q + 8, 2 q + 9".  Widening costs the same for 1 row
 // as for 8.  (With A in tensor memory a product of 16 steps takes 118 cycles
@@ -683,9 +685,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 
 constexpr int kFewRows = 128, kFewParts = 8;   // weight rows of a tile; most parts of k
 
-// NT: blocks of 8 rows; MT: blocks of 16 weight rows of a warp.  A quarter of a chunk's rows is one copy of up to 8 NT
-// lines of 64 values; each quarter begins two lines further round the 128-byte
-// swizzle, so that the four lanes of a row read different banks.
+// NT: blocks of 8 rows; MT: blocks of 16 weight rows of a warp.  A quarter of a
+// chunk's rows is one copy of up to 8 NT lines of 64 values; each quarter begins two
+// lines further round the 128-byte swizzle, so that the four lanes of a row read
+// different banks.
 template <int NT> struct FewCfg {
     // two weight blocks a warp share the loads of the rows and the steps of the loop; with more rows the registers do not reach
     static constexpr int MT = NT == 1 ? 2 : 1, kWarps = 8 / MT, kThreads = (kWarps + 1) * 32;
@@ -909,7 +912,8 @@ __global__ void __launch_bounds__(256) q4_join_parts_kernel(const float *part, i
 // q and added in float32 registers, so that no long sum runs in the tensor core.
 // Warps 0 .. 7 reduce, warp 8 copies, warp 9 issues (first CTA), warp 10 clears the
 // rows behind the last one of a run (they are another matrix's, and may be NaN)
-// and tells the first CTA that the stage is there.
+// and tells the first CTA that the stage is there.  Bound by the tensor cores: 4096 x
+// 4096 x 14336 in 304 us, 1.58 PFLOP/s.
 // ----------------------------------------------------------------------------
 constexpr int kPromote = 8, kBand = 8, kDsThreads = 352;
 
@@ -1189,7 +1193,7 @@ struct Plan {
 // the least estimated cycles: a stage of 64 steps takes 2 cycles a row of the tile
 // in the tensor cores and about 430 to be widened, a tile some 4500 for its start
 // and end, and joining parts a launch (5700) and their way to memory and back.
-// Measured at 4096 x 4096: 512 rows 18 us as 64 tiles of 128 rows, 34 us as two
+// Measured at 4096 x 4096: 512 rows 25 us as 64 tiles of 128 rows, 34 us as two
 // parts of 32 tiles of 256; 64 rows 17 us in four parts, 20 us in one.
 Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
     Plan p{};
@@ -1244,9 +1248,9 @@ int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, co
 
 // Whether the kernel for few rows is taken.  Up to 16 rows (for several matrices:
 // 16 each if they were even): 4096 x 4096 at 16 rows 7.9 us, by pairs 15; 28672 x
-// 8192 43 against 63.  Up to 32 where a single matrix has so few tiles that the
-// pairs would have to split k: 4096 x 4096 at 32 rows 10.6 us against 15.1, but
-// 28672 x 8192 68 against 63.
+// 8192 44 against 59.  Up to 32 where a single matrix has so few tiles that the
+// pairs would have to split k: 4096 x 4096 at 32 rows 10.4 us against 15.1, but
+// 28672 x 8192 68 against 59.
 bool few_rows(int64_t T, int64_t mats, bool runs, int64_t N) {
     return T <= 16 * mats || (!runs && T <= 32 && (N + 255) / 256 * 2 <= uq::num_sms() / 2);
 }
