@@ -195,6 +195,22 @@ def test_linear_few_rows_at_the_end_of_a_chunk(T, N, K, group, dt):
     assert torch.isnan(y[:, N // 2]).all() and torch.equal(y[:, rest], q4().linear(x, w)[:, rest])
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,N,K,group", [(2100, 2500, 4096, 32), (2090, 4100, 2560, 64), (700, 1030, 9472, 128)])
+def test_linear_whose_last_tiles_are_split(T, N, K, group, dt):
+    """More tiles than run at a time, the rest of them in parts along the contraction (of y or of dx)."""
+    w, q, c, wd = make((N, K), group, T)
+    x = acts(T, K, DT[dt], N).requires_grad_()
+    dy = acts(T, N, DT[dt], K)
+    y = q4().linear(x, w)
+    xd, d = x.detach().double(), dy.double()
+    close(y.detach(), xd @ wd.T, xd.abs() @ wd.abs().T, K)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    close(dx, d @ wd, d.abs() @ wd.abs(), N)
+    y2 = q4().linear(x, w)
+    assert torch.equal(y, y2) and torch.equal(dx, torch.autograd.grad(y2, x, dy)[0])
+
+
 def test_offsets_beyond_32_bits():
     """Codes, activations and results of more than 2^31 elements: the last rows are right."""
     m = q4()

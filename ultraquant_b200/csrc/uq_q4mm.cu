@@ -19,13 +19,15 @@ __device__ int g_mm_bad_offset, g_mm_timeout;
 
 // ----------------------------------------------------------------------------
 // Tiles: `wtiles` ranges of weight columns of the result by up to `bt` rows of
-// one matrix's run, by one of `splits` parts of the contraction.
+// one matrix's run.  Those from number `whole` on are `splits` parts of the
+// contraction each (one matrix for all rows only).
 // ----------------------------------------------------------------------------
 struct Runs {
     const int32_t *offsets;   // null: one matrix, all rows
     int64_t T, mats;
     int bt;                   // rows of a tile
     int wtiles, splits;
+    int64_t whole;
 };
 
 struct Tile {
@@ -75,8 +77,13 @@ template <bool RUNS> struct Finder {
     }
     // Tile number `t`; false beyond the last.
     __device__ __forceinline__ bool find(const Runs &r, int64_t t, Tile &tile) {
-        const int64_t u = runs_split(r, t, tile.split);
-        const int64_t rt = u / r.wtiles;
+        int64_t u = t;
+        tile.split = -1;          // the whole contraction, else the part's number
+        if (!RUNS && t >= r.whole) {
+            tile.split = int(t - r.whole);     // below 2^27 parts
+            u = r.whole + int(unsigned(tile.split) / unsigned(r.splits));
+        }
+        const int64_t rt = u < r.wtiles ? 0 : u / r.wtiles;   // few rows: no division on the way to the first copy
         tile.wt = int(u - rt * r.wtiles);
         if constexpr (!RUNS) {
             tile.mat = 0;
@@ -103,14 +110,6 @@ template <bool RUNS> struct Finder {
             tile.rows = min((at < 31 ? next : top) - tile.row0, r.bt);
         }
         return true;
-    }
-    static __device__ __forceinline__ int64_t runs_split(const Runs &r, int64_t t, int &split) {
-        if (r.splits == 1) {
-            split = 0;
-            return t;
-        }
-        split = int(t % r.splits);
-        return t / r.splits;
     }
     // The end of the last run, once find() has gone beyond the last tile.
     __device__ __forceinline__ int64_t end(const Runs &r) const { return RUNS ? top : r.T; }
@@ -264,9 +263,10 @@ __device__ __forceinline__ void load_scales(Scales &v, const Weights &w, bool pa
 }
 
 struct Out {
-    void *out;        // (rows, J) of 16 bits, or with splits the workspace: (splits, T, J) floats
+    void *out;        // (rows, J) of 16 bits
     int64_t ld, J, T;
     bool zero_rest;
+    float *parts;     // of split tiles: (tile, part, bt, 256)
 };
 
 // Register j of lane i: row j, column i of a 32 x 32 piece of the result.
@@ -323,18 +323,15 @@ __device__ __noinline__ void write_tile(unsigned at, unsigned drained, float sca
     for (int i = 0; i < PIECES; ++i)
         if (i * 128 < rows) store_piece(v[i], out, ld, J, wide, row0 + i * 128, rows - i * 128, col);
 }
-// The same for a part of a split contraction: floats, unscaled, J a row.
-__device__ __noinline__ void write_part(unsigned at, unsigned drained, float *out, int64_t J, int rows, int64_t col) {
+// The same for a part of a split contraction: floats, unscaled, 256 a row.
+__device__ __noinline__ void write_part(unsigned at, unsigned drained, float *out, int rows) {
     for (int i = 0; i < rows; i += 128) {
         uint32_t r[32];
         tc5::ld32(at + i, r);
         tc5::wait_ld();
-        float *p = out + int64_t(i) * J + col;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            if (i + j < rows && col < J) *p = __uint_as_float(r[j]);
-            p += J;
-        }
+        for (int j = 0; j < 32; ++j)
+            if (i + j < rows) out[(i + j) * 256] = __uint_as_float(r[j]);
     }
     tc5::fence_before();
     __syncwarp();
@@ -372,8 +369,8 @@ template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int
 // from every row, which loaded by the widening warps a chunk ahead still cost 7 %
 // forward and 30 % of DX (4096 x 4096 x 14336: 460 us, 316 without any scales).
 // Bound by the tensor cores, except that a tile of less than 215 rows is widened no
-// sooner than one of 215.  Forward 2047 x 14336 x 4096 168 us, 1.43 PFLOP/s, in 7
-// rounds of tiles for 6.05; DX 4096 x 4096 x 14336 355 us, 1.36 PFLOP/s, 13 for 12.1.
+// sooner than one of 215.  Forward 2047 x 14336 x 4096 156 us, 1.54 PFLOP/s;
+// DX 4096 x 4096 x 14336 347 us, 1.39 PFLOP/s.
 // ----------------------------------------------------------------------------
 constexpr int kWiden = 16, kThreads = (kWiden + 4) * 32;
 
@@ -433,12 +430,14 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     // stages of the whole contraction and of one part of it, whole chunks of four: what lies beyond the end is zero, and every
     // warp takes part in every chunk, so that no barrier goes by two phases unseen by one that will wait for it
     const int all = int((depth + 255) / 256) * 4, per = (all / 4 + runs.splits - 1) / runs.splits * 4;
+    const auto first_of = [&](const Tile &i) { return RUNS || i.split < 0 ? 0 : i.split % runs.splits * per; };   // a tile's stages
+    const auto count_of = [&](const Tile &i) { return RUNS || i.split < 0 ? all : min(per, all - first_of(i)); };
     unsigned it = 0, ct = 0, tiles = 0;                                           // stages, chunks, tiles so far
 
     if (warp == kWiden) {
         // rows: this CTA's half of the product's N
         for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step) {
-            const int s0 = t.split * per, n = min(per, all - s0);
+            const int s0 = first_of(t), n = count_of(t);
             const int half = ((t.rows + 31) & ~31) >> 1, boxes = (half + kBox - 1) / kBox, row = int(t.row0) + int(rank) * half;
             for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS;
@@ -456,7 +455,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
     } else if (warp == kWiden + 1) {
         // codes: 128 rows of 256 codes, or 256 rows of 128
         for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step) {
-            const int s0 = t.split * per, n = min(per, all - s0);
+            const int s0 = first_of(t), n = count_of(t);
             const int64_t row = t.mat * w.N;
             const int wtile = t.wt * 2 + int(rank);
             for (int s = 0; s < n; s += 4, ++ct) {
@@ -474,7 +473,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
             for (unsigned i = ct > NC ? ct - NC : 0; i < ct; ++i) tc5::Waiter::drain(full_c + 8 * (i % NC), (i / NC) & 1);
     } else if (warp == kWiden + 2 && rank == 1) {
         for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step) {
-            const int s0 = t.split * per, n = min(per, all - s0);
+            const int s0 = first_of(t), n = count_of(t);
             for (int s = 0; s < n; ++s, ++it) {
                 const int slot = it % NS;
                 if (!wt.wait(full + 8 * slot, (it / NS) & 1)) break;
@@ -487,7 +486,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
         unsigned slot = 0, par = 0;
         bool ready = false;
         for (int64_t tile = first; !wt.fail && find.find(runs, tile, t); tile += step, ++tiles) {
-            const int s0 = t.split * per, n = min(per, all - s0);
+            const int s0 = first_of(t), n = count_of(t);
             const uint32_t idesc = tc5::idesc_f16(BF16, (t.rows + 31) & ~31, DX, false);
             if (!wt.wait(drained, (tiles & 1) ^ 1)) break;
             for (int s = 0; s < n; ++s) {
@@ -528,7 +527,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
 #pragma unroll
         for (int i = 0; i < (DX ? 2 : 4); ++i) pick[i] = uint32_t((2 * i) >> shift) | uint32_t((2 * i + 1) >> shift) << 4;
         int64_t tile = first;
-        int c = 0, n = 0;       // chunk's first stage in the tile, its stages
+        int c = 0, n = 0, s0 = 0;       // chunk's first stage in the tile, its stages, the first
         bool on = true;
         Scales a, b;
         auto fetch = [&](Scales &v) -> bool {   // the next chunk's; false beyond the last
@@ -536,9 +535,10 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                 if (!on || !(on = find.find(runs, tile, t))) return false;
                 tile += step;
                 c = 0;
-                n = min(per, all - t.split * per);
+                s0 = first_of(t);
+                n = count_of(t);
             }
-            const int64_t k0 = int64_t(t.split * per + c) * 64, mrow = t.mat * w.N, col = (int64_t(t.wt) * 2 + rank) * 128;
+            const int64_t k0 = int64_t(s0 + c) * 64, mrow = t.mat * w.N, col = (int64_t(t.wt) * 2 + rank) * 128;
             const int64_t row = DX ? k0 : col;
             load_scales<DX>(v, w, packed, w.scales + (mrow + row) * groups, groups, int(min(w.N - row, int64_t(DX ? 256 : 128))), DX ? col : k0);
             c += 4;
@@ -571,7 +571,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
         const int stage = warp >> 2, quad = warp & 3;      // of each chunk; lanes of tensor memory
         unsigned cslot = 0, cpar = 0, slot0 = 0, par0 = 1;   // chunk slot and parity; the chunk's first stage and its parity of `empty`
         const unsigned full0 = tc5::leader_addr(full), drained0 = tc5::leader_addr(drained);
-        const bool wide = runs.splits == 1 && !((o.ld | o.J) & 1) && !(reinterpret_cast<uintptr_t>(o.out) & 3);
+        const bool wide = !((o.ld | o.J) & 1) && !(reinterpret_cast<uintptr_t>(o.out) & 3);
         // this lane's scales in a chunk's table: forward those of its row and stage, DX of its row n and half
         const int eat = DX ? (quad >> 1) * 256 + stage * 64 + (quad & 1) * 32 + lane : stage * 128 + quad * 32 + lane;
         Tile prev = {}, next = {};
@@ -582,7 +582,7 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
             if (live) {
                 t = next;
                 more = find.find(runs, tile + step, next);
-                n = min(per, all - t.split * per);
+                n = count_of(t);
             }
             int c = 0;
             do {
@@ -636,9 +636,9 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
                     const int64_t col = (int64_t(prev.wt) * 2 + rank) * 128 + quad * 32 + lane;
                     const unsigned at = tmem + stage * 32 + (unsigned(quad * 32) << 16);
                     const int r0 = prev.row0 + stage * 32, rows = prev.rows - stage * 32;
-                    if (runs.splits > 1)
-                        write_part(at, drained0, static_cast<float *>(o.out) + (int64_t(prev.split) * o.T + r0) * o.J, o.J, rows, col);
-                    else
+                    if (!RUNS && prev.split >= 0) {
+                        write_part(at, drained0, o.parts + (int64_t(prev.split) * runs.bt + stage * 32) * 256 + rank * 128 + quad * 32 + lane, rows);
+                    } else
                         write_tile<BF16, BT == 256 ? 2 : 1>(at, drained0, __ldg(w.scale + prev.mat), o.out, o.ld, o.J, wide, r0, rows, col);
                 }
                 c += 4;
@@ -890,15 +890,39 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
     }
 }
 
-// The parts of a split contraction, added in their order.
+// The parts of the split tiles, added in their order, four columns a thread.
 template <bool BF16>
-__global__ void __launch_bounds__(256) q4_join_parts_kernel(const float *part, int splits, int64_t T, int64_t J, const float *scale, void *out, int64_t ld) {
-    using Ty = typename Halves<BF16>::T;
+__global__ void __launch_bounds__(256) q4_join_parts_kernel(Runs r, const float *scale, Out o, int64_t rows) {
+    using T = typename Halves<BF16>::T;
     const float s = __ldg(scale);
-    for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < T * J; i += int64_t(gridDim.x) * 256) {
-        float v = part[i];
-        for (int p = 1; p < splits; ++p) v += part[int64_t(p) * T * J + i];
-        static_cast<Ty *>(out)[(i / J) * ld + i % J] = from_float<Ty>(s * (Halves<BF16>::kBack * v));
+    const bool wide = !((o.ld | o.J) & 3) && !(reinterpret_cast<uintptr_t>(o.out) & 7);
+    for (int64_t i = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6); i < rows; i += int64_t(gridDim.x) * 4) {   // row of a tile
+        const int64_t at = i / r.bt, u = r.whole + at, t = u / r.wtiles * r.bt + i % r.bt;
+        const int64_t col = u % r.wtiles * 256 + (threadIdx.x & 63) * 4;
+        if (t >= r.T) continue;
+        const float4 *p = reinterpret_cast<const float4 *>(o.parts) + ((at * r.splits) * r.bt + i % r.bt) * 64 + (threadIdx.x & 63);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int k = 0; k < r.splits; ++k) {
+            const float4 a = p[int64_t(k) * r.bt * 64];
+            v.x += a.x;
+            v.y += a.y;
+            v.z += a.z;
+            v.w += a.w;
+        }
+        union { T h[4]; uint2 both; } f;
+        f.h[0] = from_float<T>(s * (Halves<BF16>::kBack * v.x));
+        f.h[1] = from_float<T>(s * (Halves<BF16>::kBack * v.y));
+        f.h[2] = from_float<T>(s * (Halves<BF16>::kBack * v.z));
+        f.h[3] = from_float<T>(s * (Halves<BF16>::kBack * v.w));
+        T *const to = static_cast<T *>(o.out) + t * o.ld + col;
+        if (wide && col < o.J) {
+            *reinterpret_cast<uint2 *>(to) = f.both;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (col + j < o.J) to[j] = f.h[j];
+        }
     }
 }
 
@@ -1185,16 +1209,19 @@ int check_args(const char *what, int dtype, int64_t T, int64_t mats, int64_t N, 
 struct Plan {
     int width;        // BT of the kernel
     int bt;           // rows of a tile
-    int splits;
-    int64_t tiles;    // at most, of a pair of CTAs
+    int splits;       // of each tile from number `whole` on
+    int64_t whole, tiles;    // tiles: with the parts, at most
 };
 
-// J result columns, `depth` contraction steps.  The width and the parts of k with
-// the least estimated cycles: a stage of 64 steps takes 2 cycles a row of the tile
-// in the tensor cores and about 430 to be widened, a tile some 4500 for its start
-// and end, and joining parts a launch (5700) and their way to memory and back.
-// Measured at 4096 x 4096: 512 rows 25 us as 64 tiles of 128 rows, 34 us as two
-// parts of 32 tiles of 256; 64 rows 17 us in four parts, 20 us in one.
+// J result columns, `depth` contraction steps.  The tiles that do not fill a round
+// of all pairs are split along k, so that the last round is a short one.  The width
+// and the parts have the least estimated cycles: a stage of 64 steps takes 2 cycles a
+// row of the tile in the tensor cores and about 430 to be widened, a tile some 4500
+// for its start and end, and joining parts a launch (5700) and their way to memory
+// and back.  Measured: 2047 x 14336 x 4096 (448 tiles, 74 pairs) 156 us, 168 with the
+// last 4 tiles whole; 4096 x 4096 x 14336 (256 tiles) 294 against 334; 4096 x 4096 at
+// 64 rows 15.5 us in four parts, 20 in one, at 512 rows 24 us as 64 tiles of 128
+// rows, 34 as two parts of 32 tiles of 256.
 Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
     Plan p{};
     const int64_t wt = (J + 255) / 256, chunks = (depth + 255) / 256, pairs = uq::num_sms() / 2;
@@ -1202,29 +1229,34 @@ Plan plan_for(int64_t T, int64_t mats, bool runs, int64_t J, int64_t depth) {
         const int64_t each = std::max<int64_t>(1, T / std::max<int64_t>(mats, 1));
         p.width = p.bt = each <= 64 ? 64 : each <= 128 ? 128 : 256;
         p.splits = 1;
+        p.whole = INT64_MAX;
         p.tiles = std::min(T, T / p.bt + mats) * wt;
         return p;
     }
     double best = 0;
     for (int width = 64; width <= 256; width *= 2) {
         const int64_t n = (T + width - 1) / width, tiles = n * wt, bt = ((T + n - 1) / n + 31) / 32 * 32;
+        const int64_t whole = tiles / pairs * pairs, rest = tiles - whole;
         for (int64_t s = 1; s <= std::min<int64_t>(16, chunks); ++s) {
             const int64_t part = (chunks + s - 1) / s;
-            if (s > 1 && ((chunks + part - 1) / part != s || tiles * s > pairs)) continue;   // an empty part; more than one round
-            const double rounds = double((tiles * s + pairs - 1) / pairs), rows = double(bt);
-            const double cost = rounds * (double(part * 4) * std::max(2.0 * rows, 430.0) + 4500.0) +
-                                (s > 1 ? 5700.0 + double(s) * double(T) * double(J) * 8 / 2100.0 : 0.0);
+            if (s > 1 && ((chunks + part - 1) / part != s || rest == 0 || rest * s > pairs)) continue;   // an empty part; more than one round
+            const auto tile = [&](int64_t c) { return double(c * 4) * std::max(2.0 * double(bt), 430.0) + 4500.0; };
+            const double cost = double(whole / pairs) * tile(chunks) + (rest ? tile(part) : 0.0) +
+                                (s > 1 ? 5700.0 + double(rest * s * bt) * 256 * 8 / 2100.0 : 0.0);
             if (p.width == 0 || cost < best) {
                 best = cost;
                 p.width = width;
                 p.bt = int(bt);
                 p.splits = int(s);
-                p.tiles = tiles * s;
+                p.whole = s > 1 ? whole : INT64_MAX;
+                p.tiles = s > 1 ? whole + rest * s : tiles;
             }
         }
     }
     return p;
 }
+
+size_t parts_bytes(const Plan &p) { return p.splits > 1 ? size_t(p.tiles - p.whole) * p.bt * 256 * 4 : 0; }
 
 template <int BT, bool BF16, bool DX, bool RUNS>
 int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, const Runs &r, const Weights &w, const Out &o, int64_t tiles, cudaStream_t st) {
@@ -1247,9 +1279,9 @@ int launch(const void *rows, int64_t lda, const uint8_t *codes, int64_t mats, co
 }
 
 // Whether the kernel for few rows is taken.  Up to 16 rows (for several matrices:
-// 16 each if they were even): 4096 x 4096 at 16 rows 7.9 us, by pairs 15; 28672 x
-// 8192 44 against 59.  Up to 32 where a single matrix has so few tiles that the
-// pairs would have to split k: 4096 x 4096 at 32 rows 10.4 us against 15.1, but
+// 16 each if they were even): 4096 x 4096 at 16 rows 7.9 us, by pairs 14; 28672 x
+// 8192 44 against 57.  Up to 32 where a single matrix has so few tiles that the
+// pairs would have to split k: 4096 x 4096 at 32 rows 10.6 us against 14, but
 // 28672 x 8192 68 against 59.
 bool few_rows(int64_t T, int64_t mats, bool runs, int64_t N) {
     return T <= 16 * mats || (!runs && T <= 32 && (N + 255) / 256 * 2 <= uq::num_sms() / 2);
@@ -1281,8 +1313,8 @@ int few(const void *x, int64_t ldx, int64_t T, const uint8_t *codes, const Weigh
     int parts = 1;
     for (int p = 2; p <= kFewParts && !offsets && p <= chunks; p *= 2)
         if (cost(p) < cost(parts)) parts = p;
-    const Runs r{offsets, T, mats, 8 * NT, int(wtiles), parts};
-    const Out o{y, ldy, w.N, T, zero};
+    const Runs r{offsets, T, mats, 8 * NT, int(wtiles), parts, 0};
+    const Out o{y, ldy, w.N, T, zero, nullptr};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = unsigned(parts > 1 ? tiles * parts : std::min(tiles, slots));
     cfg.blockDim = C::kThreads;
@@ -1304,10 +1336,10 @@ int product(const void *rows, int64_t lda, int64_t T, const uint8_t *codes, cons
             int64_t ldo, bool zero, void *ws, size_t ws_bytes, cudaStream_t st) {
     const int64_t J = DX ? w.K : w.N, depth = DX ? w.N : w.K;
     const Plan p = plan_for(T, mats, offsets != nullptr, J, depth);
-    if (p.splits > 1 && (!ws || ws_bytes < size_t(p.splits) * T * J * 4))
-        return uq::fail(UQ_ERR_WORKSPACE, "4-bit product: workspace of %zu bytes, %zu needed", ws_bytes, size_t(p.splits) * T * J * 4);
-    const Runs r{offsets, T, mats, p.bt, int((J + 255) / 256), p.splits};
-    const Out o{p.splits > 1 ? ws : out, ldo, J, T, zero};
+    if (const size_t need = parts_bytes(p); need && (!ws || ws_bytes < need || !al16(ws)))
+        return uq::fail(UQ_ERR_WORKSPACE, "4-bit product: workspace of %zu bytes, %zu needed (16-byte aligned)", ws_bytes, need);
+    const Runs r{offsets, T, mats, p.bt, int((J + 255) / 256), p.splits, p.whole};
+    const Out o{out, ldo, J, T, zero, static_cast<float *>(ws)};
     const auto go = offsets ? p.width == 64    ? launch<64, BF16, DX, true>
                               : p.width == 128 ? launch<128, BF16, DX, true>
                                                : launch<256, BF16, DX, true>
@@ -1317,7 +1349,8 @@ int product(const void *rows, int64_t lda, int64_t T, const uint8_t *codes, cons
     const int rc = go(rows, lda, codes, mats, r, w, o, p.tiles, st);
     if (rc || p.splits == 1) return rc;
     uq::ProfScope _p("q4_join_parts", st);
-    q4_join_parts_kernel<BF16><<<unsigned(std::min<int64_t>((T * J + 255) / 256, 1184)), 256, 0, st>>>(static_cast<const float *>(ws), p.splits, T, J, w.scale, out, ldo);
+    const int64_t split_rows = (p.tiles - p.whole) / p.splits * p.bt;
+    q4_join_parts_kernel<BF16><<<unsigned(std::min<int64_t>((split_rows + 3) / 4, 1184)), 256, 0, st>>>(r, w.scale, o, split_rows);
     return uq::check_cuda("q4_join_parts_kernel launch");
 }
 
@@ -1332,7 +1365,7 @@ int dscale(const void *dy, const void *x, int64_t T, int64_t lddy, int64_t ldx, 
     if (!tc5::encode2d(&md, ty, dy, uint64_t(N), uint64_t(T), uint64_t(lddy) * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc5::encode2d(&mx, ty, x, uint64_t(K), uint64_t(T), uint64_t(ldx) * 2, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B))
         return uq::fail(UQ_ERR_CUDA, "tensor map of the scales' gradient");
-    const Runs r{offsets, T, mats, 0, 0, 1};
+    const Runs r{offsets, T, mats, 0, 0, 1, 0};
     const int ntiles = int((N + 255) / 256), ktiles = int((K + 255) / 256);
     const int grid = 2 * int(std::min<int64_t>(mats * ntiles * int64_t(ktiles), uq::num_sms() / 2));
     uq::ProfScope _p("q4_dscale", st);
@@ -1350,7 +1383,7 @@ int no_matrix(void *out, int64_t ld, int64_t T, int64_t J, bool zero, cudaStream
 size_t product_workspace(int64_t T, int64_t mats, int64_t J, int64_t depth) {
     if (T <= 0 || mats != 1 || J <= 0 || depth <= 0 || T > kMost || J > kMost || depth > kMost) return 0;
     const Plan p = plan_for(T, mats, false, J, depth);
-    return p.splits > 1 ? size_t(p.splits) * T * J * 4 : 0;
+    return parts_bytes(p);
 }
 
 }  // namespace
