@@ -15,6 +15,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200, sm_100a)")
 
 
+def pytest_collection_modifyitems(items):
+    """test_recipe_layer asserts the error sums of the rotated matrix, which at padded widths count the padded columns too;
+    the layer reports those of its reconstruction (test_gpu_q4_layer.py has them).  Its padded sizes fail, as they should,
+    and run last, so that ``-x`` stops behind everything else."""
+    padded = ("40-300-5-32", "24-14336-3-256", "64-96-33-128")
+    items.sort(key=lambda i: i.name.startswith("test_recipe_layer[") and any(p in i.name for p in padded))
+
+
 def load_golden(name):
     with np.load(os.path.join(GOLDEN, name), allow_pickle=False) as z:
         return {k: z[k] for k in z.files}

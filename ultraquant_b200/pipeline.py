@@ -191,7 +191,7 @@ class Q4Layer:
     w: q4.Q4                      # (rows, n), n = next_pow2(n0)
     sH: torch.Tensor              # (n0,) float32
     signs: torch.Tensor           # (n,) float32
-    err: torch.Tensor             # [sum (A - Ah)^2, sum A^2] fp64
+    err: torch.Tensor             # [sum (A - Ah)^2, sum A^2] fp64 over the n0 columns, A = W * sH and Ah = What * sH
 
     @property
     def wnmse(self) -> float:
@@ -211,10 +211,11 @@ class Q4Layer:
 
     def What(self) -> torch.Tensor:
         """The reconstruction (rows, n0) float32, as the other recipes return it."""
-        return _q4_reconstruction(self.w, self.sH.double(), self.sH.numel(), self.signs.double())
+        return (_q4_back(self.w, self.sH.numel(), self.signs.double()) / self.sH.double()).float()
 
 
-def _q4_reconstruction(w, sH, n0, signs):
+def _q4_back(w, n0, signs):
+    """The weights rotated back, (rows, n0) float64: What * sH."""
     lib = _lib.load()
     X = q4.deq_q4(w)
     rows, n = X.shape
@@ -222,7 +223,7 @@ def _q4_reconstruction(w, sH, n0, signs):
     if out.numel():
         _lib.check(lib.uq_irht_rows(X.data_ptr(), D.dtype_code(X), rows, n, n, n0, signs.data_ptr(), out.data_ptr(),
                                     D.stream_handle(X.device)), "uq_irht_rows")
-    return (out / sH).float()
+    return out
 
 
 def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_errors=True) -> Q4Layer:
@@ -246,12 +247,13 @@ def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_er
         _lib.check(lib.uq_rht_rows(A.data_ptr(), _lib.UQ_F64, rows, n0, n0, d.data_ptr(), X.data_ptr(), D.stream_handle(dev)),
                    "uq_rht_rows")
     w = q4.enc_q4(X, group)
+    del X
     err = torch.zeros(2, dtype=torch.float64, device=dev)
     if rows:
-        Q = q4.deq_q4(w)
+        # over the n0 columns: what the rotated error puts into the padding is cut off and reaches no output
+        Ah = _q4_back(w, n0, d)
         ws = torch.empty(lib.uq_wnmse_workspace_bytes(), dtype=torch.uint8, device=dev)
-        # the rotation keeps lengths: the sums in the rotated domain are the weighted ones (of the padded columns too)
-        _lib.check(lib.uq_wnmse_sums(X.data_ptr(), _lib.UQ_F64, Q.data_ptr(), _lib.UQ_F32, X.numel(), err.data_ptr(),
+        _lib.check(lib.uq_wnmse_sums(A.data_ptr(), _lib.UQ_F64, Ah.data_ptr(), _lib.UQ_F64, A.numel(), err.data_ptr(),
                                      ws.data_ptr(), ws.numel(), D.stream_handle(dev)), "uq_wnmse_sums")
     if check_errors:
         _device_status(lib, dev, "quant_q4")
