@@ -1,5 +1,5 @@
-"""pipeline.quant_q4_device and its layer: the reported error is that of the reconstruction over the matrix's own columns.
-Bounds are counted as in test_gpu_q4.py."""
+"""pipeline.quant_q4_device and its layer: the reported error is that of the reconstruction over the matrix's own columns,
+and the result does not go by the unit of the imatrix.  Bounds are counted as in test_gpu_q4.py."""
 import numpy as np
 import pytest
 import torch
@@ -44,6 +44,7 @@ def test_error_sums_are_those_of_the_reconstruction(rows, n0, group):
     Ah = oracle.irht_rows(Xq, n0)
     want = ((A - Ah) ** 2).sum() / (A ** 2).sum()
     assert abs(layer.wnmse - want) <= 1e-12
+    assert abs(layer.err[1].item() / (A ** 2).sum() - 1) <= 1e-12
     # What() is Ah / sH, both in float32: times sH off by at most 2^-23 of Ah's size
     d = A - layer.What().double().cpu().numpy() * sH
     slack = 4 * U * np.linalg.norm(Ah) * (np.linalg.norm(A - Ah) + U * np.linalg.norm(Ah)) / (A ** 2).sum()
@@ -68,15 +69,17 @@ def check_layer(layer, W, H, x, dy, group):
     x = x.detach().requires_grad_()
     y = layer(x)
     (dx,) = torch.autograd.grad(y, x, dy)
-    # rotated activations: a float32 transform (log2 n + 6 roundings of values of at most the row's length), one rounding to dt
+    # rotated activations: a float32 transform (log2 n + 6 roundings of values of at most the row's length), one rounding to
+    # dt; a subnormal one is half a step of the type at the size that the layer gives them
     xr = torch.from_numpy(oracle.rht_rows((x.detach().double() / sH).cpu().numpy())).cuda()
-    dxr = HALF[dt] * xr.abs() + (np.log2(n) + 6) * 2 * U * xr.norm(dim=1, keepdim=True) + TINY[dt]
+    unit = (layer.rotate(x.detach()).double().norm() / xr.norm()).item()
+    dxr = HALF[dt] * xr.abs() + (np.log2(n) + 6) * 2 * U * xr.norm(dim=1, keepdim=True) + TINY[dt] / unit
     bound = dxr @ Q.abs().T + 2 * (n + 2) * U * ((xr.abs() + dxr) @ Q.abs().T)
     exact = xr @ Q.T
     off = (y.detach().double() - exact).abs()
     assert (off <= bound * (1 + HALF[dt]) + HALF[dt] * exact.abs() + TINY[dt]).all(), (off / exact.abs().mean()).max()
     g = dy.double() @ Q
-    dg = HALF[dt] * g.abs() + 2 * (W.shape[0] + 2) * U * (dy.double().abs() @ Q.abs()) + TINY[dt]
+    dg = HALF[dt] * g.abs() + 2 * (W.shape[0] + 2) * U * (dy.double().abs() @ Q.abs()) + TINY[dt] * unit
     back = torch.from_numpy(oracle.irht_rows(g.cpu().numpy(), n0)).cuda() / sH
     tol = (dg.norm(dim=1, keepdim=True) + (np.log2(n) + 6) * 2 * U * g.norm(dim=1, keepdim=True)) / sH
     assert ((dx.double() - back).abs() <= tol * 1.001 + HALF[dt] * (back.abs() + tol) + TINY[dt]).all()
@@ -95,3 +98,24 @@ def test_layer_values_and_gradient(rows, n0, group, T, dt):
     W, H = make(rows, n0, n0)
     layer = pipeline.quant_q4_device(W, H, group)
     check_layer(layer, W, H, acts(T, n0, DT[dt], 1), acts(T, rows, DT[dt], 2), group)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("n0", [256, 300])
+def test_layer_does_not_go_by_the_unit_of_the_imatrix(n0, dt):
+    """The whitening and its inverse cancel: a factor on H changes nothing.  By a power of 4 the bits stay the same."""
+    from ultraquant_b200 import pipeline
+    W, H = make(48, n0, 7)
+    x, dy = acts(9, n0, DT[dt], 3), acts(9, 48, DT[dt], 4)
+    base = pipeline.quant_q4_device(W, H, 32)
+    y0, dx0 = check_layer(base, W, H, x, dy, 32)
+    for unit in (4.0 ** -100, 4.0 ** -17, 4.0 ** -3, 4.0 ** 9, 4.0 ** 40, 4.0 ** 100):
+        layer = pipeline.quant_q4_device(W, H * unit, 32)
+        y = layer(x.clone().requires_grad_())
+        assert torch.equal(y.detach(), y0), unit
+        xg = x.clone().requires_grad_()
+        assert torch.equal(torch.autograd.grad(layer(xg), xg, dy)[0], dx0), unit
+        assert torch.equal(layer.What(), base.What()) and layer.wnmse == base.wnmse
+        assert torch.equal(layer.err, base.err * unit)
+    for unit in (1e-60, 1e-10, 3e-4, 7.0, 1e12, 1e60):
+        check_layer(pipeline.quant_q4_device(W, H * unit, 32), W, H * unit, x, dy, 32)

@@ -189,9 +189,10 @@ class Q4Layer:
     without What being formed.  ``w``: the 4-bit codes of rht_rows(W * sH); ``scales`` of a call: the trained group scales
     (see q4.linear)."""
     w: q4.Q4                      # (rows, n), n = next_pow2(n0)
-    sH: torch.Tensor              # (n0,) float32
+    sH: torch.Tensor              # (n0,) float32: root of the clamped imatrix, times a power of two (quant_q4_device)
     signs: torch.Tensor           # (n,) float32
     err: torch.Tensor             # [sum (A - Ah)^2, sum A^2] fp64 over the n0 columns, A = W * sH and Ah = What * sH
+                                  # (sH without the power of two)
 
     @property
     def wnmse(self) -> float:
@@ -229,7 +230,11 @@ def _q4_back(w, n0, signs):
 def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_errors=True) -> Q4Layer:
     """The builders' recipe (buildalloc.py:21-24: clamp the imatrix, whiten, rotate, quantize) with 4-bit codes and group
     scales in place of the lattice (q4.enc_q4; no counterpart in the reference).  W (rows, n0) float32 / float64 and H (n0)
-    on the device; rows of up to 32768 columns.  The layer multiplies with the codes themselves."""
+    on the device; rows of up to 32768 columns.  The layer multiplies with the codes themselves.
+
+    sH is kept times the power of two that brings the root mean square of 1 / sH to 0.5 .. 1: whitened activations are of
+    the activations' size whatever the unit of H, and stay within a 16-bit type where those do.  Nothing else depends on
+    it: not the codes, not the reconstruction, and ``err`` is that of W times the clamped imatrix's root itself."""
     lib = _lib.load()
     dev = W.device
     if W.dim() != 2 or H.shape != (W.shape[1],) or W.shape[1] == 0:
@@ -240,6 +245,10 @@ def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_er
         raise ValueError(f"quant_q4: {n} rotated columns are not whole groups of {group}")
     H = H.to(device=dev, dtype=torch.float64)
     sH = torch.maximum(H, H.max() * 1e-3).sqrt()
+    top = sH.max()
+    power = torch.frexp((top / sH).square().mean().sqrt() / top).exponent.long().clamp(-1022, 1022)
+    unit = ((power + 1023) << 52).view(torch.float64)         # 2^power from its bits
+    sH = sH * unit
     A = (W.double() * sH).contiguous()
     d = D.signs(n, seed, dev)
     X = torch.empty((rows, n), dtype=torch.float64, device=dev)
@@ -255,6 +264,7 @@ def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_er
         ws = torch.empty(lib.uq_wnmse_workspace_bytes(), dtype=torch.uint8, device=dev)
         _lib.check(lib.uq_wnmse_sums(A.data_ptr(), _lib.UQ_F64, Ah.data_ptr(), _lib.UQ_F64, A.numel(), err.data_ptr(),
                                      ws.data_ptr(), ws.numel(), D.stream_handle(dev)), "uq_wnmse_sums")
+        err = err / unit / unit
     if check_errors:
         _device_status(lib, dev, "quant_q4")
     return Q4Layer(w, sH.float(), d.float(), err)
