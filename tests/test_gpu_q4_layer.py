@@ -1,5 +1,8 @@
 """pipeline.quant_q4_device and its layer: the reported error is that of the reconstruction over the matrix's own columns,
-and the result does not go by the unit of the imatrix.  Bounds are counted as in test_gpu_q4.py."""
+the result does not go by the unit of the imatrix, and the weights' device is the one that is launched on.  Bounds are
+counted as in test_gpu_q4.py."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -119,3 +122,47 @@ def test_layer_does_not_go_by_the_unit_of_the_imatrix(n0, dt):
         assert torch.equal(layer.err, base.err * unit)
     for unit in (1e-60, 1e-10, 3e-4, 7.0, 1e12, 1e60):
         check_layer(pipeline.quant_q4_device(W, H * unit, 32), W, H * unit, x, dy, 32)
+
+
+def test_layer_launches_with_the_weights_device_current(monkeypatch):
+    """With another device current each launch is made inside torch.cuda.device(the weights' device): seen from a device
+    number that is said to be another one."""
+    from ultraquant_b200 import _lib, pipeline
+    real = torch.cuda.device
+    inside = []
+
+    class Spy(real):
+        def __enter__(self):
+            inside.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *a):
+            inside.pop()
+            return super().__exit__(*a)
+
+    lib, met = _lib.load(), set()
+
+    class Watched:
+        def __getattr__(self, name):
+            fn = getattr(lib, name)
+            if name in ("uq_fwht", "uq_rht_rows", "uq_irht_rows", "uq_wnmse_sums", "uq_device_errors"):
+                def call(*a):
+                    met.add(name)
+                    assert inside and inside[-1] == 0, f"{name} outside the weights' device"
+                    return fn(*a)
+                return call
+            return fn
+
+    W, H = make(8, 96, 1)
+    x = acts(3, 96, torch.bfloat16, 1).requires_grad_()
+    with contextlib.ExitStack() as stack:
+        m = stack.enter_context(pytest.MonkeyPatch.context())
+        m.setattr(torch.cuda, "current_device", lambda: inside[-1] if inside else 1)
+        m.setattr(torch.cuda, "device", Spy)
+        m.setattr(_lib, "load", lambda *a: Watched())
+        layer = pipeline.quant_q4_device(W, H, 32)
+        y = layer(x)
+        layer.rotate(x.detach())
+        layer.What()
+        torch.autograd.grad(y, x, torch.ones_like(y))
+    assert met == {"uq_fwht", "uq_rht_rows", "uq_irht_rows", "uq_wnmse_sums", "uq_device_errors"}

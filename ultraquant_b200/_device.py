@@ -9,6 +9,7 @@ exactly like the reference's own ``torch.tensor(..., device)`` /
 from __future__ import annotations
 
 import threading
+from contextlib import nullcontext
 
 import numpy as np
 import torch
@@ -30,6 +31,11 @@ def device() -> torch.device:
 
 def stream_handle(dev: torch.device | None = None) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+def on(dev: torch.device):
+    """Context in which the kernels of ``dev`` are launched: with it as the current device."""
+    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

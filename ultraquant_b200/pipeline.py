@@ -37,7 +37,8 @@ class QuantResult:
 def _device_status(lib, dev, what):
     """Raise if a bounded device wait of the kernels just launched gave up
     (their outputs would be wrong).  Synchronises the stream."""
-    _lib.check(lib.uq_device_errors(D.stream_handle(dev)), what)
+    with D.on(dev):
+        _lib.check(lib.uq_device_errors(D.stream_handle(dev)), what)
 
 
 def quant_trellis_device(W: torch.Tensor, H: torch.Tensor, L=12, R=2, seg=64, scale_group=256, seed=0,
@@ -222,8 +223,9 @@ def _q4_back(w, n0, signs):
     rows, n = X.shape
     out = torch.empty((rows, n0), dtype=torch.float64, device=X.device)
     if out.numel():
-        _lib.check(lib.uq_irht_rows(X.data_ptr(), D.dtype_code(X), rows, n, n, n0, signs.data_ptr(), out.data_ptr(),
-                                    D.stream_handle(X.device)), "uq_irht_rows")
+        with D.on(X.device):
+            _lib.check(lib.uq_irht_rows(X.data_ptr(), D.dtype_code(X), rows, n, n, n0, signs.data_ptr(), out.data_ptr(),
+                                        D.stream_handle(X.device)), "uq_irht_rows")
     return out
 
 
@@ -253,8 +255,9 @@ def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_er
     d = D.signs(n, seed, dev)
     X = torch.empty((rows, n), dtype=torch.float64, device=dev)
     if rows:
-        _lib.check(lib.uq_rht_rows(A.data_ptr(), _lib.UQ_F64, rows, n0, n0, d.data_ptr(), X.data_ptr(), D.stream_handle(dev)),
-                   "uq_rht_rows")
+        with D.on(dev):
+            _lib.check(lib.uq_rht_rows(A.data_ptr(), _lib.UQ_F64, rows, n0, n0, d.data_ptr(), X.data_ptr(),
+                                       D.stream_handle(dev)), "uq_rht_rows")
     w = q4.enc_q4(X, group)
     del X
     err = torch.zeros(2, dtype=torch.float64, device=dev)
@@ -262,8 +265,9 @@ def quant_q4_device(W: torch.Tensor, H: torch.Tensor, group=32, seed=0, check_er
         # over the n0 columns: what the rotated error puts into the padding is cut off and reaches no output
         Ah = _q4_back(w, n0, d)
         ws = torch.empty(lib.uq_wnmse_workspace_bytes(), dtype=torch.uint8, device=dev)
-        _lib.check(lib.uq_wnmse_sums(A.data_ptr(), _lib.UQ_F64, Ah.data_ptr(), _lib.UQ_F64, A.numel(), err.data_ptr(),
-                                     ws.data_ptr(), ws.numel(), D.stream_handle(dev)), "uq_wnmse_sums")
+        with D.on(dev):
+            _lib.check(lib.uq_wnmse_sums(A.data_ptr(), _lib.UQ_F64, Ah.data_ptr(), _lib.UQ_F64, A.numel(), err.data_ptr(),
+                                         ws.data_ptr(), ws.numel(), D.stream_handle(dev)), "uq_wnmse_sums")
         err = err / unit / unit
     if check_errors:
         _device_status(lib, dev, "quant_q4")

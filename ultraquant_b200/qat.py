@@ -50,9 +50,10 @@ def _fwht_call(x2d: torch.Tensor, n: int, signs, colscale, direction: int, ncols
     lib = _lib.load()
     rows, ncols_in = x2d.shape
     out = torch.empty((rows, ncols_out), dtype=x2d.dtype, device=x2d.device)
-    _lib.check(lib.uq_fwht(x2d.data_ptr() if x2d.numel() else None, D.dtype_code(x2d), rows, n, max(ncols_in, 1),
-                           ncols_in, D.ptr(signs), D.ptr(colscale), direction, out.data_ptr() if out.numel() else None,
-                           max(ncols_out, 1), ncols_out, D.stream_handle(x2d.device)), "fwht")
+    with D.on(x2d.device):
+        _lib.check(lib.uq_fwht(x2d.data_ptr() if x2d.numel() else None, D.dtype_code(x2d), rows, n, max(ncols_in, 1),
+                               ncols_in, D.ptr(signs), D.ptr(colscale), direction, out.data_ptr() if out.numel() else None,
+                               max(ncols_out, 1), ncols_out, D.stream_handle(x2d.device)), "fwht")
     return out
 
 
