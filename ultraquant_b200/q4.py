@@ -161,7 +161,7 @@ def _trained(w: Q4, scales) -> torch.Tensor:
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """(..., n) as a matrix whose rows the kernels can read: unit inner stride, 16-byte aligned base and row stride."""
     if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
+        x = x.reshape(x.shape[:-1].numel(), x.shape[-1])     # not -1: there may be no columns
     T, n = x.shape
     ld, inner = x.stride()
     if T <= 1:
