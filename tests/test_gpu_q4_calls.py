@@ -1,4 +1,5 @@
 """Calls of the 4-bit operators at their edges."""
+import numpy as np
 import pytest
 import torch
 
@@ -14,6 +15,47 @@ def q4():
 def no_device_errors():
     yield
     q4().check_errors()
+
+
+def constant(shape, q, e, s, group=32):
+    *lead, N, K = shape
+    codes = torch.full((*lead, N, K // 2), (q + 8) * 17, dtype=torch.uint8, device="cuda")
+    return q4().Q4(codes, torch.full((*lead, N, K // group), e, device="cuda").to(torch.float8_e4m3fn), torch.full(tuple(lead), s, device="cuda"))
+
+
+# ---- sums before the scale -------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,N,K", [(1, 300, 8192), (12, 140, 8192), (30, 140, 64), (40, 2048, 8192), (300, 256, 8192), (515, 264, 320)])
+def test_sum_before_the_scale_may_pass_the_largest_float(T, N, K):
+    """y = s sum e q x is a bfloat16 although sum e q x is beyond float32 (weights and results of ordinary proportion)."""
+    s, x0 = 2.0 ** -24, 2.0 ** 111
+    w = constant((N, K), 7, 448.0, s)
+    x = torch.full((T, K), x0, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    y = q4().linear(x, w)
+    (dx,) = torch.autograd.grad(y, x, torch.full_like(y, x0))
+    assert float(K) * 3136 * x0 > 3.5e38
+    # exact sums of equal terms: multiples of 3136 = 49 * 2^6 below 49 * 2^13 terms, so only the result rounds
+    assert torch.equal(y, torch.full_like(y, K * 3136 * x0 * s)) and torch.equal(dx, torch.full_like(dx, N * 3136 * x0 * s))
+
+
+def test_sum_before_the_scale_may_pass_the_largest_float_with_experts():
+    w = constant((5, 136, 1024), -8, 448.0, 2.0 ** -30)
+    for counts in ([1, 0, 3, 2, 1], [40, 0, 70, 2, 300]):
+        T = sum(counts)
+        off = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+        x = torch.full((T, 1024), 2.0 ** 112, device="cuda", dtype=torch.bfloat16).requires_grad_()
+        y = q4().grouped_linear(x, off, w)
+        (dx,) = torch.autograd.grad(y, x, torch.full_like(y, 2.0 ** 112))
+        assert torch.equal(y, torch.full_like(y, -1024 * 3584 * 2.0 ** 82)) and torch.equal(dx, torch.full_like(dx, -136 * 3584 * 2.0 ** 82))
+
+
+@pytest.mark.parametrize("T", [2, 40])
+def test_scales_from_the_smallest_to_the_largest(T):
+    """s from 2^-126 to 2^120: the result neither overflows nor is lost where it is an ordinary number."""
+    for k in (-126, -117, -60, -1, 0, 1, 60, 112, 113, 114, 120):
+        w = constant((72, 128), 3, 1.0, 2.0 ** k)
+        x = torch.full((T, 128), 2.0 ** -max(min(k, 100), -100), device="cuda", dtype=torch.bfloat16)
+        assert torch.equal(q4().linear(x, w), torch.full((T, 72), 384 * 2.0 ** (k - max(min(k, 100), -100)), device="cuda", dtype=torch.bfloat16)), k
 
 
 # ---- nothing to do ---------------------------------------------------------------------------------------------

@@ -269,13 +269,20 @@ struct Out {
     float *parts;     // of split tiles: (tile, part, bt, 256)
 };
 
+// A finished sum times the matrix's s, then 1 / kUnit: sum / kUnit alone may be beyond
+// float32 where the result is not (weights of 2^-10 and bfloat16 activations of 2^115).
+// In this order nothing passes the range before the result does; a result below 2^-112
+// is off by at most 2^-136 more (half of float32's least step, times 2^14), a quarter
+// of bfloat16's least rounding.
+template <bool BF16> __device__ __forceinline__ float finish(float v, float s) { return (s * v) * Halves<BF16>::kBack; }
+
 // Register j of lane i: row j, column i of a 32 x 32 piece of the result.
 // pack_piece: rows 2 j and 2 j + 1 in the halves of v[j], scaled and rounded.
 template <bool BF16> __device__ __forceinline__ void pack_piece(const uint32_t (&r)[32], float s, uint32_t (&v)[16]) {
     using T = typename Halves<BF16>::T;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-        T two[2] = {from_float<T>(s * (Halves<BF16>::kBack * __uint_as_float(r[2 * j]))), from_float<T>(s * (Halves<BF16>::kBack * __uint_as_float(r[2 * j + 1])))};
+        T two[2] = {from_float<T>(finish<BF16>(__uint_as_float(r[2 * j]), s)), from_float<T>(finish<BF16>(__uint_as_float(r[2 * j + 1]), s))};
         v[j] = *reinterpret_cast<const uint32_t *>(two);
     }
 }
@@ -857,7 +864,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
                         const float v = acc[m][0][u][i] + acc[m][1][u][i];
                         const int64_t n = int64_t(t.wt) * kFewRows + c;
                         if (parts > 1) sums[r * kFewRows + c] = v;
-                        else if (r < t.rows && n < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + n] = from_float<T>(scale * (Halves<BF16>::kBack * v));
+                        else if (r < t.rows && n < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + n] = from_float<T>(finish<BF16>(v, scale));
                     }
         }
         if (RUNS && o.zero_rest && !wt.fail) zero_rows<T>(o, find.begin, find.end(runs), kFewWarps * 32);
@@ -883,7 +890,7 @@ q4_few_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_constan
 #pragma unroll
                 for (int p = 0; p < kFewParts; ++p) v += f[p];
                 const int64_t col = int64_t(t.wt) * kFewRows + n;
-                if (col < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + col] = from_float<T>(scale * (Halves<BF16>::kBack * v));
+                if (col < w.N) static_cast<T *>(o.out)[int64_t(t.row0 + r) * o.ld + col] = from_float<T>(finish<BF16>(v, scale));
             }
         }
         tc5::cluster_sync();   // no block leaves while another reads its sums
@@ -911,10 +918,10 @@ __global__ void __launch_bounds__(256) q4_join_parts_kernel(Runs r, const float 
             v.w += a.w;
         }
         union { T h[4]; uint2 both; } f;
-        f.h[0] = from_float<T>(s * (Halves<BF16>::kBack * v.x));
-        f.h[1] = from_float<T>(s * (Halves<BF16>::kBack * v.y));
-        f.h[2] = from_float<T>(s * (Halves<BF16>::kBack * v.z));
-        f.h[3] = from_float<T>(s * (Halves<BF16>::kBack * v.w));
+        f.h[0] = from_float<T>(finish<BF16>(v.x, s));
+        f.h[1] = from_float<T>(finish<BF16>(v.y, s));
+        f.h[2] = from_float<T>(finish<BF16>(v.z, s));
+        f.h[3] = from_float<T>(finish<BF16>(v.w, s));
         T *const to = static_cast<T *>(o.out) + t * o.ld + col;
         if (wide && col < o.J) {
             *reinterpret_cast<uint2 *>(to) = f.both;
