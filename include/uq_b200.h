@@ -412,7 +412,8 @@ int uq_q4_round_scales(const float *c, int64_t mats, int64_t n, uint8_t *scales,
  * rows offsets[i] .. offsets[i + 1] - 1 are multiplied by matrix i; each offset
  * is taken as at least its predecessors and at most T (a violation is reported
  * by uq_q4_errors).  Rows outside offsets[0] .. offsets[mats] are set to zero if
- * zero_rest, else left as they were.  x: 16-byte aligned, ldx a multiple of 8. */
+ * zero_rest, else left as they were.  x: 16-byte aligned, ldx a multiple of 8.
+ * y shares no memory with what is read. */
 size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K);
 int uq_q4_linear(const void *x, int dtype, int64_t T, int64_t ldx, const uint8_t *codes,
                  const uint8_t *scales, const float *scale, int64_t mats, int64_t N, int64_t K,

@@ -58,6 +58,66 @@ def test_scales_from_the_smallest_to_the_largest(T):
         assert torch.equal(q4().linear(x, w), torch.full((T, 72), 384 * 2.0 ** (k - max(min(k, 100), -100)), device="cuda", dtype=torch.bfloat16)), k
 
 
+# ---- outputs that are given ------------------------------------------------------------------------------------
+
+def experts(seed=0, N=64, K=64):
+    g = torch.Generator().manual_seed(seed)
+    return q4().enc_q4(torch.randn(3, N, K, generator=g), 32), torch.tensor([0, 300, 301, 700], dtype=torch.int32, device="cuda")
+
+
+def rows(T, n, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(T, n, generator=g, device="cuda").bfloat16()
+
+
+def test_out_that_overlaps_what_is_read_is_refused():
+    m = q4()
+    w, off = experts()
+    x = rows(700, 64, 1)
+    want = m.grouped_linear(x, off, w)
+    kept = x.clone()
+    for out in (x, torch.as_strided(x, (700, 64), (64, 1), 0)):
+        with pytest.raises(ValueError, match="overlap"):
+            m.grouped_linear(x, off, w, out=out)
+    buf = torch.zeros(701 * 64, device="cuda", dtype=torch.bfloat16)
+    a, b = buf[: 700 * 64].view(700, 64), buf[64:].view(700, 64)
+    with pytest.raises(ValueError, match="overlap"):
+        m.grouped_linear(a, off, w, out=b)
+    wide = torch.zeros(700, 160, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        m.grouped_linear(wide[:, :64], off, w, out=wide[:, 63:127])
+    with pytest.raises(ValueError, match="overlap"):
+        m.grouped_linear(wide[:, 96:160], off, w, out=wide[:, 40:104])
+    assert torch.equal(x, kept) and not wide.any() and not buf.any()
+    # offsets and weights are read as well
+    raw = torch.empty(700 * 64 * 2, dtype=torch.uint8, device="cuda")
+    inside = raw[: 4 * 4].view(torch.int32)
+    inside.copy_(off)
+    with pytest.raises(ValueError, match="overlap"):
+        m.grouped_linear(x, inside, w, out=raw.view(torch.bfloat16).view(700, 64))
+    assert torch.equal(inside, off) and torch.equal(m.grouped_linear(x, off, w), want)
+
+
+def test_out_beside_what_is_read_is_taken():
+    """Parts of one buffer that share no element: before, behind, and columns of the same rows."""
+    m = q4()
+    w, off = experts()
+    x = rows(700, 64, 2)
+    want = m.grouped_linear(x, off, w)
+    buf = torch.zeros(1400 * 64, device="cuda", dtype=torch.bfloat16)
+    a, b = buf[: 700 * 64].view(700, 64), buf[700 * 64 :].view(700, 64)
+    for i, o in ((a, b), (b, a)):
+        i.copy_(x)
+        assert torch.equal(m.grouped_linear(i, off, w, out=o), want)
+    wide = torch.zeros(700, 128, device="cuda", dtype=torch.bfloat16)
+    for i, o in ((wide[:, :64], wide[:, 64:]), (wide[:, 64:], wide[:, :64])):
+        i.copy_(x)
+        assert torch.equal(m.grouped_linear(i, off, w, out=o), want)
+    half = torch.zeros(1400, 64, device="cuda", dtype=torch.bfloat16)     # every other row
+    half[::2] = x
+    assert torch.equal(m.grouped_linear(half[::2], off, w, out=half[1::2]), want) and torch.equal(half[::2], x)
+
+
 # ---- nothing to do ---------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("shape", [(64,), (3, 64), (2, 3, 64), (2, 0, 3, 64), (0, 64)])

@@ -178,6 +178,29 @@ def _ld(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else -(-x.shape[1] // 8) * 8
 
 
+def _extent(t: torch.Tensor) -> tuple[int, int, int, int]:
+    """(first byte, rows, bytes from row to row, bytes of a row) of a matrix with unit inner stride or a contiguous tensor."""
+    size = t.element_size()
+    if t.dim() != 2 or t.shape[0] <= 1 or t.is_contiguous():
+        return t.data_ptr(), 1, 0, t.numel() * size
+    return t.data_ptr(), t.shape[0], t.stride(0) * size, t.shape[1] * size
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the two share a byte.  Columns of the same rows do not; of interleaved rows of different strides this is not
+    looked into (they count as sharing)."""
+    if not a.numel() or not b.numel():
+        return False
+    (pa, ra, sa, wa), (pb, rb, sb, wb) = _extent(a), _extent(b)
+    if pa + (ra - 1) * sa + wa <= pb or pb + (rb - 1) * sb + wb <= pa:
+        return False
+    step = sa or sb
+    if not step or (ra > 1 and rb > 1 and sa != sb):
+        return True
+    d = (pb - pa) % step          # where b's rows begin between two of a's
+    return d < wa or d + wb > step
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -305,8 +328,8 @@ def grouped_linear(x: torch.Tensor, offsets: torch.Tensor, w: Q4, scales: torch.
     """Rows offsets[i] .. offsets[i + 1] - 1 of x (rows, K) times matrix i of w (experts, N, K), each expert with any number
     of rows, none among them; offsets int32 on the device, never falling, at most the rows of x (each is taken as at least
     its predecessors; ``check_errors`` reports one that is not).  Returns (rows, N); rows outside offsets[0] ..
-    offsets[-1] are zero, or, in an ``out`` that is given, left as they were.  Differentiable like ``linear``, without
-    ``out``."""
+    offsets[-1] are zero, or, in an ``out`` that is given, left as they were.  ``out`` may be columns of a larger matrix; it
+    shares no memory with what is read.  Differentiable like ``linear``, without ``out``."""
     _checked(x, w, offsets, "grouped_linear")
     if scales is not None:
         _trained(w, scales)
@@ -318,6 +341,9 @@ def grouped_linear(x: torch.Tensor, offsets: torch.Tensor, w: Q4, scales: torch.
         if out.dtype != x.dtype or out.shape != (x.shape[0], w.rows) or out.device != w.device or out.stride(1) != 1 or (
                 out.shape[0] > 1 and out.stride(0) < w.rows):
             raise ValueError(f"grouped_linear: out has to be {x.dtype} {(x.shape[0], w.rows)} with rows of unit stride")
+        x = _rows(x)
+        if any(_overlap(out, t) for t in (x, offsets, w.codes, w.scales, w.scale)):
+            raise ValueError("grouped_linear: out overlaps the activations, offsets or weights that are read")
     return _forward(_rows(x), w, offsets, out)
 
 
