@@ -118,6 +118,28 @@ def test_out_beside_what_is_read_is_taken():
     assert torch.equal(m.grouped_linear(half[::2], off, w, out=half[1::2]), want) and torch.equal(half[::2], x)
 
 
+def test_out_that_a_backward_pass_needs_is_noticed():
+    m = q4()
+    w, off = experts()
+    v = m.enc_q4(torch.randn(40, 64, generator=torch.Generator().manual_seed(3)), 32)
+    s = v.group_scales().requires_grad_()
+    buf = rows(700, 64, 3)
+    y = m.linear(buf, v, s)                                  # keeps buf for the gradient of s
+    m.grouped_linear(rows(700, 64, 4), off, w, out=buf)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), s)
+
+
+def test_out_that_wants_a_gradient_is_refused():
+    m = q4()
+    w, off = experts()
+    out = torch.zeros(700, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="gradient"):
+        m.grouped_linear(rows(700, 64, 5), off, w, out=out)
+    with torch.no_grad():
+        assert m.grouped_linear(rows(700, 64, 5), off, w, out=out) is out
+
+
 # ---- nothing to do ---------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("shape", [(64,), (3, 64), (2, 3, 64), (2, 0, 3, 64), (0, 64)])

@@ -341,9 +341,12 @@ def grouped_linear(x: torch.Tensor, offsets: torch.Tensor, w: Q4, scales: torch.
         if out.dtype != x.dtype or out.shape != (x.shape[0], w.rows) or out.device != w.device or out.stride(1) != 1 or (
                 out.shape[0] > 1 and out.stride(0) < w.rows):
             raise ValueError(f"grouped_linear: out has to be {x.dtype} {(x.shape[0], w.rows)} with rows of unit stride")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("grouped_linear: out wants a gradient, which is not passed through it")
         x = _rows(x)
         if any(_overlap(out, t) for t in (x, offsets, w.codes, w.scales, w.scale)):
             raise ValueError("grouped_linear: out overlaps the activations, offsets or weights that are read")
+        torch.autograd.graph.increment_version(out)   # a backward pass that needs what was there notices
     return _forward(_rows(x), w, offsets, out)
 
 
