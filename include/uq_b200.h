@@ -458,10 +458,15 @@ int uq_q4_embed_dscale(const void *tokens, int tokens64, int64_t T, const void *
                        const uint8_t *codes, int64_t V, int64_t K, int group, float alpha, float *dc,
                        void *workspace, size_t workspace_bytes, void *stream);
 
-/* Synchronises `stream` and reports (and clears) what the 4-bit operators met
- * since the last call: a bounded wait that gave up (UQ_ERR_TIMEOUT; outputs
- * are wrong), a token or an offset out of range (UQ_ERR_INVALID). */
+/* Synchronises `stream`, and takes and reports all that the 4-bit operators met
+ * on the device, on any stream, since the last call: a bounded wait that gave up
+ * (UQ_ERR_TIMEOUT; outputs are wrong), a token or an offset out of range
+ * (UQ_ERR_INVALID where no wait gave up). uq_last_error() names each. */
 int uq_q4_errors(void *stream);
+
+/* Launches the products' bounded wait on a barrier at which nothing arrives, with
+ * a limit of 50 ms: the next uq_q4_errors reports UQ_ERR_TIMEOUT. */
+int uq_q4_wait_selftest(void *stream);
 
 /* ---------------------------------------------------------------------
  * Device status (no counterpart in the reference)

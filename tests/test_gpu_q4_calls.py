@@ -152,3 +152,75 @@ def test_gradients_of_a_matrix_without_rows(shape):
     assert y.shape == (*shape[:-1], 0)
     dx, dc = torch.autograd.grad(y, (x, s), torch.ones_like(y))
     assert torch.equal(dx, torch.zeros_like(x)) and dc.shape == (0, 2)
+
+
+# ---- what check_errors tells -----------------------------------------------------------------------------------
+
+def test_every_error_is_named_once():
+    m = q4()
+    w, off = experts()
+    table = m.enc_q4(torch.randn(20, 64, generator=torch.Generator().manual_seed(1)), 32)
+    bad = torch.tensor([0, 400, 301, 700], dtype=torch.int32, device="cuda")
+    m.embedding(torch.tensor([25], device="cuda"), table)
+    m.grouped_linear(rows(700, 64, 1), bad, w)
+    with pytest.raises(ValueError) as e:
+        m.check_errors()
+    assert "token" in str(e.value) and "offsets" in str(e.value)
+    m.check_errors()
+
+
+def test_a_wait_that_gives_up_is_reported():
+    """The products' bounded wait on a barrier that nothing arrives at, with a limit of 50 ms: it ends, and the report
+    raises once, together with what else was met."""
+    from ultraquant_b200 import _lib
+    m, lib = q4(), _lib.load()
+    st = torch.cuda.current_stream().cuda_stream
+    assert lib.uq_q4_wait_selftest(st) == _lib.UQ_OK
+    with pytest.raises(_lib.UQError, match="timed out"):
+        m.check_errors()
+    m.check_errors()
+    table = m.enc_q4(torch.randn(20, 64, generator=torch.Generator().manual_seed(1)), 32)
+    assert lib.uq_q4_wait_selftest(st) == _lib.UQ_OK
+    m.embedding(torch.tensor([-1], device="cuda"), table)
+    with pytest.raises(_lib.UQError, match="timed out.*token"):
+        m.check_errors()
+    m.check_errors()
+
+
+def test_errors_are_read_on_their_own_stream():
+    """A side stream's check neither waits for another stream's work nor loses what that one meets later."""
+    m = q4()
+    table = m.enc_q4(torch.randn(20, 64, generator=torch.Generator().manual_seed(1)), 32)
+    tok = torch.tensor([99], device="cuda")
+    m.embedding(tok, table)                                  # loads what is launched below
+    with pytest.raises(ValueError, match="token"):
+        m.check_errors()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        torch.cuda._sleep(200_000_000)                       # some 0.1 s
+        m.embedding(tok, table)
+    with torch.cuda.stream(b):
+        m.check_errors()
+        assert not a.query(), "the check waited for another stream"
+    with torch.cuda.stream(a), pytest.raises(ValueError, match="token"):
+        m.check_errors()
+
+
+def test_profile_case_reports_a_product_that_gave_up(monkeypatch):
+    from ultraquant_b200 import _lib, profile_case
+    lib = _lib.load()
+    st = torch.cuda.current_stream().cuda_stream
+    real = profile_case.build_case
+
+    def build(args, lib_, stream):
+        run, units, unit = real(args, lib_, stream)
+
+        def with_wait():
+            run()
+            _lib.check(lib.uq_q4_wait_selftest(st), "selftest")
+        return with_wait, units, unit
+
+    monkeypatch.setattr(profile_case, "build_case", build)
+    with pytest.raises(_lib.UQError, match="timed out"):
+        profile_case.measure("q4few", rows=2, n=256, n0=128, iters=1)

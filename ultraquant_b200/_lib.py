@@ -95,6 +95,7 @@ SIGNATURES = {
     "uq_q4_embed_dscale_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
     "uq_q4_embed_dscale": (_i32, [_p, _i32, _i64, _p, _i32, _i64, _p, _i64, _i64, _i32, _f32, _p, _p, _sz, _p]),
     "uq_q4_errors": (_i32, [_p]),
+    "uq_q4_wait_selftest": (_i32, [_p]),
     "uq_device_errors": (_i32, [_p]),
     "uq_wait_timeout_selftest": (_i32, [_f64, _p]),
     "uq_inject_device_flag": (_i32, [_i32]),

@@ -543,6 +543,9 @@ __global__ void __launch_bounds__(256) q4_join_kernel(const uint32_t *keys, int6
     }
 }
 
+// In one step: see uq_q4mm.cu.
+__global__ void q4_take_token_flag_kernel(int *out) { *out = atomicExch(&g_q4_bad_token, 0); }
+
 int blocks_for(int64_t work, int per_sm) {
     return int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(uq::num_sms()) * per_sm)));
 }
@@ -746,15 +749,22 @@ int uq_q4_embed_dscale(const void *tokens, int tokens64, int64_t T, const void *
 }
 
 int uq_q4_errors(void *stream) {
-    if (cudaStreamSynchronize(UQ_STREAM(stream)) != cudaSuccess) return uq::check_cuda("uq_q4_errors");
-    int bad = 0, zero = 0, timeout = 0, offset = 0;
-    if (cudaMemcpyFromSymbol(&bad, g_q4_bad_token, sizeof(int)) != cudaSuccess || !mm_take_flags(&timeout, &offset))
-        return uq::check_cuda("read 4-bit operator flags");
-    if (bad && cudaMemcpyToSymbol(g_q4_bad_token, &zero, sizeof(int)) != cudaSuccess) return uq::check_cuda("clear 4-bit operator flags");
-    if (timeout) return uq::fail(UQ_ERR_TIMEOUT, "a bounded device wait of a 4-bit product timed out");
-    if (bad) return uq::fail(UQ_ERR_INVALID, "a token lies outside the table");
-    if (offset) return uq::fail(UQ_ERR_INVALID, "offsets fall, or go beyond the rows");
-    return UQ_OK;
+    const cudaStream_t st = UQ_STREAM(stream);
+    if (cudaStreamSynchronize(st) != cudaSuccess) return uq::check_cuda("uq_q4_errors");
+    int met[3] = {0, 0, 0}, *taken = nullptr;   // a wait that gave up, an offset, a token
+    if (cudaMallocAsync(&taken, sizeof(met), st) != cudaSuccess) return uq::check_cuda("uq_q4_errors");
+    mm_take_flags(taken, st);
+    { uq::ProfScope _p("q4_take_token_flag", st); q4_take_token_flag_kernel<<<1, 1, 0, st>>>(taken + 2); }
+    const int rc = uq::check_cuda("q4_take_flags_kernel launch");
+    const cudaError_t copied = cudaMemcpyAsync(met, taken, sizeof(met), cudaMemcpyDeviceToHost, st);
+    cudaFreeAsync(taken, st);
+    if (cudaStreamSynchronize(st) != cudaSuccess || copied != cudaSuccess) return uq::check_cuda("read 4-bit operator flags");
+    if (rc) return rc;
+    if (!met[0] && !met[1] && !met[2]) return UQ_OK;
+    return uq::fail(met[0] ? UQ_ERR_TIMEOUT : UQ_ERR_INVALID, "%s%s%s%s%s",
+                    met[0] ? "a bounded device wait of a 4-bit product timed out" : "", met[0] && (met[1] || met[2]) ? "; " : "",
+                    met[2] ? "a token lies outside the table" : "", met[2] && met[1] ? "; " : "",
+                    met[1] ? "offsets fall, or go beyond the rows" : "");
 }
 
 }  // extern "C"

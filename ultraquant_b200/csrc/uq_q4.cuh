@@ -16,8 +16,9 @@
 namespace uq {
 namespace q4 {
 
-// What the products met on the device since the last call (uq_q4mm.cu); false: CUDA error.
-bool mm_take_flags(int *timeout, int *offset);
+// Launches what writes to `out` (device) what the products met since the last call,
+// and clears it: [0] a wait that gave up, [1] an offset out of range (uq_q4mm.cu).
+void mm_take_flags(int *out, cudaStream_t st);
 inline bool group_ok(int g) { return g == 32 || g == 64 || g == 128 || g == 256; }
 inline bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

@@ -1380,6 +1380,28 @@ int dscale(const void *dy, const void *x, int64_t T, int64_t lddy, int64_t ldx, 
     return uq::check_cuda("q4_dscale_kernel launch");
 }
 
+// In one step, so that what a kernel on another stream meets meanwhile is either
+// told now or kept.
+__global__ void q4_take_flags_kernel(int *out) {
+    out[0] = atomicExch(&g_mm_timeout, 0);
+    out[1] = atomicExch(&g_mm_bad_offset, 0);
+}
+
+// The products' wait on a barrier at which nothing arrives, of two warps: the second
+// wait of each ends at once.
+__global__ void __launch_bounds__(64) q4_wait_selftest_kernel() {
+    __shared__ uint64_t bar;
+    __shared__ int gave_up;
+    if (threadIdx.x == 0) {
+        gave_up = 0;
+        tma::mbar_init(tc5::smem_addr(&bar), 1);
+    }
+    __syncthreads();
+    tc5::WaiterFor<50> wt{&gave_up, &g_mm_timeout};
+    wt.wait(tc5::smem_addr(&bar), 0);
+    wt.wait(tc5::smem_addr(&bar), 0);
+}
+
 // No matrix: every row is outside every run.
 int no_matrix(void *out, int64_t ld, int64_t T, int64_t J, bool zero, cudaStream_t st) {
     if (!zero || T == 0 || J == 0) return UQ_OK;
@@ -1397,17 +1419,19 @@ size_t product_workspace(int64_t T, int64_t mats, int64_t J, int64_t depth) {
 
 namespace uq {
 namespace q4 {
-bool mm_take_flags(int *timeout, int *offset) {
-    const int zero = 0;
-    return cudaMemcpyFromSymbol(offset, g_mm_bad_offset, sizeof(int)) == cudaSuccess &&
-           cudaMemcpyFromSymbol(timeout, g_mm_timeout, sizeof(int)) == cudaSuccess &&
-           (!*offset || cudaMemcpyToSymbol(g_mm_bad_offset, &zero, sizeof(int)) == cudaSuccess) &&
-           (!*timeout || cudaMemcpyToSymbol(g_mm_timeout, &zero, sizeof(int)) == cudaSuccess);
+void mm_take_flags(int *out, cudaStream_t st) {
+    uq::ProfScope _p("q4_take_flags", st);
+    q4_take_flags_kernel<<<1, 1, 0, st>>>(out);
 }
 }  // namespace q4
 }  // namespace uq
 
 extern "C" {
+
+int uq_q4_wait_selftest(void *stream) {
+    q4_wait_selftest_kernel<<<1, 64, 0, UQ_STREAM(stream)>>>();
+    return uq::check_cuda("q4_wait_selftest_kernel launch");
+}
 
 size_t uq_q4_linear_workspace_bytes(int64_t T, int64_t mats, int64_t N, int64_t K) {
     return T > 0 && mats == 1 && !few_rows(T, 1, false, N) ? product_workspace(T, mats, N, K) : 0;

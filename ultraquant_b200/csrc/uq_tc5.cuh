@@ -128,24 +128,24 @@ __device__ __forceinline__ void mbar_arrive_remote(unsigned cluster_addr) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(cluster_addr) : "memory");
 }
 
-// A block's waits, each by a whole warp and at most 2 s long: the first that
+// A block's waits, each by a whole warp and at most LIMIT_MS long: the first that
 // gives up sets *gave_up (shared memory), at which every other wait of the
 // block gives up too, and *flag (global memory), which the host reads.
-__device__ __noinline__ bool wait_slow(unsigned addr, unsigned parity, volatile int *gave_up, int *flag) {
+template <unsigned LIMIT_MS> __device__ __noinline__ bool wait_slow(unsigned addr, unsigned parity, volatile int *gave_up, int *flag) {
     unsigned long long t0, now;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
     for (;;) {
         for (int i = 0; i < 64; ++i)
             if (mbar_test(addr, parity)) return true;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
-        if (*gave_up || now - t0 > 2000000000ull) {
+        if (*gave_up || now - t0 > LIMIT_MS * 1000000ull) {
             *gave_up = 1;
             atomicExch(flag, 1);
             return false;
         }
     }
 }
-struct Waiter {
+template <unsigned LIMIT_MS> struct WaiterFor {
     volatile int *gave_up;
     int *flag;
     bool fail = false;
@@ -153,7 +153,7 @@ struct Waiter {
         if (fail) return false;
         bool ok = mbar_test(addr, parity);
         if (!__all_sync(0xffffffffu, ok)) {
-            if (!ok) ok = wait_slow(addr, parity, gave_up, flag);
+            if (!ok) ok = wait_slow<LIMIT_MS>(addr, parity, gave_up, flag);
             fail = !__all_sync(0xffffffffu, ok);
         }
         return !fail;
@@ -168,6 +168,7 @@ struct Waiter {
         } while (now - t0 < 2000000000ull);
     }
 };
+using Waiter = WaiterFor<2000>;
 
 #endif  // __CUDACC__
 

@@ -240,6 +240,7 @@ def measure(kernel: str, rows: int = 4096, n: int = 4096, n0: int = 0, L: int = 
     lib.uq_profile_enable(0)
     lib.uq_profile_reset()
     _lib.check(lib.uq_device_errors(st), kernel)
+    _lib.check(lib.uq_q4_errors(st), kernel)
     ms = tot.value / iters            # device time of the kernel per run (all its launches)
     rec["ms_per_run"] = ms
     if unit == "bytes":

@@ -145,8 +145,8 @@ def round_scales(w: Q4, scales: torch.Tensor) -> Q4:
 
 
 def check_errors(device=None) -> None:
-    """Waits for the current stream and raises what the operators' kernels have met since the last call: ValueError for a
-    token or an offset out of range, UQError for a wait that gave up."""
+    """Waits for the current stream and raises what the operators' kernels of the device have met since the last call:
+    UQError for a wait that gave up, else ValueError for a token or an offset out of range; the message names all."""
     dev = torch.device(device) if device is not None else D.device()
     _run(dev if dev.index is not None else D.device(), "uq_q4_errors")
 
