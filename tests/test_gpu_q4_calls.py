@@ -224,3 +224,40 @@ def test_profile_case_reports_a_product_that_gave_up(monkeypatch):
     monkeypatch.setattr(profile_case, "build_case", build)
     with pytest.raises(_lib.UQError, match="timed out"):
         profile_case.measure("q4few", rows=2, n=256, n0=128, iters=1)
+
+
+# ---- a frequent token ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,dt", [(1 << 20, torch.bfloat16), ((1 << 20) + 17, torch.float32)])
+def test_gradient_of_a_token_that_is_everywhere(T, dt):
+    """A padding token's gradient: T rows of odd whole numbers, whose sum passes 2^24 early.  Pieces of 32 rows are exact in
+    float32 and their sum is the 64-bit one rounded once, with no error that grows with T."""
+    m = q4()
+    w = constant((5, 64), 1, 1.0, 1.0)
+    w.codes.fill_(0x88)                                      # q = 0 but for the first element of each group
+    w.codes[:, 0] = 0x89
+    w.codes[:, 16] = 0x89
+    g = torch.Generator(device="cuda").manual_seed(T)
+    d = torch.zeros(T, 64, device="cuda", dtype=dt)
+    d[:, 0] = (torch.randint(0, 64, (T,), generator=g, device="cuda") * 2 + 65).to(dt)
+    d[:, 32] = (torch.randint(0, 64, (T,), generator=g, device="cuda") * 2 + 1).to(dt)
+    s = w.group_scales().requires_grad_()
+    tok = torch.full((T,), 3, device="cuda")
+    tok[5], tok[T // 2] = 1, 4
+    for alpha in (1.0, -0.3):
+        (dc,) = torch.autograd.grad(m.embedding(tok, w, alpha, s, dtype=dt), s, d)
+        here = tok == 3
+        want = torch.stack([d[here, 0].double().sum(), d[here, 32].double().sum()]) * torch.tensor(alpha, dtype=torch.float32, device="cuda").double()
+        assert want.abs().max() > 2 ** 24
+        assert torch.equal(dc[3], want.float()), (dc[3].double() / want - 1).tolist()
+        assert torch.equal(dc[1], (d[5, [0, 32]].double() * torch.tensor(alpha, dtype=torch.float32).item()).float())
+
+
+def test_gradient_of_a_frequent_token_keeps_infinities():
+    m = q4()
+    w = constant((5, 64), 1, 1.0, 1.0)
+    s = w.group_scales().requires_grad_()
+    d = torch.ones(500, 64, device="cuda", dtype=torch.bfloat16)
+    d[7, 0], d[300, 40] = float("inf"), float("nan")
+    (dc,) = torch.autograd.grad(m.embedding(torch.full((500,), 2, device="cuda"), w, 1.0, s), s, d)
+    assert dc[2, 0].item() == float("inf") and torch.isnan(dc[2, 1]) and not dc[[0, 1, 3, 4]].any()
