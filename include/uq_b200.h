@@ -394,8 +394,10 @@ int uq_q4_encode(const void *W, int w_dtype, int64_t mats, int64_t rows, int64_t
                  int group, uint8_t *codes, uint8_t *scales, float *scale, void *workspace,
                  size_t workspace_bytes, void *stream);
 
-/* out (mats, rows, cols) contiguous, UQ_F32, UQ_BF16 or UQ_F16: s e q, one
- * rounding (none to float32 while nothing underflows). */
+/* out (mats, rows, cols) contiguous, UQ_F32, UQ_BF16 or UQ_F16: s e q. With s a
+ * power of two (as the encoder leaves it) exact in float32 while nothing
+ * underflows, and rounded once to 16 bits; s e and its product with q round to
+ * float32 for any other s. */
 int uq_q4_decode(const uint8_t *codes, const uint8_t *scales, const float *scale, int64_t mats,
                  int64_t rows, int64_t cols, int group, void *out, int out_dtype, void *stream);
 
@@ -440,7 +442,8 @@ int uq_q4_linear_dscale(const void *dy, const void *x, int dtype, int64_t T, int
                         void *stream);
 
 /* out[t, :] = alpha w[tokens[t], :], (T, K) contiguous, UQ_F32, UQ_BF16 or
- * UQ_F16, one rounding after the float32 factor alpha s e.  tokens: int32, or
+ * UQ_F16: alpha s, its product with e and that with q each rounded to float32,
+ * then once to 16 bits.  tokens: int32, or
  * int64 when tokens64.  A token outside 0 .. V - 1 gives a row of NaN and is
  * reported by uq_q4_errors. */
 int uq_q4_embed(const void *tokens, int tokens64, int64_t T, const uint8_t *codes, const uint8_t *scales,
@@ -450,8 +453,9 @@ int uq_q4_embed(const void *tokens, int tokens64, int64_t T, const uint8_t *code
 /* Gradient of uq_q4_embed with respect to c = s e: dc[v, j] = alpha
  * sum_{t: tokens[t] = v} sum_{k in group j} q[v, k] dout[t, k], (V, K / group)
  * floats, written whole.  dout (T, K), row stride ld, UQ_F32, UQ_BF16 or
- * UQ_F16.  The rows of a token are added in the order of t, in fixed pieces:
- * the same call gives the same bits.  Tokens outside 0 .. V - 1 add nothing.
+ * UQ_F16.  The rows of a token are added in the order of t, in fixed pieces of
+ * 32 sorted rows whose sums are joined without loss: the same call gives the same
+ * bits, and the rounding does not grow with a token's rows.  Tokens outside 0 .. V - 1 add nothing.
  * T < 2^30. */
 size_t uq_q4_embed_dscale_workspace_bytes(int64_t T, int64_t V, int64_t K, int group);
 int uq_q4_embed_dscale(const void *tokens, int tokens64, int64_t T, const void *dout, int dtype, int64_t ld,

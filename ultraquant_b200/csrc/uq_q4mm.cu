@@ -375,9 +375,21 @@ template <typename T> __device__ void zero_rows(const Out &o, int64_t begin, int
 // rows are there (second); warp 19 brings each chunk's scales, an odd few bytes
 // from every row, which loaded by the widening warps a chunk ahead still cost 7 %
 // forward and 30 % of DX (4096 x 4096 x 14336: 460 us, 316 without any scales).
-// Bound by the tensor cores, except that a tile of less than 215 rows is widened no
-// sooner than one of 215.  Forward 2047 x 14336 x 4096 156 us, 1.54 PFLOP/s;
-// DX 4096 x 4096 x 14336 347 us, 1.39 PFLOP/s.
+// Bound by the tensor cores from about 215 rows a tile on (forward 2047 x 14336 x 4096
+// 156 us, 1.54 PFLOP/s; DX 4096 x 4096 x 14336 344 us, 1.40 PFLOP/s).  Below, a stage
+// takes some 430 cycles however few its rows, about three times what its bytes need, by
+// neither the widening's arithmetic nor the products but by the way of a chunk through
+// copies, barriers and the store of A.  28672 x 8192 in us, as it is / without the
+// arithmetic / without the products / without both: forward 32 rows 58 / 57 / 56 / 55,
+// 128 rows 67 / 65 / 63 / 61, 256 rows 93 / 92 / 65 / 71; DX 32 rows 62 / 61 / 61 / 60,
+// 256 rows 119 / 112 / 95 / 92.
+// The sums of a tile's whole contraction stay in the tensor core's float32
+// accumulator, unlike those of q4_dscale_kernel: the result is rounded to 16 bits, and
+// what sums of 14336 terms are off (some 6e-6 of the results' size: 0.16 % of them round
+// to the neighbour) is a 300th of that rounding.
+// 640 threads leave 96 registers each.  Spilled (bytes stored and loaded): nothing
+// forward without offsets, 112 and 220 by DX in bfloat16 and 256 rows, up to 264 and
+// 156 by the forms with offsets; up to 30 and 46 by write_tile.
 // ----------------------------------------------------------------------------
 constexpr int kWiden = 16, kThreads = (kWiden + 4) * 32;
 
@@ -678,8 +690,8 @@ q4_product_kernel(const __grid_constant__ CUtensorMap map_rows, const __grid_con
 // products straight from registers: the contraction order is free as long as both operands agree, so lane quarter q
 // takes 64 consecutive values of a row (two 16-byte pieces) where the instruction
 // says "columns 2 q, 2 q + 1, 2 q + 8, 2 q + 9".  Widening costs the same for 1 row
-// as for 8.  (With A in tensor memory a product of 16 steps takes 118 cycles
-// however few rows there are: 3 times the time that memory needs.)
+// as for 8.  (Through q4_product_kernel the codes pass at a third of memory's rate
+// however few rows there are.)
 // ----------------------------------------------------------------------------
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool bf16) {
     if (bf16)
@@ -940,7 +952,8 @@ __global__ void __launch_bounds__(256) q4_join_parts_kernel(Runs r, const float 
 // half); both operands come as lines of 64 columns, one line per row t, in stages
 // of 64 rows.  The sums of kPromote
 // stages are taken from tensor memory (two accumulators in turn), multiplied by
-// q and added in float32 registers, so that no long sum runs in the tensor core.
+// q and added in float32 registers: the result is float32, where what a longer sum
+// loses in the tensor core would show (5.4e-7 of the result at 4096 rows).
 // Warps 0 .. 7 reduce, warp 8 copies, warp 9 issues (first CTA), warp 10 clears the
 // rows behind the last one of a run (they are another matrix's, and may be NaN)
 // and tells the first CTA that the stage is there.  Bound by the tensor cores: 4096 x
@@ -1223,7 +1236,7 @@ struct Plan {
 // J result columns, `depth` contraction steps.  The tiles that do not fill a round
 // of all pairs are split along k, so that the last round is a short one.  The width
 // and the parts have the least estimated cycles: a stage of 64 steps takes 2 cycles a
-// row of the tile in the tensor cores and about 430 to be widened, a tile some 4500
+// row of the tile in the tensor cores and about 430 to pass the ring, a tile some 4500
 // for its start and end, and joining parts a launch (5700) and their way to memory
 // and back.  Measured: 2047 x 14336 x 4096 (448 tiles, 74 pairs) 156 us, 168 with the
 // last 4 tiles whole; 4096 x 4096 x 14336 (256 tiles) 294 against 334; 4096 x 4096 at

@@ -126,7 +126,8 @@ def enc_q4(W, group: int = 32) -> Q4:
 
 
 def deq_q4(w: Q4, dtype=torch.float32) -> torch.Tensor:
-    """The values: scale * scales * q, rounded once to ``dtype`` (float32 holds them exactly)."""
+    """The values: scale * scales * q.  With a power of two as ``scale`` (the encoder's) float32 holds them exactly and a
+    16-bit ``dtype`` rounds once; with any other the float32 products round as well."""
     if dtype not in _OUT:
         raise TypeError(f"deq_q4: dtype {dtype} is not built (float32, bfloat16, float16)")
     out = w.codes.new_empty(w.shape, dtype=dtype)
